@@ -3,9 +3,9 @@ C++ bench harnesses.
 
 Plain hipcc invocations: every `csrc/*.hip` file is compiled to an object in
 `_build/`, then linked into `lib/libfeatherops_amd.so` (no torch involved).
-`csrc/torch_op.cpp` (host C++ only) is compiled with g++ against torch's
+`csrc/torch_op*.cpp` (host C++ only) are compiled with g++ against torch's
 headers into `lib/libfeather_torch_ops.so`, which registers
-torch.ops.feather_ops.scaled_mm and links the library above.
+torch.ops.feather_ops and links the library above.
 The C++ benches in `cpp_benchmarks/` link against libfeatherops_amd.so
 (mirroring the reference's cpp_benchmarks/build_benchmark_scaled_mm_hip.sh,
 which links the kernel's extern "C" ABI directly).
@@ -87,21 +87,23 @@ def build_library(jobs: int = 8) -> Path:
 
 
 def build_torch_ops() -> Path:
-    """lib/libfeather_torch_ops.so from csrc/torch_op.cpp (needs libfeatherops_amd.so)."""
+    """lib/libfeather_torch_ops.so from csrc/torch_op*.cpp (needs libfeatherops_amd.so)."""
     import torch
     from torch.utils import cpp_extension
 
     rocm = os.environ.get("ROCM_PATH", "/opt/rocm")
     torch_lib = Path(torch.__file__).resolve().parent / "lib"
-    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall",
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-Wall",
            "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
-    cmd += [f"-I{p}" for p in cpp_extension.include_paths()]
-    cmd += [f"-I{rocm}/include", f"-I{INCLUDE}", str(CSRC / "torch_op.cpp"),
-            f"-L{torch_lib}", "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch",
-            f"-L{LIB_DIR}", "-lfeatherops_amd", "-Wl,-rpath,$ORIGIN"]
+    cmd += [f"-I{p}" for p in cpp_extension.include_paths()] + [f"-I{rocm}/include", f"-I{INCLUDE}"]
+    sources = sorted(CSRC.glob("torch_op*.cpp"))
+    objects = [BUILD_DIR / (s.stem + ".o") for s in sources]
+    with ThreadPoolExecutor(max_workers=len(sources)) as ex:
+        list(ex.map(lambda so: _run([*cmd, "-c", str(so[0]), "-o", str(so[1])]), zip(sources, objects)))
     tmp = OPS_LIB_PATH.with_suffix(".so.tmp")
-    _run([*cmd, "-o", str(tmp)])
+    _run([cmd[0], "-shared", *map(str, objects), f"-L{torch_lib}", "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch",
+          f"-L{LIB_DIR}", "-lfeatherops_amd", "-Wl,-rpath,$ORIGIN", "-o", str(tmp)])
     os.replace(tmp, OPS_LIB_PATH)
     return OPS_LIB_PATH
 

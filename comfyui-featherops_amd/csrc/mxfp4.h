@@ -1,0 +1,205 @@
+// MXFP4: 32 consecutive values of a row share one power of two, each held in 4
+// bits. The formats, their packed layout in HBM and the helpers that every
+// kernel of this family uses.
+//
+//   code   e2m1 [s:1][e:2][m:1]: 0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives;
+//          the earlier value of a pair in the low half of its byte
+//   scale  e8m0: byte b stands for 2^(b - 127), 255 for NaN
+//
+// A block of 32 values with largest magnitude amax takes the scale
+// 2^max(floor(log2 amax) - 2, -127) (so amax / scale is in [4, 8)) and the codes
+// nearest to v / scale, ties to the even code, 6 beyond 6. A NaN or an infinity
+// in the block makes it NaN as a whole (scale 255): a 4-bit code holds neither,
+// and a block scaled by infinity would turn its other values to zero unseen.
+//
+// Packed layout, the operand order of the block-scaled 16x16x128 MFMA, for R
+// rows and K columns, ksteps = ceil(K / 128), groups = ceil(R / 64):
+//   codes  [4 * groups][ksteps][64][16 bytes]: lane l of row tile t and step s
+//          holds row 16 t + l % 16, columns 128 s + 32 (l / 16) .. + 31
+//   scales [groups][ksteps][64][4]: byte f of lane l belongs to row tile
+//          4 g + f of that lane's row and block
+// so a wave's operand load is one contiguous KB and the scales of four row tiles
+// are one dword per lane, selected by the instruction. Columns beyond K are zero
+// codes under scale 2^-127; rows beyond R may hold anything (no row's result
+// depends on another row).
+#pragma once
+
+#include "feather_common.h"
+
+namespace feather {
+
+constexpr int kMxBlock = 32;
+constexpr int kMxStepK = 128;
+constexpr int kMxGroupRows = 64;
+
+__host__ __device__ inline int64_t mx_ksteps(int64_t cols) { return (cols + kMxStepK - 1) / kMxStepK; }
+__host__ __device__ inline int64_t mx_groups(int64_t rows) { return (rows + kMxGroupRows - 1) / kMxGroupRows; }
+
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+
+// The scale byte of a block whose largest magnitude is amax (not negative; any
+// NaN or infinity among the block's values arrives as one).
+__device__ __forceinline__ uint32_t mx_scale_byte(float amax) {
+    const uint32_t e = f32_bits(amax) >> 23;
+    return e == 255u ? 255u : (e > 2u ? e - 2u : 0u);
+}
+// The scale as the fp32 operand of the conversion instructions (2^-127 is a
+// subnormal, which they take; checked on gfx950 for every scale byte).
+__device__ __forceinline__ float mx_scale_f32(uint32_t byte) {
+    return bits_f32(byte == 0u ? 0x00400000u : byte << 23);
+}
+
+// The larger of |a| and |b| as bits: integer order is magnitude order, with
+// infinities and NaN above every finite value.
+__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2_t, a),
+                                                                  __builtin_bit_cast(u16x2_t, b)));
+}
+
+// 16 bytes at any 2-byte alignment (global memory takes unaligned 16-byte
+// accesses; an aligned one costs nothing extra).
+__device__ __forceinline__ uint4 load16_unaligned(const void* p) {
+    uint4 v;
+    __builtin_memcpy(&v, p, 16);
+    return v;
+}
+
+enum MxType { kMxF16 = 0, kMxBf16 = 1, kMxF32 = 2 };
+template <int T>
+constexpr int kMxElemBytes = T == kMxF32 ? 4 : 2;
+
+// One lane's 32 values as loaded: 4 dwords per uint4, 4 (16-bit) or 8 of them.
+template <int T>
+struct MxRaw {
+    static constexpr int kVecs = T == kMxF32 ? 8 : 4;
+    uint4 v[kVecs];
+
+    // values [0, n) from p, zeros beyond
+    __device__ __forceinline__ void load(const uint8_t* p, int n) {
+        if (n == kMxBlock) {
+#pragma unroll
+            for (int i = 0; i < kVecs; ++i) v[i] = load16_unaligned(p + 16 * i);
+        } else {
+            uint32_t w[kVecs * 4];
+#pragma unroll
+            for (int i = 0; i < kVecs * 4; ++i) {
+                if constexpr (T == kMxF32) {
+                    w[i] = i < n ? reinterpret_cast<const uint32_t*>(p)[i] : 0u;
+                } else {
+                    const uint16_t* q = reinterpret_cast<const uint16_t*>(p);
+                    w[i] = (2 * i < n ? static_cast<uint32_t>(q[2 * i]) : 0u) |
+                           (2 * i + 1 < n ? static_cast<uint32_t>(q[2 * i + 1]) << 16 : 0u);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < kVecs; ++i) v[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+        }
+    }
+
+    // the block's codes; *scale_byte gets its scale
+    __device__ __forceinline__ uint4 quantize(uint32_t* scale_byte) const {
+        uint32_t w[kVecs * 4];
+#pragma unroll
+        for (int i = 0; i < kVecs; ++i) {
+            w[4 * i] = v[i].x;
+            w[4 * i + 1] = v[i].y;
+            w[4 * i + 2] = v[i].z;
+            w[4 * i + 3] = v[i].w;
+        }
+        uint32_t o[4] = {0u, 0u, 0u, 0u};
+        float s;
+        if constexpr (T == kMxF32) {
+            uint32_t m = 0u;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) m = max(m, w[i] & 0x7fffffffu);
+            *scale_byte = mx_scale_byte(bits_f32(m));
+            s = mx_scale_f32(*scale_byte);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                o[i] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(o[i], bits_f32(w[8 * i]), bits_f32(w[8 * i + 1]), s, 0);
+                o[i] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(o[i], bits_f32(w[8 * i + 2]), bits_f32(w[8 * i + 3]), s, 1);
+                o[i] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(o[i], bits_f32(w[8 * i + 4]), bits_f32(w[8 * i + 5]), s, 2);
+                o[i] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(o[i], bits_f32(w[8 * i + 6]), bits_f32(w[8 * i + 7]), s, 3);
+            }
+        } else {
+            uint32_t m = 0u;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) m = max_u16x2(m, w[i] & 0x7fff7fffu);
+            const uint32_t m16 = max(m & 0xffffu, m >> 16);
+            *scale_byte = mx_scale_byte(T == kMxBf16 ? bits_f32(m16 << 16) : half_bits_to_f32(static_cast<uint16_t>(m16)));
+            s = mx_scale_f32(*scale_byte);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if constexpr (T == kMxBf16) {
+                    o[i] = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(o[i], __builtin_bit_cast(bf16x2_t, w[4 * i]), s, 0);
+                    o[i] = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(o[i], __builtin_bit_cast(bf16x2_t, w[4 * i + 1]), s, 1);
+                    o[i] = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(o[i], __builtin_bit_cast(bf16x2_t, w[4 * i + 2]), s, 2);
+                    o[i] = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(o[i], __builtin_bit_cast(bf16x2_t, w[4 * i + 3]), s, 3);
+                } else {
+                    o[i] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(o[i], __builtin_bit_cast(f16x2_t, w[4 * i]), s, 0);
+                    o[i] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(o[i], __builtin_bit_cast(f16x2_t, w[4 * i + 1]), s, 1);
+                    o[i] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(o[i], __builtin_bit_cast(f16x2_t, w[4 * i + 2]), s, 2);
+                    o[i] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(o[i], __builtin_bit_cast(f16x2_t, w[4 * i + 3]), s, 3);
+                }
+            }
+        }
+        return make_uint4(o[0], o[1], o[2], o[3]);
+    }
+};
+
+// D(16x16, fp32) += A(16x128) * B(128x16), both MXFP4. Lane l supplies row
+// (column) l % 16 and columns (rows) 32 (l / 16) .. + 31 as 16 bytes, and that
+// block's scale in byte kByteA (kByteB) of its scale register; it receives D rows
+// 4 (l / 16) .. + 3 of column l % 16. Checked against 64-bit sums on gfx950.
+template <int kByteA, int kByteB>
+__device__ __forceinline__ f32x4 mfma_mx(uint4 a, uint4 b, f32x4 c, uint32_t scale_a, uint32_t scale_b) {
+    const i32x8 a8 = {static_cast<int>(a.x), static_cast<int>(a.y), static_cast<int>(a.z), static_cast<int>(a.w), 0, 0, 0, 0};
+    const i32x8 b8 = {static_cast<int>(b.x), static_cast<int>(b.y), static_cast<int>(b.z), static_cast<int>(b.w), 0, 0, 0, 0};
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a8, b8, c, 4, 4, kByteA, static_cast<int>(scale_a), kByteB,
+                                                            static_cast<int>(scale_b));
+}
+
+// Host side launches (mxfp4_quant.hip, mxfp4_mm.hip, mxfp4_rows.hip); sizes are
+// checked by the C entries.
+int mx_quantize(const void* x, int dtype, int64_t rows, int64_t cols, int64_t row_stride, uint8_t* codes,
+                uint8_t* scales, hipStream_t stream);
+int mx_dequantize(const uint8_t* codes, const uint8_t* scales, void* out, int dtype, int64_t rows, int64_t cols,
+                  hipStream_t stream);
+int mx_prepack(const uint8_t* codes_rows, const uint8_t* scales_rows, uint8_t* codes, uint8_t* scales, int64_t rows,
+               int64_t cols, hipStream_t stream);
+int mx_unprepack(const uint8_t* codes, const uint8_t* scales, uint8_t* codes_rows, uint8_t* scales_rows, int64_t rows,
+                 int64_t cols, hipStream_t stream);
+
+// Operands of a product C (M, N) = A (M, K) . B (N, K)^T + bias.
+struct MxMmArgs {
+    const uint8_t* a;         // packed codes (a_type kMxPacked) or row-major 16-bit values
+    const uint8_t* a_scales;  // packed scales, unused for 16-bit activations
+    int a_type;               // kMxF16, kMxBf16 or kMxPacked
+    int64_t a_stride;         // elements between rows of 16-bit activations
+    const uint8_t* b;
+    const uint8_t* b_scales;
+    const uint16_t* bias;  // output type, or null
+    uint16_t* c;
+    int64_t M;
+    int N, K;
+    int out_bf16;
+    uint8_t* ws;  // arrival counters, then fp32 partial sums
+    size_t ws_bytes;
+};
+constexpr int kMxPacked = 3;
+constexpr size_t kMxCounterBytes = 65536;
+
+// What a product's call runs: few-row kernel (tile 0) or an LDS tile, and its K split.
+struct MxPlan {
+    int tile;
+    int ksplit;
+    size_t ws_bytes;
+};
+MxPlan mx_rows_plan(int64_t M, int64_t N, int64_t K);
+MxPlan mx_tile_plan(int64_t M, int64_t N, int64_t K);
+bool mx_takes_rows(int64_t M, int64_t N, int64_t K, int a_type);
+int mx_mm_rows(const MxMmArgs& p, hipStream_t stream);
+int mx_mm_tiles(const MxMmArgs& p, hipStream_t stream);
+
+}  // namespace feather

@@ -1,0 +1,313 @@
+// C (M, N) = A (M, K) . B (N, K)^T + bias with both operands packed MXFP4
+// (mxfp4.h), on the block-scaled 16x16x128 MFMA with fp32 accumulators.
+#include <algorithm>
+
+#include "featherops_amd.h"
+#include "lds_dma.h"
+#include "mxfp4.h"
+
+namespace feather {
+namespace {
+
+template <int... I, class F>
+__device__ __forceinline__ void unrolled_impl(std::integer_sequence<int, I...>, F&& f) {
+    (f(std::integral_constant<int, I>{}), ...);
+}
+// f(0_c) .. f(n-1_c): indices as constants, which the MFMA's scale selectors need.
+template <int N, class F>
+__device__ __forceinline__ void unrolled(F&& f) {
+    unrolled_impl(std::make_integer_sequence<int, N>{}, f);
+}
+
+// 4 bytes per lane from sbase + voff into LDS at lds_addr + 4 * lane (dma16_lds for dwords).
+__device__ __forceinline__ void dma4_lds(const void* sbase, uint32_t voff, uint32_t lds_addr) {
+    asm volatile(
+        "s_nop 0\n\t"
+        "global_load_lds_dword %0, %1"
+        :
+        : "v"(voff), "s"(sbase), "{m0}"(lds_addr)
+        : "memory");
+}
+
+struct TileArgs {
+    const uint8_t* a;
+    const uint8_t* as;
+    const uint8_t* b;
+    const uint8_t* bs;
+    const uint16_t* bias;
+    uint16_t* c;
+    int64_t M;
+    int N, ksteps, a_groups, b_groups;
+    int tiles_m, tiles_n, ksplit, group_m;
+    uint32_t* counters;
+    float* partials;
+};
+
+// One workgroup computes a BM x BN tile of C over its share of the K steps with
+// WM x WN waves. The weights take the MFMA's first operand, so a lane ends with
+// four consecutive columns of one row of C and stores them together.
+//
+// Per K step the tile's operands (BM + BN rows of 64 bytes, and a dword of scales
+// per lane and 64 rows) are copied from HBM into a ring of kStages LDS buffers; a
+// fragment is one contiguous KB in HBM, in LDS and in the wave's ds_read_b128, so
+// there is no swizzle and no bank conflict. Every iteration waits for the stage
+// after the one it multiplies, issues the copies of the stage kStages ahead into the
+// buffer it has emptied, and reads the next stage's fragments into the other half
+// of its fragment registers under this stage's MFMAs. Copies past the last step
+// repeat it, so the wait counts are constants.
+template <int BM, int BN, int WM, int WN, int kStages, bool kBf16>
+__global__ __launch_bounds__(64 * WM * WN, WM * WN == 4 ? 1 : 2) void mx_tile_kernel(const TileArgs p) {
+    constexpr int kWaves = WM * WN;
+    constexpr int TM = BM / WM, TN = BN / WN;  // wave tile
+    constexpr int FM = TM / 16, FN = TN / 16;  // its fragments
+    constexpr int kGroupsM = BM / 64, kGroupsN = BN / 64;
+    constexpr int kCodeCopies = (BM + BN) / 16, kScaleCopies = kGroupsM + kGroupsN;
+    constexpr int kCodes = (kCodeCopies + kWaves - 1) / kWaves, kScales = (kScaleCopies + kWaves - 1) / kWaves;
+    constexpr int kPerWave = kCodes + kScales;  // copies of a stage by every wave (surplus ones repeat the last)
+    constexpr int kStageBytes = kCodeCopies * 1024 + kScaleCopies * 256;
+    constexpr int kScaleBase = kCodeCopies * 1024;
+    constexpr int SM = (FM + 3) / 4, SN = (FN + 3) / 4;  // scale dwords of the wave's rows and columns
+    static_assert(kStages * kStageBytes <= 160 * 1024, "LDS");
+    static_assert((kStages - 1) * kPerWave < 64, "vmcnt range");
+    static_assert(FM % 2 == 0 && FN % 2 == 0 && (FM % 4 == 0 || FM == 2) && (FN % 4 == 0 || FN == 2), "scale bytes");
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[kStages * kStageBytes];
+
+    const int tid = threadIdx.x;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int lane = tid & 63;
+    const int wm = wave / WN, wn = wave % WN;
+
+    // Workgroup -> tile: an XCD's workgroups (p % 8) take a contiguous run of the raster, which walks
+    // group_m tile rows at a time, so an XCD's L2 holds few rows and columns of tiles at once.
+    const int total = p.tiles_m * p.tiles_n * p.ksplit;
+    const int xcd = blockIdx.x % kNumXcd;
+    const int run = total / kNumXcd, more = total % kNumXcd;
+    const int t = xcd * run + min(xcd, more) + blockIdx.x / kNumXcd;
+    const int q = t % p.ksplit;
+    const int lin = t / p.ksplit;
+    const int per_group = p.group_m * p.tiles_n;
+    const int first_m = lin / per_group * p.group_m;
+    const int rows_here = min(p.group_m, p.tiles_m - first_m);
+    const int tm = first_m + lin % per_group % rows_here;
+    const int tn = lin % per_group / rows_here;
+    const int64_t m0 = static_cast<int64_t>(tm) * BM;
+    const int n0 = tn * BN;
+    const int k0 = static_cast<int>(static_cast<int64_t>(p.ksteps) * q / p.ksplit);
+    const int steps = static_cast<int>(static_cast<int64_t>(p.ksteps) * (q + 1) / p.ksplit) - k0;
+
+    // This wave's copies: their addresses at step k0. Groups of 64 rows past an operand's end read its last one.
+    const uint8_t* src[kPerWave];
+    uint32_t dst[kPerWave];
+    const uint32_t lds = lds_addr_of(smem);
+#pragma unroll
+    for (int i = 0; i < kCodes; ++i) {
+        const int j = min(i * kWaves + wave, kCodeCopies - 1);
+        const bool is_a = j < BM / 16;
+        const int f = is_a ? j : j - BM / 16;
+        const int64_t g = is_a ? min(static_cast<int>(m0 / 64) + f / 4, p.a_groups - 1) : min(n0 / 64 + f / 4, p.b_groups - 1);
+        src[i] = (is_a ? p.a : p.b) + ((g * 4 + f % 4) * p.ksteps + k0) * 1024;
+        dst[i] = lds + j * 1024;
+    }
+#pragma unroll
+    for (int i = 0; i < kScales; ++i) {
+        const int j = min(i * kWaves + wave, kScaleCopies - 1);
+        const bool is_a = j < kGroupsM;
+        const int64_t g = is_a ? min(static_cast<int>(m0 / 64) + j, p.a_groups - 1) : min(n0 / 64 + j - kGroupsM, p.b_groups - 1);
+        src[kCodes + i] = (is_a ? p.as : p.bs) + (g * p.ksteps + k0) * 256;
+        dst[kCodes + i] = lds + kScaleBase + j * 256;
+    }
+    auto issue = [&](int step, int slot) {
+        const int s = min(step, steps - 1);
+#pragma unroll
+        for (int i = 0; i < kCodes; ++i) dma16_lds(src[i] + static_cast<int64_t>(s) * 1024, lane * 16, dst[i] + slot * kStageBytes);
+#pragma unroll
+        for (int i = kCodes; i < kPerWave; ++i) dma4_lds(src[i] + static_cast<int64_t>(s) * 256, lane * 4, dst[i] + slot * kStageBytes);
+    };
+
+    struct Frags {
+        uint4 a[FM], b[FN];
+        uint32_t sa[SM], sb[SN];
+    };
+    auto read = [&](Frags& f, int slot) {
+        const uint8_t* base = smem + slot * kStageBytes;
+#pragma unroll
+        for (int i = 0; i < FN; ++i) f.b[i] = *reinterpret_cast<const uint4*>(base + (BM / 16 + wn * FN + i) * 1024 + lane * 16);
+#pragma unroll
+        for (int i = 0; i < FM; ++i) f.a[i] = *reinterpret_cast<const uint4*>(base + (wm * FM + i) * 1024 + lane * 16);
+#pragma unroll
+        for (int i = 0; i < SN; ++i) {
+            f.sb[i] = *reinterpret_cast<const uint32_t*>(base + kScaleBase + (kGroupsM + wn * TN / 64 + i) * 256 + lane * 4);
+            if constexpr (FN == 2) f.sb[i] >>= 16 * (wn % 2);
+        }
+#pragma unroll
+        for (int i = 0; i < SM; ++i) {
+            f.sa[i] = *reinterpret_cast<const uint32_t*>(base + kScaleBase + (wm * TM / 64 + i) * 256 + lane * 4);
+            if constexpr (FM == 2) f.sa[i] >>= 16 * (wm % 2);
+        }
+    };
+
+    f32x4 acc[FM][FN];
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    auto multiply = [&](const Frags& f) {
+        unrolled<FM>([&](auto i) {
+            unrolled<FN>([&](auto j) {
+                acc[i][j] = mfma_mx<j % 4, i % 4>(f.b[j], f.a[i], acc[i][j], f.sb[j / 4], f.sa[i / 4]);
+            });
+        });
+    };
+
+#pragma unroll
+    for (int s = 0; s < kStages; ++s) issue(s, s);
+    Frags f0, f1;
+    wait_vmcnt<(kStages - 1) * kPerWave>();
+    stage_barrier();
+    read(f0, 0);
+    int slot = 0;  // of the step being multiplied
+    auto iterate = [&](int k, Frags& now, Frags& next) {
+        const int after = slot + 1 == kStages ? 0 : slot + 1;
+        // stage k + 1 has landed; this wave's reads of stage k are done
+        wait_vmcnt_lgkm0<(kStages - 2) * kPerWave>();
+        stage_barrier();
+        issue(k + kStages, slot);
+        read(next, after);
+        multiply(now);
+        slot = after;
+    };
+    int k = 0;
+    for (; k + 1 < steps; k += 2) {
+        iterate(k, f0, f1);
+        iterate(k + 1, f1, f0);
+    }
+    if (k < steps) multiply(f0);
+    wait_vmcnt<0>();
+
+    const int lm = lane & 15;
+    const int ln = (lane >> 4) * 4;
+    if (p.ksplit > 1) {
+        // Each split writes its fp32 accumulators to the workspace in fragment order and counts itself
+        // in; the last to arrive adds the splits' sums in split order and goes on to the epilogue.
+        // Ordering: the partials are written and read with agent-scope (sc1) accesses alone, which
+        // are coherent across the XCDs. A store is acknowledged (vmcnt) once it is visible at agent
+        // scope; every wave waits for that before the barrier that precedes the arrival count, and
+        // the last arrival's loads depend on the count's answer.
+        constexpr int kTileBytes = BM * BN * 4;
+        constexpr int kCoherent = 16;  // sc1
+        typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+        const __amdgpu_buffer_rsrc_t prs = __builtin_amdgcn_make_buffer_rsrc(
+            p.partials + static_cast<int64_t>(lin) * p.ksplit * (kTileBytes / 4), 0, p.ksplit * kTileBytes, 0x00020000);
+        auto at = [&](int i, int j) { return (((wave * FM + i) * FN + j) * 64 + lane) * 16; };
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+#pragma unroll
+            for (int j = 0; j < FN; ++j)
+                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, acc[i][j]), prs, q * kTileBytes + at(i, j), 0, kCoherent);
+        __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+        __shared__ int last_flag;
+        __syncthreads();
+        if (tid == 0)
+            last_flag = __hip_atomic_fetch_add(&p.counters[lin], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
+                        static_cast<uint32_t>(p.ksplit - 1);
+        __syncthreads();
+        if (!last_flag) return;
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+#pragma unroll
+            for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int s = 0; s < p.ksplit; ++s) {
+#pragma unroll
+            for (int i = 0; i < FM; ++i)
+#pragma unroll
+                for (int j = 0; j < FN; ++j)
+                    acc[i][j] += __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(prs, s * kTileBytes + at(i, j), 0, kCoherent));
+        }
+        if (tid == 0)  // ready for the next call on this stream
+            __hip_atomic_store(&p.counters[lin], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+
+    // epilogue: bias added in fp32, one rounding to the output type
+    unrolled<FN>([&](auto j) {
+        const int n = n0 + wn * TN + j * 16 + ln;
+        if (n >= p.N) return;
+        const int have = min(4, p.N - n);
+        float bias[4] = {0.f, 0.f, 0.f, 0.f};
+        if (p.bias) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (e < have) bias[e] = out_bits_to_f32<kBf16>(p.bias[n + e]);
+        }
+        unrolled<FM>([&](auto i) {
+            const int64_t m = m0 + wm * TM + i * 16 + lm;
+            if (m >= p.M) return;
+            const f32x4 v = acc[i][j];
+            const uint32_t o[2] = {f32x2_to_out_bits<kBf16>(v[0] + bias[0], v[1] + bias[1]),
+                                   f32x2_to_out_bits<kBf16>(v[2] + bias[2], v[3] + bias[3])};
+            uint16_t* c = p.c + m * p.N + n;
+            if (have == 4) {
+                __builtin_memcpy(c, o, 8);
+            } else {
+                for (int e = 0; e < have; ++e) c[e] = static_cast<uint16_t>(o[e >> 1] >> (16 * (e & 1)));
+            }
+        });
+    });
+}
+
+struct Tile {
+    int bm, bn;
+};
+// ids 1.. of the plan
+constexpr Tile kTiles[] = {{0, 0}, {64, 64}, {64, 128}, {128, 128}, {256, 256}};
+
+int tile_env() {
+    static const int v = [] {
+        const char* e = getenv("FEATHEROPS_MX_TILE");
+        return e ? atoi(e) : 0;
+    }();
+    return v;
+}
+
+template <int BM, int BN, int WM, int WN, int kStages>
+void launch(const TileArgs& a, bool bf16, hipStream_t stream) {
+    const unsigned grid = static_cast<unsigned>(a.tiles_m * a.tiles_n * a.ksplit);
+    if (bf16) mx_tile_kernel<BM, BN, WM, WN, kStages, true><<<grid, 64 * WM * WN, 0, stream>>>(a);
+    else mx_tile_kernel<BM, BN, WM, WN, kStages, false><<<grid, 64 * WM * WN, 0, stream>>>(a);
+}
+
+}  // namespace
+
+MxPlan mx_tile_plan(int64_t M, int64_t N, int64_t K) {
+    const int64_t ksteps = mx_ksteps(K);
+    int tile = 4;
+    auto count = [&](int t) { return ((M + kTiles[t].bm - 1) / kTiles[t].bm) * ((N + kTiles[t].bn - 1) / kTiles[t].bn); };
+    while (tile > 1 && count(tile) < 200) --tile;
+    if (tile_env()) tile = tile_env();
+    int ksplit = 1;
+    const int64_t tiles = count(tile);
+    if (tiles < 128) ksplit = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(256 / tiles, ksteps / 4)));
+    size_t ws = 0;
+    if (ksplit > 1) ws = kMxCounterBytes + static_cast<size_t>(tiles) * ksplit * kTiles[tile].bm * kTiles[tile].bn * 4;
+    return {tile, ksplit, ws};
+}
+
+int mx_mm_tiles(const MxMmArgs& p, hipStream_t stream) {
+    MxPlan plan = mx_tile_plan(p.M, p.N, p.K);
+    if (plan.ws_bytes > p.ws_bytes) plan.ksplit = 1;
+    const Tile t = kTiles[plan.tile];
+    const int64_t tiles_m = (p.M + t.bm - 1) / t.bm, tiles_n = (p.N + t.bn - 1) / t.bn;
+    if (tiles_m * tiles_n * plan.ksplit > (int64_t(1) << 22)) return FEATHER_ERR_UNSUPPORTED;
+    const TileArgs a{p.a, p.a_scales, p.b, p.b_scales, p.bias, p.c, p.M, p.N, static_cast<int>(mx_ksteps(p.K)),
+                     static_cast<int>(mx_groups(p.M)), static_cast<int>(mx_groups(p.N)), static_cast<int>(tiles_m),
+                     static_cast<int>(tiles_n), plan.ksplit, 4, reinterpret_cast<uint32_t*>(p.ws),
+                     reinterpret_cast<float*>(p.ws + kMxCounterBytes)};
+    switch (plan.tile) {
+        case 1: launch<64, 64, 2, 2, 6>(a, p.out_bf16, stream); break;
+        case 2: launch<64, 128, 2, 2, 6>(a, p.out_bf16, stream); break;
+        case 3: launch<128, 128, 2, 2, 5>(a, p.out_bf16, stream); break;
+        default: launch<256, 256, 4, 2, 4>(a, p.out_bf16, stream); break;
+    }
+    return hipGetLastError() == hipSuccess ? FEATHER_OK : FEATHER_ERR_LAUNCH;
+}
+
+}  // namespace feather

@@ -1,0 +1,440 @@
+// torch ops of the MXFP4 operators and the block norms over the C ABI (no
+// counterpart in the reference):
+//   feather_ops::quantize_mxfp4, dequantize_mxfp4, prepack_mxfp4, unprepack_mxfp4
+//   feather_ops::mxfp4_mm          16-bit activations, quantised in the call
+//   feather_ops::mxfp4_mm_packed   activations that are packed MXFP4 already
+//   feather_ops::modulated_norm(_mxfp4), gated_residual_norm(_mxfp4)
+// Arguments are checked before anything is launched; launches go to torch's current
+// stream of the first tensor's device. Views whose rows have one stride are read in
+// place, others are made contiguous first.
+#include <ATen/ATen.h>
+#include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPStream.h>
+#include <torch/library.h>
+
+#include <cstdint>
+#include <tuple>
+
+#include "featherops_amd.h"
+#include "torch_workspace.h"
+
+namespace {
+
+using OptTensor = std::optional<at::Tensor>;
+
+hipStream_t stream_of(const at::Tensor& t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
+
+void check_status(int st, const char* what) {
+    TORCH_CHECK(st == FEATHER_OK, what, " failed: ", feather_status_string(st), " (status ", st, ")");
+}
+
+int value_code(at::ScalarType t, const char* what) {
+    switch (t) {
+        case at::kHalf: return FEATHER_DTYPE_F16;
+        case at::kBFloat16: return FEATHER_DTYPE_BF16;
+        case at::kFloat: return FEATHER_DTYPE_F32;
+        default: TORCH_CHECK(false, what, " must be float16, bfloat16 or float32, got ", t);
+    }
+    return -1;
+}
+
+// t as (rows, cols) with contiguous rows, one stride between them; a view where t allows one.
+at::Tensor as_rows(const at::Tensor& t) {
+    const int64_t cols = t.size(-1);
+    at::Tensor r = t.dim() == 2 ? t : t.reshape({cols ? t.numel() / cols : 0, cols});
+    if ((cols > 1 && r.stride(1) != 1) || (r.size(0) > 1 && r.stride(0) < 0)) r = r.contiguous();
+    return r;
+}
+
+struct Packed {
+    at::Tensor codes, scales;
+};
+
+Packed empty_packed(int64_t rows, int64_t cols, const at::Tensor& like) {
+    const int64_t groups = (rows + 63) / 64, steps = (cols + 127) / 128;
+    const auto options = like.options().dtype(at::kByte);
+    return {at::empty({groups * 4, steps, 64, 16}, options), at::empty({groups, steps, 64, 4}, options)};
+}
+
+// The packed form's shapes (see featherops_amd.h): messages name the operand.
+void check_packed(const at::Tensor& codes, const at::Tensor& scales, int64_t rows, int64_t cols, const char* what) {
+    TORCH_CHECK(codes.is_cuda() && scales.is_cuda(), what, " must be CUDA tensors");
+    TORCH_CHECK(codes.device() == scales.device(), what, " codes and scales must be on the same device");
+    TORCH_CHECK(codes.scalar_type() == at::kByte && scales.scalar_type() == at::kByte, what, " must be uint8");
+    const int64_t groups = (rows + 63) / 64, steps = (cols + 127) / 128;
+    TORCH_CHECK(codes.dim() == 4 && codes.size(0) == groups * 4 && codes.size(1) == steps && codes.size(2) == 64 &&
+                    codes.size(3) == 16 && scales.dim() == 4 && scales.size(0) == groups && scales.size(1) == steps &&
+                    scales.size(2) == 64 && scales.size(3) == 4,
+                what, " must be packed for (", rows, ", ", cols, "): codes (", groups * 4, ", ", steps,
+                ", 64, 16), scales (", groups, ", ", steps, ", 64, 4)");
+    TORCH_CHECK(codes.is_contiguous() && scales.is_contiguous(), what, " must be contiguous");
+    TORCH_CHECK(reinterpret_cast<uintptr_t>(codes.data_ptr()) % 16 == 0 &&
+                    reinterpret_cast<uintptr_t>(scales.data_ptr()) % 16 == 0,
+                what, " data pointers must be 16-byte aligned");
+}
+
+const uint8_t* bytes(const at::Tensor& t) { return static_cast<const uint8_t*>(t.data_ptr()); }
+uint8_t* bytes_out(const at::Tensor& t) { return static_cast<uint8_t*>(t.data_ptr()); }
+
+std::tuple<at::Tensor, at::Tensor> quantize_mxfp4(const at::Tensor& x) {
+    TORCH_CHECK(x.is_cuda(), "x must be a CUDA tensor");
+    TORCH_CHECK(x.dim() >= 1 && x.size(-1) >= 1, "x must have at least one column");
+    const int code = value_code(x.scalar_type(), "x");
+    const c10::DeviceGuard guard(x.device());
+    const at::Tensor r = as_rows(x);
+    const int64_t rows = r.size(0), cols = r.size(1);
+    const Packed q = empty_packed(rows, cols, x);
+    check_status(feather_mxfp4_quantize(r.data_ptr(), code, rows, cols, r.stride(0), bytes_out(q.codes),
+                                        bytes_out(q.scales), stream_of(x)),
+                 "quantize_mxfp4");
+    return {q.codes, q.scales};
+}
+
+at::Tensor dequantize_mxfp4(const at::Tensor& codes, const at::Tensor& scales, int64_t rows, int64_t cols,
+                            at::ScalarType dtype) {
+    TORCH_CHECK(rows >= 0 && cols >= 1, "rows must not be negative, cols must be positive");
+    check_packed(codes, scales, rows, cols, "q");
+    const int code = value_code(dtype, "dtype");
+    const c10::DeviceGuard guard(codes.device());
+    const at::Tensor out = at::empty({rows, cols}, codes.options().dtype(dtype));
+    check_status(feather_mxfp4_dequantize(bytes(codes), bytes(scales), out.data_ptr(), code, rows, cols, stream_of(codes)),
+                 "dequantize_mxfp4");
+    return out;
+}
+
+std::tuple<at::Tensor, at::Tensor> prepack_mxfp4(const at::Tensor& codes, const at::Tensor& scales, int64_t cols) {
+    TORCH_CHECK(codes.is_cuda() && scales.is_cuda(), "codes and scales must be CUDA tensors");
+    TORCH_CHECK(codes.device() == scales.device(), "codes and scales must be on the same device");
+    TORCH_CHECK(codes.element_size() == 1 && scales.element_size() == 1, "codes and scales must be 1-byte types");
+    const int64_t blocks = (cols + 31) / 32;
+    TORCH_CHECK(cols >= 1 && codes.dim() == 2 && scales.dim() == 2 && codes.size(0) == scales.size(0) &&
+                    codes.size(1) == blocks * 16 && scales.size(1) == blocks,
+                "codes must be (rows, ", blocks * 16, ") and scales (rows, ", blocks, ") for ", cols, " columns");
+    const c10::DeviceGuard guard(codes.device());
+    const at::Tensor c = codes.contiguous(), s = scales.contiguous();
+    const int64_t rows = c.size(0);
+    const auto options = codes.options().dtype(at::kByte);
+    const Packed q = empty_packed(rows, cols, at::empty({0}, options));
+    check_status(feather_mxfp4_prepack(bytes(c), bytes(s), bytes_out(q.codes), bytes_out(q.scales), rows, cols, stream_of(c)),
+                 "prepack_mxfp4");
+    return {q.codes, q.scales};
+}
+
+std::tuple<at::Tensor, at::Tensor> unprepack_mxfp4(const at::Tensor& codes, const at::Tensor& scales, int64_t rows,
+                                                   int64_t cols) {
+    TORCH_CHECK(rows >= 0 && cols >= 1, "rows must not be negative, cols must be positive");
+    check_packed(codes, scales, rows, cols, "q");
+    const c10::DeviceGuard guard(codes.device());
+    const int64_t blocks = (cols + 31) / 32;
+    const at::Tensor c = at::empty({rows, blocks * 16}, codes.options()), s = at::empty({rows, blocks}, codes.options());
+    check_status(feather_mxfp4_unprepack(bytes(codes), bytes(scales), bytes_out(c), bytes_out(s), rows, cols, stream_of(codes)),
+                 "unprepack_mxfp4");
+    return {c, s};
+}
+
+void check_mm_out(const OptTensor& bias, const at::Device& dev, int64_t N, at::ScalarType out_dtype) {
+    TORCH_CHECK(out_dtype == at::kHalf || out_dtype == at::kBFloat16, "out_dtype must be float16 or bfloat16");
+    if (bias.has_value()) {
+        TORCH_CHECK(bias->device() == dev, "bias must be on the same device as a");
+        TORCH_CHECK(bias->scalar_type() == out_dtype, "bias must have the output's dtype");
+        TORCH_CHECK(bias->dim() == 1 && bias->size(0) == N && (N == 1 || bias->stride(0) == 1),
+                    "bias must be contiguous with N (", N, ") elements");
+    }
+}
+
+at::Tensor run_mm(const void* a, const uint8_t* a_scales, int a_dtype, int64_t a_stride, const at::Tensor& b_codes,
+                  const at::Tensor& b_scales, const OptTensor& bias, int64_t M, int64_t N, int64_t K,
+                  at::ScalarType out_dtype) {
+    const hipStream_t stream = stream_of(b_codes);
+    const at::Tensor c = at::empty({M, N}, b_codes.options().dtype(out_dtype));
+    const size_t ws_bytes = feather_mxfp4_mm_workspace_size(M, N, K, a_dtype);
+    at::Tensor ws;
+    if (ws_bytes) ws = feather::workspace_for(b_codes.device(), stream, ws_bytes);
+    check_status(feather_mxfp4_mm(a, a_scales, a_dtype, a_stride, bytes(b_codes), bytes(b_scales),
+                                  bias.has_value() ? static_cast<const uint16_t*>(bias->data_ptr()) : nullptr,
+                                  static_cast<uint16_t*>(c.data_ptr()), M, N, K,
+                                  out_dtype == at::kBFloat16 ? FEATHER_DTYPE_BF16 : FEATHER_DTYPE_F16,
+                                  ws_bytes ? ws.data_ptr() : nullptr, ws_bytes ? static_cast<size_t>(ws.numel()) : 0, stream),
+                 "mxfp4_mm");
+    return c;
+}
+
+at::Tensor mxfp4_mm(const at::Tensor& a, const at::Tensor& b_codes, const at::Tensor& b_scales, int64_t N,
+                    const OptTensor& bias, at::ScalarType out_dtype) {
+    TORCH_CHECK(a.is_cuda(), "a must be a CUDA tensor");
+    TORCH_CHECK(a.scalar_type() == at::kHalf || a.scalar_type() == at::kBFloat16, "a must be float16 or bfloat16");
+    TORCH_CHECK(a.dim() == 2 && a.size(1) >= 1, "a must be 2D with at least one column");
+    TORCH_CHECK(N >= 1, "N must be positive");
+    TORCH_CHECK(b_codes.device() == a.device(), "b must be on the same device as a");
+    const int64_t M = a.size(0), K = a.size(1);
+    check_packed(b_codes, b_scales, N, K, "b");
+    check_mm_out(bias, a.device(), N, out_dtype);
+    const c10::DeviceGuard guard(a.device());
+    const at::Tensor r = as_rows(a);
+    const int code = a.scalar_type() == at::kHalf ? FEATHER_DTYPE_F16 : FEATHER_DTYPE_BF16;
+    if (feather_mxfp4_mm_takes_16bit(M, N, K))
+        return run_mm(r.data_ptr(), nullptr, code, r.stride(0), b_codes, b_scales, bias, M, N, K, out_dtype);
+    const Packed q = empty_packed(M, K, a);
+    check_status(feather_mxfp4_quantize(r.data_ptr(), code, M, K, r.stride(0), bytes_out(q.codes), bytes_out(q.scales),
+                                        stream_of(a)),
+                 "mxfp4_mm");
+    return run_mm(q.codes.data_ptr(), bytes(q.scales), FEATHER_DTYPE_MXFP4, 0, b_codes, b_scales, bias, M, N, K, out_dtype);
+}
+
+at::Tensor mxfp4_mm_packed(const at::Tensor& a_codes, const at::Tensor& a_scales, int64_t M, int64_t K,
+                           const at::Tensor& b_codes, const at::Tensor& b_scales, int64_t N, const OptTensor& bias,
+                           at::ScalarType out_dtype) {
+    TORCH_CHECK(M >= 0 && N >= 1 && K >= 1, "M must not be negative, N and K must be positive");
+    check_packed(a_codes, a_scales, M, K, "a");
+    check_packed(b_codes, b_scales, N, K, "b");
+    TORCH_CHECK(b_codes.device() == a_codes.device(), "b must be on the same device as a");
+    check_mm_out(bias, a_codes.device(), N, out_dtype);
+    const c10::DeviceGuard guard(a_codes.device());
+    return run_mm(a_codes.data_ptr(), bytes(a_scales), FEATHER_DTYPE_MXFP4, 0, b_codes, b_scales, bias, M, N, K, out_dtype);
+}
+
+// ---- norms ----
+
+// A vector or one vector per group of rows: t broadcast against x (..., cols). Rows of x that
+// share a row of t are consecutive unless t repeats along a leading dimension alone, in which
+// case it is written out.
+struct RowVectors {
+    at::Tensor t;  // keeps a copy alive until the launch
+    const void* p = nullptr;
+    int64_t group = 1, stride = 0;
+};
+
+RowVectors row_vectors(const at::Tensor& x, const at::Tensor& t, at::ScalarType dtype, const char* what) {
+    const int64_t cols = x.size(-1), rows = x.numel() / cols;
+    TORCH_CHECK(t.device() == x.device(), what, " must be on the same device as x");
+    value_code(t.scalar_type(), what);
+    TORCH_CHECK(t.dim() >= 1 && t.size(-1) == cols && t.dim() <= x.dim(), what, " must end in x's ", cols,
+                " columns and broadcast against x");
+    const int64_t skip = x.dim() - t.dim();
+    int64_t group = 1, i = x.dim() - 2;
+    for (; i >= 0 && (i < skip || t.size(i - skip) == 1); --i) group *= x.size(i);
+    bool whole = true;  // every dimension before the shared ones is t's own
+    for (int64_t j = i; j >= 0; --j) {
+        const int64_t n = j < skip ? 1 : t.size(j - skip);
+        TORCH_CHECK(n == x.size(j) || n == 1, what, " must broadcast against x");
+        whole = whole && n == x.size(j);
+    }
+    RowVectors r;
+    r.t = whole ? t : t.expand(x.sizes());
+    if (!whole) group = 1;
+    r.t = as_rows(r.t);
+    if (r.t.scalar_type() != dtype) r.t = r.t.to(dtype);
+    r.p = r.t.data_ptr();
+    r.group = group > 0 ? group : 1;
+    r.stride = r.t.size(0) > 1 ? r.t.stride(0) : 0;
+    if (rows == 0) r.stride = 0;
+    return r;
+}
+
+at::Tensor column_vector(const at::Tensor& x, const at::Tensor& t, at::ScalarType dtype, const char* what) {
+    TORCH_CHECK(t.device() == x.device(), what, " must be on the same device as x");
+    value_code(t.scalar_type(), what);
+    TORCH_CHECK(t.dim() == 1 && t.size(0) == x.size(-1), what, " must have x's ", x.size(-1), " columns");
+    const at::Tensor c = t.scalar_type() == dtype ? t : t.to(dtype);
+    return c.size(0) > 1 && c.stride(0) != 1 ? c.contiguous() : c;
+}
+
+struct NormOut {
+    at::Tensor stream, y;
+    Packed q;
+};
+
+NormOut run_norm(const at::Tensor& x, const OptTensor& h, const OptTensor& gate, const OptTensor& post_weight,
+                 const OptTensor& weight, const OptTensor& bias, const OptTensor& scale, const OptTensor& shift,
+                 bool layer, double eps, double residual_scale, std::optional<at::ScalarType> out_dtype, bool codes) {
+    TORCH_CHECK(x.is_cuda(), "x must be a CUDA tensor");
+    TORCH_CHECK(x.dim() >= 1 && x.size(-1) >= 1 && x.size(-1) <= 16384, "x must have 1 to 16384 columns");
+    const int64_t cols = x.size(-1), rows = x.numel() / cols;
+    const int x_code = value_code(x.scalar_type(), "x");
+    if (h.has_value()) {
+        TORCH_CHECK(h->device() == x.device(), "h must be on the same device as x");
+        TORCH_CHECK(h->sizes() == x.sizes(), "h must have x's shape");
+        TORCH_CHECK(!out_dtype.has_value() || *out_dtype == h->scalar_type(), "out_dtype must be h's dtype");
+    }
+    const at::ScalarType block = h.has_value() ? h->scalar_type() : out_dtype.value_or(x.scalar_type());
+    const int y_code = value_code(block, h.has_value() ? "h" : "out_dtype");
+    TORCH_CHECK(x_code == FEATHER_DTYPE_F32 || x_code == y_code, "x must be float32 or of the block's dtype (", block, ")");
+    // the vectors share one type: the block's if they all have it, otherwise fp32
+    at::ScalarType mods = block;
+    for (const OptTensor* t : {&gate, &post_weight, &weight, &bias, &scale, &shift})
+        if (t->has_value() && (*t)->scalar_type() != block) mods = at::kFloat;
+
+    const c10::DeviceGuard guard(x.device());
+    const at::Tensor xr = as_rows(x);
+    at::Tensor hr, pw, w, b;
+    RowVectors g, sc, sh;
+    if (h.has_value()) hr = as_rows(*h);
+    if (gate.has_value()) g = row_vectors(x, *gate, mods, "gate");
+    if (scale.has_value()) sc = row_vectors(x, *scale, mods, "scale");
+    if (shift.has_value()) sh = row_vectors(x, *shift, mods, "shift");
+    if (scale.has_value() && shift.has_value() && sc.group != sh.group) {  // one for the rows, one for groups: both by row
+        sc = row_vectors(x, scale->expand(x.sizes()), mods, "scale");
+        sh = row_vectors(x, shift->expand(x.sizes()), mods, "shift");
+    }
+    if (post_weight.has_value()) pw = column_vector(x, *post_weight, mods, "post_weight");
+    if (weight.has_value()) w = column_vector(x, *weight, mods, "weight");
+    if (bias.has_value()) b = column_vector(x, *bias, mods, "bias");
+
+    NormOut out;
+    if (h.has_value()) out.stream = at::empty(x.sizes(), x.options());
+    if (codes) out.q = empty_packed(rows, cols, x);
+    else out.y = at::empty(x.sizes(), x.options().dtype(block));
+    feather_block_norm_args a{};
+    a.x = xr.data_ptr();
+    a.h = h.has_value() ? hr.data_ptr() : nullptr;
+    a.gate = g.p;
+    a.post_weight = pw.defined() ? pw.data_ptr() : nullptr;
+    a.weight = w.defined() ? w.data_ptr() : nullptr;
+    a.bias = b.defined() ? b.data_ptr() : nullptr;
+    a.scale = sc.p;
+    a.shift = sh.p;
+    a.x_out = out.stream.defined() ? out.stream.data_ptr() : nullptr;
+    a.y = codes ? nullptr : out.y.data_ptr();
+    a.codes = codes ? bytes_out(out.q.codes) : nullptr;
+    a.scales = codes ? bytes_out(out.q.scales) : nullptr;
+    a.rows = rows;
+    a.cols = cols;
+    a.x_row_stride = xr.stride(0);
+    a.h_row_stride = h.has_value() ? hr.stride(0) : 0;
+    a.gate_group = g.group;
+    a.gate_row_stride = g.stride;
+    a.mod_group = scale.has_value() ? sc.group : sh.group;
+    a.scale_row_stride = sc.stride;
+    a.shift_row_stride = sh.stride;
+    a.x_dtype = x_code;
+    a.y_dtype = y_code;
+    a.mod_dtype = value_code(mods, "mods");
+    a.norm = layer ? 1 : 0;
+    a.eps = static_cast<float>(eps);
+    a.residual_scale = static_cast<float>(residual_scale);
+    check_status(feather_block_norm(&a, stream_of(x)), h.has_value() ? "gated_residual_norm" : "modulated_norm");
+    return out;
+}
+
+at::Tensor modulated_norm(const at::Tensor& x, const OptTensor& weight, const OptTensor& bias, const OptTensor& scale,
+                          const OptTensor& shift, bool layer, double eps, std::optional<at::ScalarType> out_dtype) {
+    return run_norm(x, {}, {}, {}, weight, bias, scale, shift, layer, eps, 1.0, out_dtype, false).y;
+}
+
+std::tuple<at::Tensor, at::Tensor> modulated_norm_mxfp4(const at::Tensor& x, const OptTensor& weight,
+                                                        const OptTensor& bias, const OptTensor& scale,
+                                                        const OptTensor& shift, bool layer, double eps) {
+    const NormOut o = run_norm(x, {}, {}, {}, weight, bias, scale, shift, layer, eps, 1.0, {}, true);
+    return {o.q.codes, o.q.scales};
+}
+
+std::tuple<at::Tensor, at::Tensor> gated_residual_norm(const at::Tensor& x, const at::Tensor& h, const OptTensor& gate,
+                                                       const OptTensor& post_weight, const OptTensor& weight,
+                                                       const OptTensor& bias, const OptTensor& scale,
+                                                       const OptTensor& shift, bool layer, double eps,
+                                                       double residual_scale, std::optional<at::ScalarType> out_dtype) {
+    const NormOut o = run_norm(x, h, gate, post_weight, weight, bias, scale, shift, layer, eps, residual_scale, out_dtype, false);
+    return {o.stream, o.y};
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> gated_residual_norm_mxfp4(
+    const at::Tensor& x, const at::Tensor& h, const OptTensor& gate, const OptTensor& post_weight,
+    const OptTensor& weight, const OptTensor& bias, const OptTensor& scale, const OptTensor& shift, bool layer,
+    double eps, double residual_scale) {
+    const NormOut o = run_norm(x, h, gate, post_weight, weight, bias, scale, shift, layer, eps, residual_scale, {}, true);
+    return {o.stream, o.q.codes, o.q.scales};
+}
+
+// ---- fake tensors ----
+
+std::tuple<at::Tensor, at::Tensor> quantize_mxfp4_meta(const at::Tensor& x) {
+    const Packed q = empty_packed(x.numel() / x.size(-1), x.size(-1), x);
+    return {q.codes, q.scales};
+}
+at::Tensor dequantize_mxfp4_meta(const at::Tensor& codes, const at::Tensor&, int64_t rows, int64_t cols, at::ScalarType dtype) {
+    return at::empty({rows, cols}, codes.options().dtype(dtype));
+}
+std::tuple<at::Tensor, at::Tensor> prepack_mxfp4_meta(const at::Tensor& codes, const at::Tensor&, int64_t cols) {
+    const Packed q = empty_packed(codes.size(0), cols, codes);
+    return {q.codes, q.scales};
+}
+std::tuple<at::Tensor, at::Tensor> unprepack_mxfp4_meta(const at::Tensor& codes, const at::Tensor&, int64_t rows, int64_t cols) {
+    const int64_t blocks = (cols + 31) / 32;
+    return {at::empty({rows, blocks * 16}, codes.options()), at::empty({rows, blocks}, codes.options())};
+}
+at::Tensor mxfp4_mm_meta(const at::Tensor& a, const at::Tensor&, const at::Tensor&, int64_t N, const OptTensor&,
+                         at::ScalarType out_dtype) {
+    return at::empty({a.size(0), N}, a.options().dtype(out_dtype));
+}
+at::Tensor mxfp4_mm_packed_meta(const at::Tensor& a_codes, const at::Tensor&, int64_t M, int64_t, const at::Tensor&,
+                                const at::Tensor&, int64_t N, const OptTensor&, at::ScalarType out_dtype) {
+    return at::empty({M, N}, a_codes.options().dtype(out_dtype));
+}
+at::Tensor modulated_norm_meta(const at::Tensor& x, const OptTensor&, const OptTensor&, const OptTensor&, const OptTensor&,
+                               bool, double, std::optional<at::ScalarType> out_dtype) {
+    return at::empty(x.sizes(), x.options().dtype(out_dtype.value_or(x.scalar_type())));
+}
+std::tuple<at::Tensor, at::Tensor> modulated_norm_mxfp4_meta(const at::Tensor& x, const OptTensor&, const OptTensor&,
+                                                             const OptTensor&, const OptTensor&, bool, double) {
+    return quantize_mxfp4_meta(x);
+}
+std::tuple<at::Tensor, at::Tensor> gated_residual_norm_meta(const at::Tensor& x, const at::Tensor& h, const OptTensor&,
+                                                            const OptTensor&, const OptTensor&, const OptTensor&,
+                                                            const OptTensor&, const OptTensor&, bool, double, double,
+                                                            std::optional<at::ScalarType>) {
+    return {at::empty(x.sizes(), x.options()), at::empty(x.sizes(), h.options())};
+}
+std::tuple<at::Tensor, at::Tensor, at::Tensor> gated_residual_norm_mxfp4_meta(
+    const at::Tensor& x, const at::Tensor&, const OptTensor&, const OptTensor&, const OptTensor&, const OptTensor&,
+    const OptTensor&, const OptTensor&, bool, double, double) {
+    const auto [codes, scales] = quantize_mxfp4_meta(x);
+    return {at::empty(x.sizes(), x.options()), codes, scales};
+}
+
+}  // namespace
+
+TORCH_LIBRARY_FRAGMENT(feather_ops, m) {
+    m.def("quantize_mxfp4(Tensor x) -> (Tensor, Tensor)");
+    m.def("dequantize_mxfp4(Tensor codes, Tensor scales, int rows, int cols, ScalarType dtype) -> Tensor");
+    m.def("prepack_mxfp4(Tensor codes, Tensor scales, int cols) -> (Tensor, Tensor)");
+    m.def("unprepack_mxfp4(Tensor codes, Tensor scales, int rows, int cols) -> (Tensor, Tensor)");
+    m.def("mxfp4_mm(Tensor a, Tensor b_codes, Tensor b_scales, int N, Tensor? bias, ScalarType out_dtype) -> Tensor");
+    m.def("mxfp4_mm_packed(Tensor a_codes, Tensor a_scales, int M, int K, Tensor b_codes, Tensor b_scales, int N, "
+          "Tensor? bias, ScalarType out_dtype) -> Tensor");
+    m.def("modulated_norm(Tensor x, Tensor? weight, Tensor? bias, Tensor? scale, Tensor? shift, bool layer, float eps, "
+          "ScalarType? out_dtype) -> Tensor");
+    m.def("modulated_norm_mxfp4(Tensor x, Tensor? weight, Tensor? bias, Tensor? scale, Tensor? shift, bool layer, "
+          "float eps) -> (Tensor, Tensor)");
+    m.def("gated_residual_norm(Tensor x, Tensor h, Tensor? gate, Tensor? post_weight, Tensor? weight, Tensor? bias, "
+          "Tensor? scale, Tensor? shift, bool layer, float eps, float residual_scale, ScalarType? out_dtype) -> "
+          "(Tensor, Tensor)");
+    m.def("gated_residual_norm_mxfp4(Tensor x, Tensor h, Tensor? gate, Tensor? post_weight, Tensor? weight, "
+          "Tensor? bias, Tensor? scale, Tensor? shift, bool layer, float eps, float residual_scale) -> "
+          "(Tensor, Tensor, Tensor)");
+}
+
+TORCH_LIBRARY_IMPL(feather_ops, CUDA, m) {
+    m.impl("quantize_mxfp4", &quantize_mxfp4);
+    m.impl("dequantize_mxfp4", &dequantize_mxfp4);
+    m.impl("prepack_mxfp4", &prepack_mxfp4);
+    m.impl("unprepack_mxfp4", &unprepack_mxfp4);
+    m.impl("mxfp4_mm", &mxfp4_mm);
+    m.impl("mxfp4_mm_packed", &mxfp4_mm_packed);
+    m.impl("modulated_norm", &modulated_norm);
+    m.impl("modulated_norm_mxfp4", &modulated_norm_mxfp4);
+    m.impl("gated_residual_norm", &gated_residual_norm);
+    m.impl("gated_residual_norm_mxfp4", &gated_residual_norm_mxfp4);
+}
+
+TORCH_LIBRARY_IMPL(feather_ops, Meta, m) {
+    m.impl("quantize_mxfp4", &quantize_mxfp4_meta);
+    m.impl("dequantize_mxfp4", &dequantize_mxfp4_meta);
+    m.impl("prepack_mxfp4", &prepack_mxfp4_meta);
+    m.impl("unprepack_mxfp4", &unprepack_mxfp4_meta);
+    m.impl("mxfp4_mm", &mxfp4_mm_meta);
+    m.impl("mxfp4_mm_packed", &mxfp4_mm_packed_meta);
+    m.impl("modulated_norm", &modulated_norm_meta);
+    m.impl("modulated_norm_mxfp4", &modulated_norm_mxfp4_meta);
+    m.impl("gated_residual_norm", &gated_residual_norm_meta);
+    m.impl("gated_residual_norm_mxfp4", &gated_residual_norm_mxfp4_meta);
+}

@@ -62,6 +62,17 @@ SIGNATURES: dict[str, tuple] = {
     "feather_bf16_to_fp16": (_int, [_vp, _vp, _i64, _vp]),
     "feather_bf16_to_fp16_rne": (_int, [_vp, _vp, _i64, _vp]),
     "feather_dequantize_e5m2": (_int, [_vp, _vp, _vp, _int, _i64, _i64, _vp]),
+    "feather_mxfp4_codes_bytes": (ctypes.c_size_t, [_i64, _i64]),
+    "feather_mxfp4_scales_bytes": (ctypes.c_size_t, [_i64, _i64]),
+    "feather_mxfp4_quantize": (_int, [_vp, _int, _i64, _i64, _i64, _vp, _vp, _vp]),
+    "feather_mxfp4_dequantize": (_int, [_vp, _vp, _vp, _int, _i64, _i64, _vp]),
+    "feather_mxfp4_prepack": (_int, [_vp, _vp, _vp, _vp, _i64, _i64, _vp]),
+    "feather_mxfp4_unprepack": (_int, [_vp, _vp, _vp, _vp, _i64, _i64, _vp]),
+    "feather_mxfp4_mm_takes_16bit": (_int, [_i64, _i64, _i64]),
+    "feather_mxfp4_mm_workspace_size": (ctypes.c_size_t, [_i64, _i64, _i64, _int]),
+    "feather_mxfp4_mm": (_int, [_vp, _vp, _int, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _int, _vp,
+                                ctypes.c_size_t, _vp]),
+    "feather_block_norm": (_int, [_vp, _vp]),
     "feather_status_string": (ctypes.c_char_p, [_int]),
     "feather_abi_version": (_int, []),
 }

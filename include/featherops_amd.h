@@ -40,6 +40,7 @@ extern "C" {
 #define FEATHER_DTYPE_F16 0
 #define FEATHER_DTYPE_BF16 1
 #define FEATHER_DTYPE_F32 2
+#define FEATHER_DTYPE_MXFP4 3 /* packed MXFP4 codes and scales, see below */
 #define FEATHER_B_E4M3FN 0
 #define FEATHER_B_E5M2 1
 
@@ -314,6 +315,101 @@ int feather_bf16_to_fp16_rne(const uint16_t* in, uint16_t* out, int64_t n, hipSt
  * Replaces quant.py:99-102 (FeatherFP8E5M2PackedLayout.dequantize). */
 int feather_dequantize_e5m2(const uint8_t* packed, const float* scale, void* out, int out_dtype, int64_t N, int64_t K,
                             hipStream_t stream);
+
+/*
+ * MXFP4: 4-bit codes (e2m1: 0, 0.5, 1, 1.5, 2, 3, 4, 6, a sign) of 32 consecutive
+ * values of a row under one power of two (e8m0: byte b stands for 2^(b - 127), 255
+ * for NaN). A block's scale is 2^max(floor(log2 amax) - 2, -127), its codes the
+ * values nearest to v / scale (ties to the even code, 6 beyond 6); a block with a
+ * NaN or an infinity becomes NaN as a whole. A last block shorter than 32 counts as
+ * continued by zeros. No counterpart in the reference.
+ *
+ * Row-major form (checkpoints), blocks = ceil(cols / 32): codes (rows, blocks * 16)
+ * bytes, the earlier value of a pair in the low half; scales (rows, blocks).
+ * Packed form (operands), steps = ceil(cols / 128), groups = ceil(rows / 64):
+ *   codes  [4 * groups][steps][64][16]: row r, column k in byte (k % 32) / 2 of
+ *          [r / 16][k / 128][16 * (k % 128 / 32) + r % 16]
+ *   scales [groups][steps][64][4]: that block's in byte r / 16 % 4 of
+ *          [r / 64][k / 128][16 * (k % 128 / 32) + r % 16]
+ * Buffers of the packed form are 16-byte aligned. rows <= 2^30, cols < 2^24.
+ */
+size_t feather_mxfp4_codes_bytes(int64_t rows, int64_t cols);  /* of the packed form; 0 for sizes outside the domain */
+size_t feather_mxfp4_scales_bytes(int64_t rows, int64_t cols);
+
+/* (rows, cols) fp16 / bf16 / fp32 values, row_stride elements between rows, any
+ * alignment of the element type -> packed form. */
+int feather_mxfp4_quantize(const void* x, int x_dtype, int64_t rows, int64_t cols, int64_t row_stride, uint8_t* codes,
+                           uint8_t* scales, hipStream_t stream);
+
+/* Packed form -> (rows, cols) values of out_dtype, contiguous, each rounded once. */
+int feather_mxfp4_dequantize(const uint8_t* codes, const uint8_t* scales, void* out, int out_dtype, int64_t rows,
+                             int64_t cols, hipStream_t stream);
+
+/* Row-major form -> packed form, and back. */
+int feather_mxfp4_prepack(const uint8_t* codes_rows, const uint8_t* scales_rows, uint8_t* codes, uint8_t* scales,
+                          int64_t rows, int64_t cols, hipStream_t stream);
+int feather_mxfp4_unprepack(const uint8_t* codes, const uint8_t* scales, uint8_t* codes_rows, uint8_t* scales_rows,
+                            int64_t rows, int64_t cols, hipStream_t stream);
+
+/*
+ * C (M, N) = out(q(A) . B^T + bias): fp32 sums of the 4-bit operands' exact
+ * products, the bias added in fp32, one rounding to output_dtype (fp16 or bf16).
+ *   a_dtype FEATHER_DTYPE_MXFP4: a and a_scales are A (M, K) in the packed form.
+ *   a_dtype F16 / BF16: a holds A's values, a_row_stride elements between rows, and
+ *     is quantised on the way (the values of feather_mxfp4_quantize); a_scales is
+ *     not read. Served where feather_mxfp4_mm_takes_16bit says so (few rows),
+ *     FEATHER_ERR_UNSUPPORTED elsewhere: the caller quantises A and calls again.
+ *   b, b_scales: B (N, K) in the packed form. bias: (N,) of the output type, or NULL.
+ * Any M >= 0, N >= 1, K >= 1; c is contiguous, at any alignment of its type.
+ * Workspace: the size below, the contract of feather_launch_scaled_mm_ws (its first
+ * 64 KB zero before the first use and left zero); with less, K is not split and the
+ * sums run in another order.
+ */
+int feather_mxfp4_mm_takes_16bit(int64_t M, int64_t N, int64_t K);
+size_t feather_mxfp4_mm_workspace_size(int64_t M, int64_t N, int64_t K, int a_dtype);
+int feather_mxfp4_mm(const void* a, const uint8_t* a_scales, int a_dtype, int64_t a_row_stride, const uint8_t* b,
+                     const uint8_t* b_scales, const uint16_t* bias, uint16_t* c, int64_t M, int64_t N, int64_t K,
+                     int output_dtype, void* workspace, size_t workspace_bytes, hipStream_t stream);
+
+/*
+ * The norms around a block, one pass over (rows, cols), cols <= 16384:
+ *   h' = post_weight ? norm(h) * post_weight : h
+ *   s  = residual_scale * x + gate * h'   (fp32; s = x where h is NULL), x_out = s
+ *   y  = norm(s) * weight + bias;  y = y * (1 + scale) + shift
+ * norm 0: v / sqrt(mean(v^2) + eps); 1: (v - mean) / sqrt(variance + eps), statistics
+ * in fp32 on s before it is rounded. Pointers other than x may be NULL: the factor,
+ * the term or the output is then left out. Row r reads its gate at
+ * gate + r / gate_group * gate_row_stride, its scale and shift at r / mod_group
+ * likewise (rows of one sample share them, or all rows with a group of `rows`).
+ *   x, x_out: x_dtype. h, y: y_dtype, which is x_dtype unless x is fp32. The vectors:
+ *   mod_dtype, y_dtype or fp32. Last dimensions are contiguous, row strides count
+ *   elements, x_out and y are contiguous; any alignment of the element types.
+ *   Either y, or codes and scales: y quantised from fp32 into the packed MXFP4 form
+ *   (bytes of rows past the last one are left as they are).
+ * No counterpart in the reference.
+ */
+typedef struct feather_block_norm_args {
+    const void* x;
+    const void* h;
+    const void* gate;
+    const void* post_weight;
+    const void* weight;
+    const void* bias;
+    const void* scale;
+    const void* shift;
+    void* x_out;
+    void* y;
+    uint8_t* codes;
+    uint8_t* scales;
+    int64_t rows, cols;
+    int64_t x_row_stride, h_row_stride;
+    int64_t gate_group, gate_row_stride;
+    int64_t mod_group, scale_row_stride, shift_row_stride;
+    int x_dtype, y_dtype, mod_dtype;
+    int norm;
+    float eps, residual_scale;
+} feather_block_norm_args;
+int feather_block_norm(const feather_block_norm_args* args, hipStream_t stream);
 
 /* Text for a status code. */
 const char* feather_status_string(int status);
