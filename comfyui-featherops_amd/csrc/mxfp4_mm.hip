@@ -1,6 +1,8 @@
 // C (M, N) = A (M, K) . B (N, K)^T + bias with both operands packed MXFP4
 // (mxfp4.h), on the block-scaled 16x16x128 MFMA with fp32 accumulators.
 #include <algorithm>
+#include <type_traits>
+#include <utility>
 
 #include "featherops_amd.h"
 #include "lds_dma.h"
@@ -116,33 +118,30 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN == 4 ? 1 : 2) void mx_tile_ke
         src[kCodes + i] = (is_a ? p.as : p.bs) + (g * p.ksteps + k0) * 256;
         dst[kCodes + i] = lds + kScaleBase + j * 256;
     }
-    auto issue = [&](int step, int slot) {
-        const int s = min(step, steps - 1);
-#pragma unroll
-        for (int i = 0; i < kCodes; ++i) dma16_lds(src[i] + static_cast<int64_t>(s) * 1024, lane * 16, dst[i] + slot * kStageBytes);
-#pragma unroll
-        for (int i = kCodes; i < kPerWave; ++i) dma4_lds(src[i] + static_cast<int64_t>(s) * 256, lane * 4, dst[i] + slot * kStageBytes);
+    auto copy = [&](auto i, int step, int slot) {
+        if constexpr (i < kCodes) dma16_lds(src[i] + static_cast<int64_t>(step) * 1024, lane * 16, dst[i] + slot * kStageBytes);
+        else dma4_lds(src[i] + static_cast<int64_t>(step) * 256, lane * 4, dst[i] + slot * kStageBytes);
     };
 
     struct Frags {
         uint4 a[FM], b[FN];
         uint32_t sa[SM], sb[SN];
     };
-    auto read = [&](Frags& f, int slot) {
-        const uint8_t* base = smem + slot * kStageBytes;
-#pragma unroll
-        for (int i = 0; i < FN; ++i) f.b[i] = *reinterpret_cast<const uint4*>(base + (BM / 16 + wn * FN + i) * 1024 + lane * 16);
-#pragma unroll
-        for (int i = 0; i < FM; ++i) f.a[i] = *reinterpret_cast<const uint4*>(base + (wm * FM + i) * 1024 + lane * 16);
-#pragma unroll
-        for (int i = 0; i < SN; ++i) {
-            f.sb[i] = *reinterpret_cast<const uint32_t*>(base + kScaleBase + (kGroupsM + wn * TN / 64 + i) * 256 + lane * 4);
-            if constexpr (FN == 2) f.sb[i] >>= 16 * (wn % 2);
-        }
-#pragma unroll
-        for (int i = 0; i < SM; ++i) {
+    constexpr int kReads = SM + SN + FM + FN;
+    auto read = [&](auto r, Frags& f, const uint8_t* base) {
+        if constexpr (r < SN) {
+            f.sb[r] = *reinterpret_cast<const uint32_t*>(base + kScaleBase + (kGroupsM + wn * TN / 64 + r) * 256 + lane * 4);
+            if constexpr (FN == 2) f.sb[r] >>= 16 * (wn % 2);
+        } else if constexpr (r < SN + SM) {
+            constexpr int i = r - SN;
             f.sa[i] = *reinterpret_cast<const uint32_t*>(base + kScaleBase + (wm * TM / 64 + i) * 256 + lane * 4);
             if constexpr (FM == 2) f.sa[i] >>= 16 * (wm % 2);
+        } else if constexpr (r < SN + SM + FN) {
+            constexpr int i = r - SN - SM;
+            f.b[i] = *reinterpret_cast<const uint4*>(base + (BM / 16 + wn * FN + i) * 1024 + lane * 16);
+        } else {
+            constexpr int i = r - SN - SM - FN;
+            f.a[i] = *reinterpret_cast<const uint4*>(base + (wm * FM + i) * 1024 + lane * 16);
         }
     };
 
@@ -151,29 +150,40 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN == 4 ? 1 : 2) void mx_tile_ke
     for (int i = 0; i < FM; ++i)
 #pragma unroll
         for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    auto multiply = [&](const Frags& f) {
-        unrolled<FM>([&](auto i) {
-            unrolled<FN>([&](auto j) {
-                acc[i][j] = mfma_mx<j % 4, i % 4>(f.b[j], f.a[i], acc[i][j], f.sb[j / 4], f.sa[i / 4]);
-            });
-        });
+    auto multiply = [&](auto n, const Frags& f) {
+        constexpr int i = n / FN, j = n % FN;
+        acc[i][j] = mfma_mx<j % 4, i % 4>(f.b[j], f.a[i], acc[i][j], f.sb[j / 4], f.sa[i / 4]);
     };
 
 #pragma unroll
-    for (int s = 0; s < kStages; ++s) issue(s, s);
+    for (int s = 0; s < kStages; ++s) unrolled<kPerWave>([&](auto i) { copy(i, min(s, steps - 1), s); });
     Frags f0, f1;
     wait_vmcnt<(kStages - 1) * kPerWave>();
     stage_barrier();
-    read(f0, 0);
+    unrolled<kReads>([&](auto r) { read(r, f0, smem); });
     int slot = 0;  // of the step being multiplied
-    auto iterate = [&](int k, Frags& now, Frags& next) {
+    // One step. The copies and the next step's reads are pinned between the MFMAs, all of them in the
+    // first three quarters: left alone, the compiler reads each fragment into the registers of the one
+    // just used up, after its last MFMA, and every step waits for LDS with the matrix cores idle.
+    constexpr int kMfmas = FM * FN, kOps = kPerWave + kReads, kOver = kMfmas >= 8 ? kMfmas * 3 / 4 : kMfmas;
+    auto iterate = [&](int k, const Frags& now, Frags& next) {
         const int after = slot + 1 == kStages ? 0 : slot + 1;
+        const int ahead = min(k + kStages, steps - 1);
+        const uint8_t* base = smem + after * kStageBytes;
         // stage k + 1 has landed; this wave's reads of stage k are done
         wait_vmcnt_lgkm0<(kStages - 2) * kPerWave>();
         stage_barrier();
-        issue(k + kStages, slot);
-        read(next, after);
-        multiply(now);
+        unrolled<kMfmas>([&](auto n) {
+            multiply(n, now);
+            constexpr int first = n < kOver ? n * kOps / kOver : kOps, last = n < kOver ? (n + 1) * kOps / kOver : kOps;
+            unrolled<last - first>([&](auto o) {
+                // the copies in even steps among the reads
+                constexpr int op = first + o, copies = (op + 1) * kPerWave / kOps, before = op * kPerWave / kOps;
+                if constexpr (copies > before) copy(std::integral_constant<int, before>{}, ahead, slot);
+                else read(std::integral_constant<int, op - before>{}, next, base);
+            });
+            __builtin_amdgcn_sched_barrier(0);
+        });
         slot = after;
     };
     int k = 0;
@@ -181,11 +191,10 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN == 4 ? 1 : 2) void mx_tile_ke
         iterate(k, f0, f1);
         iterate(k + 1, f1, f0);
     }
-    if (k < steps) multiply(f0);
+    if (k < steps) unrolled<kMfmas>([&](auto n) { multiply(n, f0); });
     wait_vmcnt<0>();
 
     const int lm = lane & 15;
-    const int ln = (lane >> 4) * 4;
     if (p.ksplit > 1) {
         // Each split writes its fp32 accumulators to the workspace in fragment order and counts itself
         // in; the last to arrive adds the splits' sums in split order and goes on to the epilogue.
@@ -227,28 +236,44 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN == 4 ? 1 : 2) void mx_tile_ke
             __hip_atomic_store(&p.counters[lin], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
 
-    // epilogue: bias added in fp32, one rounding to the output type
-    unrolled<FN>([&](auto j) {
-        const int n = n0 + wn * TN + j * 16 + ln;
-        if (n >= p.N) return;
-        const int have = min(4, p.N - n);
-        float bias[4] = {0.f, 0.f, 0.f, 0.f};
+    // Epilogue: bias added in fp32, one rounding to the output type. A lane has four columns of each
+    // fragment; neighbouring quarters of the wave (lane ^ 16) trade one fragment of a pair for the other,
+    // so that every lane stores 8 columns and a row gets 64 contiguous bytes from one instruction.
+    const int kb = lane >> 4;
+    unrolled<FN / 2>([&](auto h) {
+        constexpr int j = 2 * h;
+        const int n = n0 + wn * TN + (j + (kb & 1)) * 16 + (kb >> 1) * 8;  // after the trade
+        float bias[2][4] = {};
         if (p.bias) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (e < have) bias[e] = out_bits_to_f32<kBf16>(p.bias[n + e]);
+            for (int f = 0; f < 2; ++f)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    bias[f][e] = out_bits_to_f32<kBf16>(p.bias[min(n0 + wn * TN + (j + f) * 16 + kb * 4 + e, p.N - 1)]);
         }
         unrolled<FM>([&](auto i) {
             const int64_t m = m0 + wm * TM + i * 16 + lm;
-            if (m >= p.M) return;
-            const f32x4 v = acc[i][j];
-            const uint32_t o[2] = {f32x2_to_out_bits<kBf16>(v[0] + bias[0], v[1] + bias[1]),
-                                   f32x2_to_out_bits<kBf16>(v[2] + bias[2], v[3] + bias[3])};
+            uint32_t o[2][2];
+#pragma unroll
+            for (int f = 0; f < 2; ++f)
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                    o[f][e] = f32x2_to_out_bits<kBf16>(acc[i][j + f][2 * e] + bias[f][2 * e], acc[i][j + f][2 * e + 1] + bias[f][2 * e + 1]);
+            uint32_t v[4];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const auto r = __builtin_amdgcn_permlane16_swap(o[0][e], o[1][e], false, false);
+                v[e] = r[0];
+                v[2 + e] = r[1];
+            }
+            if (m >= p.M || n >= p.N) return;
             uint16_t* c = p.c + m * p.N + n;
-            if (have == 4) {
-                __builtin_memcpy(c, o, 8);
+            if (n + 8 <= p.N) {
+                __builtin_memcpy(c, v, 16);
             } else {
-                for (int e = 0; e < have; ++e) c[e] = static_cast<uint16_t>(o[e >> 1] >> (16 * (e & 1)));
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (n + e < p.N) c[e] = static_cast<uint16_t>(v[e >> 1] >> (16 * (e & 1)));
             }
         });
     });
@@ -258,14 +283,11 @@ struct Tile {
     int bm, bn;
 };
 // ids 1.. of the plan
-constexpr Tile kTiles[] = {{0, 0}, {64, 64}, {64, 128}, {128, 128}, {256, 256}};
+constexpr Tile kTiles[] = {{0, 0}, {64, 64}, {64, 128}, {128, 128}, {256, 256}, {256, 256}, {128, 256}, {256, 128}, {128, 128}, {128, 256}, {64, 64}, {64, 128}, {256, 192}};
 
 int tile_env() {
-    static const int v = [] {
-        const char* e = getenv("FEATHEROPS_MX_TILE");
-        return e ? atoi(e) : 0;
-    }();
-    return v;
+    const char* e = getenv("FEATHEROPS_MX_TILE");
+    return e ? atoi(e) : 0;
 }
 
 template <int BM, int BN, int WM, int WN, int kStages>
@@ -284,8 +306,10 @@ MxPlan mx_tile_plan(int64_t M, int64_t N, int64_t K) {
     while (tile > 1 && count(tile) < 200) --tile;
     if (tile_env()) tile = tile_env();
     int ksplit = 1;
+    const char* ks = getenv("FEATHEROPS_MX_KS");
     const int64_t tiles = count(tile);
     if (tiles < 128) ksplit = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(256 / tiles, ksteps / 4)));
+    if (ks && atoi(ks)) ksplit = atoi(ks);
     size_t ws = 0;
     if (ksplit > 1) ws = kMxCounterBytes + static_cast<size_t>(tiles) * ksplit * kTiles[tile].bm * kTiles[tile].bn * 4;
     return {tile, ksplit, ws};
@@ -305,6 +329,13 @@ int mx_mm_tiles(const MxMmArgs& p, hipStream_t stream) {
         case 1: launch<64, 64, 2, 2, 6>(a, p.out_bf16, stream); break;
         case 2: launch<64, 128, 2, 2, 6>(a, p.out_bf16, stream); break;
         case 3: launch<128, 128, 2, 2, 5>(a, p.out_bf16, stream); break;
+        case 5: launch<256, 256, 2, 2, 4>(a, p.out_bf16, stream); break;
+        case 6: launch<128, 256, 2, 2, 5>(a, p.out_bf16, stream); break;
+        case 7: launch<256, 128, 2, 2, 5>(a, p.out_bf16, stream); break;
+        case 8: launch<128, 128, 2, 4, 8>(a, p.out_bf16, stream); break;
+        case 9: launch<128, 256, 2, 4, 5>(a, p.out_bf16, stream); break;
+        case 10: launch<64, 64, 2, 2, 12>(a, p.out_bf16, stream); break;
+        case 11: launch<64, 128, 2, 2, 12>(a, p.out_bf16, stream); break;
         default: launch<256, 256, 4, 2, 4>(a, p.out_bf16, stream); break;
     }
     return hipGetLastError() == hipSuccess ? FEATHER_OK : FEATHER_ERR_LAUNCH;
