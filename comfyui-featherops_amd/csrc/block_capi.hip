@@ -64,13 +64,13 @@ int feather_mxfp4_unprepack(const uint8_t* codes, const uint8_t* scales, uint8_t
     return mx_unprepack(codes, scales, codes_rows, scales_rows, rows, cols, stream);
 }
 
-int feather_mxfp4_mm_takes_16bit(int64_t M, int64_t N, int64_t K) {
-    return mm_sizes_ok(M, N, K) && mx_takes_rows(M, N, K, kMxBf16) ? 1 : 0;
+int feather_mxfp4_mm_takes_16bit(int64_t M, int64_t N, int64_t K, int64_t a_row_stride) {
+    return mm_sizes_ok(M, N, K) && M <= kMxFewRows && mx_rows_in_reach(M, a_row_stride) ? 1 : 0;
 }
 
 size_t feather_mxfp4_mm_workspace_size(int64_t M, int64_t N, int64_t K, int a_dtype) {
     if (!mm_sizes_ok(M, N, K) || M == 0) return 0;
-    return (mx_takes_rows(M, N, K, a_dtype) ? mx_rows_plan(M, N, K) : mx_tile_plan(M, N, K)).ws_bytes;
+    return M <= kMxFewRows ? mx_rows_workspace(M, N, K) : mx_tiles_workspace(M, N, K);
 }
 
 int feather_mxfp4_mm(const void* a, const uint8_t* a_scales, int a_dtype, int64_t a_row_stride, const uint8_t* b,
@@ -86,7 +86,7 @@ int feather_mxfp4_mm(const void* a, const uint8_t* a_scales, int a_dtype, int64_
     const MxMmArgs args{static_cast<const uint8_t*>(a), a_scales, a_dtype, a_row_stride, b, b_scales, bias, c, M,
                         static_cast<int>(N), static_cast<int>(K), output_dtype == FEATHER_DTYPE_BF16,
                         static_cast<uint8_t*>(workspace), workspace ? workspace_bytes : 0};
-    if (mx_takes_rows(M, N, K, a_dtype)) return mx_mm_rows(args, stream);
+    if (M <= kMxFewRows) return mx_mm_rows(args, stream);
     if (!packed) return FEATHER_ERR_UNSUPPORTED;
     return mx_mm_tiles(args, stream);
 }

@@ -69,81 +69,122 @@ enum MxType { kMxF16 = 0, kMxBf16 = 1, kMxF32 = 2 };
 template <int T>
 constexpr int kMxElemBytes = T == kMxF32 ? 4 : 2;
 
-// One lane's 32 values as loaded: 4 dwords per uint4, 4 (16-bit) or 8 of them.
-template <int T>
-struct MxRaw {
-    static constexpr int kVecs = T == kMxF32 ? 8 : 4;
-    uint4 v[kVecs];
+template <int kCtrl>
+__device__ __forceinline__ uint32_t quad_perm(uint32_t v) {
+    return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), kCtrl, 0xf, 0xf, true));
+}
+constexpr int kQuadXor1 = 0xB1, kQuadXor2 = 0x4E;
+constexpr int kQuadLane[4] = {0x00, 0x55, 0xAA, 0xFF};
 
-    // values [0, n) from p, zeros beyond
-    __device__ __forceinline__ void load(const uint8_t* p, int n) {
-        if (n == kMxBlock) {
+// Transposes 4 x 4 dwords over four neighbouring lanes: lane s's r[v] becomes lane v's r[s].
+__device__ __forceinline__ void quad_transpose(uint32_t (&r)[4], int lane) {
+    const bool odd = lane & 1, high = lane & 2;
 #pragma unroll
-            for (int i = 0; i < kVecs; ++i) v[i] = load16_unaligned(p + 16 * i);
-        } else {
-            uint32_t w[kVecs * 4];
-#pragma unroll
-            for (int i = 0; i < kVecs * 4; ++i) {
-                if constexpr (T == kMxF32) {
-                    w[i] = i < n ? reinterpret_cast<const uint32_t*>(p)[i] : 0u;
-                } else {
-                    const uint16_t* q = reinterpret_cast<const uint16_t*>(p);
-                    w[i] = (2 * i < n ? static_cast<uint32_t>(q[2 * i]) : 0u) |
-                           (2 * i + 1 < n ? static_cast<uint32_t>(q[2 * i + 1]) << 16 : 0u);
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < kVecs; ++i) v[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
-        }
+    for (int i = 0; i < 4; i += 2) {
+        const uint32_t got = quad_perm<kQuadXor1>(odd ? r[i] : r[i + 1]);
+        if (odd) r[i] = got;
+        else r[i + 1] = got;
     }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const uint32_t got = quad_perm<kQuadXor2>(high ? r[i] : r[i + 2]);
+        if (high) r[i] = got;
+        else r[i + 2] = got;
+    }
+}
 
-    // the block's codes; *scale_byte gets its scale
-    __device__ __forceinline__ uint4 quantize(uint32_t* scale_byte) const {
+// A wave's 16 rows x 128 columns of values on their way to (or from) an operand fragment, in which lane l
+// has row l % 16 and block l / 16. In memory order four neighbouring lanes share the rows' 64-byte
+// (16-bit values) runs instead: piece v of lane l is values 8 (l % 4) .. + 7 of the block that belongs to
+// lane 4 (l / 4) + v, row 4 (l / 4) % 16 + v. A load then touches 64 contiguous bytes per four lanes
+// where whole blocks per lane would touch 16 bytes of each of 64 runs; the codes, a quarter of the
+// values' size, are transposed afterwards.
+__device__ __forceinline__ int mx_piece_row(int lane, int v) { return (lane & 12) + v; }
+__device__ __forceinline__ int mx_piece_col(int lane) { return (lane >> 4) * kMxBlock + (lane & 3) * 8; }
+
+template <int T>
+struct MxPieces {
+    static constexpr int kVecs = T == kMxF32 ? 2 : 1;  // 16-byte vectors of a piece
+    uint4 v[4][kVecs];
+
+    // piece i from p
+    __device__ __forceinline__ void load(int i, const uint8_t* p) {
+#pragma unroll
+        for (int k = 0; k < kVecs; ++k) v[i][k] = load16_unaligned(p + 16 * k);
+    }
+    // piece i: its values [0, n), zeros beyond
+    __device__ __forceinline__ void load_part(int i, const uint8_t* p, int n) {
         uint32_t w[kVecs * 4];
 #pragma unroll
-        for (int i = 0; i < kVecs; ++i) {
-            w[4 * i] = v[i].x;
-            w[4 * i + 1] = v[i].y;
-            w[4 * i + 2] = v[i].z;
-            w[4 * i + 3] = v[i].w;
-        }
-        uint32_t o[4] = {0u, 0u, 0u, 0u};
-        float s;
-        if constexpr (T == kMxF32) {
-            uint32_t m = 0u;
-#pragma unroll
-            for (int i = 0; i < 32; ++i) m = max(m, w[i] & 0x7fffffffu);
-            *scale_byte = mx_scale_byte(bits_f32(m));
-            s = mx_scale_f32(*scale_byte);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                o[i] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(o[i], bits_f32(w[8 * i]), bits_f32(w[8 * i + 1]), s, 0);
-                o[i] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(o[i], bits_f32(w[8 * i + 2]), bits_f32(w[8 * i + 3]), s, 1);
-                o[i] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(o[i], bits_f32(w[8 * i + 4]), bits_f32(w[8 * i + 5]), s, 2);
-                o[i] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(o[i], bits_f32(w[8 * i + 6]), bits_f32(w[8 * i + 7]), s, 3);
-            }
-        } else {
-            uint32_t m = 0u;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) m = max_u16x2(m, w[i] & 0x7fff7fffu);
-            const uint32_t m16 = max(m & 0xffffu, m >> 16);
-            *scale_byte = mx_scale_byte(T == kMxBf16 ? bits_f32(m16 << 16) : half_bits_to_f32(static_cast<uint16_t>(m16)));
-            s = mx_scale_f32(*scale_byte);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if constexpr (T == kMxBf16) {
-                    o[i] = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(o[i], __builtin_bit_cast(bf16x2_t, w[4 * i]), s, 0);
-                    o[i] = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(o[i], __builtin_bit_cast(bf16x2_t, w[4 * i + 1]), s, 1);
-                    o[i] = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(o[i], __builtin_bit_cast(bf16x2_t, w[4 * i + 2]), s, 2);
-                    o[i] = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(o[i], __builtin_bit_cast(bf16x2_t, w[4 * i + 3]), s, 3);
-                } else {
-                    o[i] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(o[i], __builtin_bit_cast(f16x2_t, w[4 * i]), s, 0);
-                    o[i] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(o[i], __builtin_bit_cast(f16x2_t, w[4 * i + 1]), s, 1);
-                    o[i] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(o[i], __builtin_bit_cast(f16x2_t, w[4 * i + 2]), s, 2);
-                    o[i] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(o[i], __builtin_bit_cast(f16x2_t, w[4 * i + 3]), s, 3);
-                }
+        for (int k = 0; k < kVecs * 4; ++k) {
+            if constexpr (T == kMxF32) {
+                w[k] = k < n ? reinterpret_cast<const uint32_t*>(p)[k] : 0u;
+            } else {
+                const uint16_t* q = reinterpret_cast<const uint16_t*>(p);
+                w[k] = (2 * k < n ? static_cast<uint32_t>(q[2 * k]) : 0u) |
+                       (2 * k + 1 < n ? static_cast<uint32_t>(q[2 * k + 1]) << 16 : 0u);
             }
         }
+#pragma unroll
+        for (int k = 0; k < kVecs; ++k) v[i][k] = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
+    }
+
+    // the codes of the lane's own block; *scale_byte gets its scale
+    __device__ __forceinline__ uint4 quantize(int lane, uint32_t* scale_byte) const {
+        uint32_t w[4][kVecs * 4], amax[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+#pragma unroll
+            for (int k = 0; k < kVecs; ++k) {
+                w[i][4 * k] = v[i][k].x;
+                w[i][4 * k + 1] = v[i][k].y;
+                w[i][4 * k + 2] = v[i][k].z;
+                w[i][4 * k + 3] = v[i][k].w;
+            }
+            uint32_t m = 0u;
+            if constexpr (T == kMxF32) {
+#pragma unroll
+                for (int k = 0; k < 8; ++k) m = max(m, w[i][k] & 0x7fffffffu);
+            } else {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) m = max_u16x2(m, w[i][k] & 0x7fff7fffu);
+                m = max(m & 0xffffu, m >> 16);
+            }
+            m = max(m, quad_perm<kQuadXor1>(m));
+            amax[i] = max(m, quad_perm<kQuadXor2>(m));
+        }
+        // every lane works out its own block's scale and hands it to the four that convert the block
+        const int s = lane & 3;
+        const uint32_t own = s & 2 ? (s & 1 ? amax[3] : amax[2]) : (s & 1 ? amax[1] : amax[0]);
+        *scale_byte = mx_scale_byte(T == kMxF32    ? bits_f32(own)
+                                    : T == kMxBf16 ? bits_f32(own << 16)
+                                                   : half_bits_to_f32(static_cast<uint16_t>(own)));
+        const uint32_t scale = f32_bits(mx_scale_f32(*scale_byte));
+        const float by[4] = {bits_f32(quad_perm<kQuadLane[0]>(scale)), bits_f32(quad_perm<kQuadLane[1]>(scale)),
+                             bits_f32(quad_perm<kQuadLane[2]>(scale)), bits_f32(quad_perm<kQuadLane[3]>(scale))};
+        uint32_t o[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            uint32_t c = 0u;
+            if constexpr (T == kMxF32) {
+                c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, bits_f32(w[i][0]), bits_f32(w[i][1]), by[i], 0);
+                c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, bits_f32(w[i][2]), bits_f32(w[i][3]), by[i], 1);
+                c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, bits_f32(w[i][4]), bits_f32(w[i][5]), by[i], 2);
+                c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, bits_f32(w[i][6]), bits_f32(w[i][7]), by[i], 3);
+            } else if constexpr (T == kMxBf16) {
+                c = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(c, __builtin_bit_cast(bf16x2_t, w[i][0]), by[i], 0);
+                c = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(c, __builtin_bit_cast(bf16x2_t, w[i][1]), by[i], 1);
+                c = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(c, __builtin_bit_cast(bf16x2_t, w[i][2]), by[i], 2);
+                c = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(c, __builtin_bit_cast(bf16x2_t, w[i][3]), by[i], 3);
+            } else {
+                c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(c, __builtin_bit_cast(f16x2_t, w[i][0]), by[i], 0);
+                c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(c, __builtin_bit_cast(f16x2_t, w[i][1]), by[i], 1);
+                c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(c, __builtin_bit_cast(f16x2_t, w[i][2]), by[i], 2);
+                c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(c, __builtin_bit_cast(f16x2_t, w[i][3]), by[i], 3);
+            }
+            o[i] = c;
+        }
+        quad_transpose(o, lane);
         return make_uint4(o[0], o[1], o[2], o[3]);
     }
 };
@@ -190,15 +231,12 @@ struct MxMmArgs {
 constexpr int kMxPacked = 3;
 constexpr size_t kMxCounterBytes = 65536;
 
-// What a product's call runs: few-row kernel (tile 0) or an LDS tile, and its K split.
-struct MxPlan {
-    int tile;
-    int ksplit;
-    size_t ws_bytes;
-};
-MxPlan mx_rows_plan(int64_t M, int64_t N, int64_t K);
-MxPlan mx_tile_plan(int64_t M, int64_t N, int64_t K);
-bool mx_takes_rows(int64_t M, int64_t N, int64_t K, int a_type);
+// Few rows (mxfp4_rows.hip; 16-bit activations if their rows are within reach of 32-bit offsets), or
+// LDS tiles (mxfp4_mm.hip): packed activations. Workspace bytes: 0 for none.
+constexpr int64_t kMxFewRows = 32;
+inline bool mx_rows_in_reach(int64_t M, int64_t stride) { return M <= 1 || (M - 1) * stride <= (int64_t(1) << 29); }
+size_t mx_rows_workspace(int64_t M, int64_t N, int64_t K);
+size_t mx_tiles_workspace(int64_t M, int64_t N, int64_t K);
 int mx_mm_rows(const MxMmArgs& p, hipStream_t stream);
 int mx_mm_tiles(const MxMmArgs& p, hipStream_t stream);
 

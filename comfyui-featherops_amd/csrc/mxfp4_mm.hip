@@ -38,7 +38,7 @@ struct TileArgs {
     const uint8_t* bs;
     const uint16_t* bias;
     uint16_t* c;
-    int64_t M;
+    int64_t M, ldc;  // rows of this launch, elements between rows of c
     int N, ksteps, a_groups, b_groups;
     int tiles_m, tiles_n, ksplit, group_m;
     uint32_t* counters;
@@ -58,7 +58,7 @@ struct TileArgs {
 // of its fragment registers under this stage's MFMAs. Copies past the last step
 // repeat it, so the wait counts are constants.
 template <int BM, int BN, int WM, int WN, int kStages, bool kBf16>
-__global__ __launch_bounds__(64 * WM * WN, WM * WN == 4 ? 1 : 2) void mx_tile_kernel(const TileArgs p) {
+__global__ __launch_bounds__(64 * WM * WN, 2) void mx_tile_kernel(const TileArgs p) {
     constexpr int kWaves = WM * WN;
     constexpr int TM = BM / WM, TN = BN / WN;  // wave tile
     constexpr int FM = TM / 16, FN = TN / 16;  // its fragments
@@ -118,9 +118,10 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN == 4 ? 1 : 2) void mx_tile_ke
         src[kCodes + i] = (is_a ? p.as : p.bs) + (g * p.ksteps + k0) * 256;
         dst[kCodes + i] = lds + kScaleBase + j * 256;
     }
-    auto copy = [&](auto i, int step, int slot) {
-        if constexpr (i < kCodes) dma16_lds(src[i] + static_cast<int64_t>(step) * 1024, lane * 16, dst[i] + slot * kStageBytes);
-        else dma4_lds(src[i] + static_cast<int64_t>(step) * 256, lane * 4, dst[i] + slot * kStageBytes);
+    // (the step in the lane's offset, one instruction for all copies, not in each copy's address)
+    auto copy = [&](auto i, int step, int slot_bytes) {
+        if constexpr (i < kCodes) dma16_lds(src[i], lane * 16 + step * 1024, dst[i] + slot_bytes);
+        else dma4_lds(src[i], lane * 4 + step * 256, dst[i] + slot_bytes);
     };
 
     struct Frags {
@@ -156,22 +157,24 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN == 4 ? 1 : 2) void mx_tile_ke
     };
 
 #pragma unroll
-    for (int s = 0; s < kStages; ++s) unrolled<kPerWave>([&](auto i) { copy(i, min(s, steps - 1), s); });
+    for (int s = 0; s < kStages - 1; ++s) unrolled<kPerWave>([&](auto i) { copy(i, min(s, steps - 1), s * kStageBytes); });
     Frags f0, f1;
-    wait_vmcnt<(kStages - 1) * kPerWave>();
+    wait_vmcnt<(kStages - 2) * kPerWave>();
     stage_barrier();
     unrolled<kReads>([&](auto r) { read(r, f0, smem); });
-    int slot = 0;  // of the step being multiplied
+    int slot = 0;  // of the step being multiplied, in bytes as are the others
     // One step. The copies and the next step's reads are pinned between the MFMAs, all of them in the
     // first three quarters: left alone, the compiler reads each fragment into the registers of the one
     // just used up, after its last MFMA, and every step waits for LDS with the matrix cores idle.
     constexpr int kMfmas = FM * FN, kOps = kPerWave + kReads, kOver = kMfmas >= 8 ? kMfmas * 3 / 4 : kMfmas;
     auto iterate = [&](int k, const Frags& now, Frags& next) {
-        const int after = slot + 1 == kStages ? 0 : slot + 1;
-        const int ahead = min(k + kStages, steps - 1);
-        const uint8_t* base = smem + after * kStageBytes;
-        // stage k + 1 has landed; this wave's reads of stage k are done
-        wait_vmcnt_lgkm0<(kStages - 2) * kPerWave>();
+        const int after = slot == (kStages - 1) * kStageBytes ? 0 : slot + kStageBytes;
+        const int free_slot = slot == 0 ? (kStages - 1) * kStageBytes : slot - kStageBytes;
+        const int ahead = min(k + kStages - 1, steps - 1);
+        const uint8_t* base = smem + after;
+        // Stage k + 1 has landed; the buffer of stage k - 1 is free: the MFMAs of that step, which are
+        // issued, waited for its reads. The reads of stage k may still be under way.
+        wait_vmcnt<(kStages - 3) * kPerWave>();
         stage_barrier();
         unrolled<kMfmas>([&](auto n) {
             multiply(n, now);
@@ -179,7 +182,7 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN == 4 ? 1 : 2) void mx_tile_ke
             unrolled<last - first>([&](auto o) {
                 // the copies in even steps among the reads
                 constexpr int op = first + o, copies = (op + 1) * kPerWave / kOps, before = op * kPerWave / kOps;
-                if constexpr (copies > before) copy(std::integral_constant<int, before>{}, ahead, slot);
+                if constexpr (copies > before) copy(std::integral_constant<int, before>{}, ahead, free_slot);
                 else read(std::integral_constant<int, op - before>{}, next, base);
             });
             __builtin_amdgcn_sched_barrier(0);
@@ -267,7 +270,7 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN == 4 ? 1 : 2) void mx_tile_ke
                 v[2 + e] = r[1];
             }
             if (m >= p.M || n >= p.N) return;
-            uint16_t* c = p.c + m * p.N + n;
+            uint16_t* c = p.c + m * p.ldc + n;
             if (n + 8 <= p.N) {
                 __builtin_memcpy(c, v, 16);
             } else {
@@ -281,13 +284,93 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN == 4 ? 1 : 2) void mx_tile_ke
 
 struct Tile {
     int bm, bn;
+    int per_cu;   // workgroups a CU holds
+    double base;  // us of a launch with next to no K
+    double lo, one, two, three;  // us per K step: few workgroups, one, two, three on every CU
 };
-// ids 1.. of the plan
-constexpr Tile kTiles[] = {{0, 0}, {64, 64}, {64, 128}, {128, 128}, {256, 256}, {256, 256}, {128, 256}, {256, 128}, {128, 128}, {128, 256}, {64, 64}, {64, 128}, {256, 192}};
+// Tiles of the plan (ids 1..) and their measured times: MI355X, packed operands, weights from HBM,
+// M 64 .. 32768, N 2317 .. 13824, K 640 .. 14336. Small tiles fill the chip where there are few rows;
+// large ones read each operand fewer times (a CU takes ~50 GB/s per tile from beyond its L2 whatever the
+// ring's depth), and at 256 x 256 the matrix cores are the bound.
+constexpr Tile kTiles[] = {
+    {0, 0, 0, 0, 0, 0, 0, 0},
+    {64, 64, 3, 3.2, 0.15, 0.20, 0.29, 0.345},
+    {64, 128, 2, 3.7, 0.16, 0.23, 0.37, 0},
+    {128, 128, 2, 4.5, 0.27, 0.36, 0.58, 0},
+    {128, 256, 1, 5.4, 0.38, 0.57, 0, 0},
+    {256, 256, 1, 6.7, 0.55, 0.93, 0, 0},
+};
+constexpr int kNumTiles = 6, kLargest = 5;
+constexpr int kCus = 256;
 
-int tile_env() {
-    const char* e = getenv("FEATHEROPS_MX_TILE");
-    return e ? atoi(e) : 0;
+int64_t tiles_of(int64_t n, int t) { return (n + t - 1) / t; }
+
+// Time of `wgs` workgroups of a tile, `steps` K steps each.
+double tile_time(const Tile& t, int64_t wgs, double steps) {
+    const int64_t slots = static_cast<int64_t>(kCus) * t.per_cu;
+    const double full = t.per_cu == 3 ? t.three : t.per_cu == 2 ? t.two : t.one;
+    double time = static_cast<double>(wgs / slots) * full * steps;
+    const int64_t rest = wgs % slots;
+    if (rest > 2 * kCus) time += t.three * steps;
+    else if (rest > kCus) time += t.two * steps;
+    else if (rest > 0) time += (t.lo + (t.one - t.lo) * static_cast<double>(rest) / kCus) * steps;
+    return t.base + time;
+}
+
+// The fastest tile and K split for (M, N) on its own.
+struct Choice {
+    int tile, ksplit;
+    double time;
+};
+Choice choose(int64_t M, int64_t N, int64_t ksteps) {
+    Choice best{1, 1, 1e30};
+    for (int id = 1; id < kNumTiles; ++id) {
+        const Tile& t = kTiles[id];
+        const int64_t tiles = tiles_of(M, t.bm) * tiles_of(N, t.bn);
+        for (int ks : {1, 2, 3, 4, 6, 8}) {
+            // a split leaves every part eight steps or more, and keeps to one round of workgroups (and the
+            // arrival counters' 64 KB); it costs the exchange of the partial sums
+            if (ks > 1 && (ksteps / ks < 8 || tiles * ks > kCus * t.per_cu)) break;
+            double time = tile_time(t, tiles * ks, static_cast<double>((ksteps + ks - 1) / ks));
+            if (ks > 1) time += 0.8 + static_cast<double>(tiles * ks) * t.bm * t.bn * 8 / 5e6;
+            if (time < best.time) best = {id, ks, time};
+        }
+    }
+    return best;
+}
+
+size_t split_bytes(int64_t M, int64_t N, const Choice& c) {
+    if (c.ksplit == 1) return 0;
+    const Tile& t = kTiles[c.tile];
+    return kMxCounterBytes + static_cast<size_t>(tiles_of(M, t.bm) * tiles_of(N, t.bn)) * c.ksplit * t.bm * t.bn * 4;
+}
+
+// The plan: one tile for the whole result, or whole rounds of the largest tile for its first columns (or
+// rows) and the tile that suits the rest, where those would leave most of the chip idle in a last round.
+struct Plan {
+    int64_t m1, n1;  // the second part starts at row m1 or column n1 (the other is 0); both 0: one part
+    Choice first, rest;
+};
+Plan make_plan(int64_t M, int64_t N, int64_t ksteps) {
+    Plan best{0, 0, choose(M, N, ksteps), {}};
+    const Tile& t = kTiles[kLargest];
+    const int64_t tm = tiles_of(M, t.bm), tn = tiles_of(N, t.bn);
+    const int64_t whole = tm * tn / kCus * kCus;
+    if (whole == 0 || whole == tm * tn) return best;
+    double time = best.first.time;
+    for (int by_rows = 0; by_rows < 2; ++by_rows) {
+        const int64_t lines = by_rows ? whole / tn : whole / tm;
+        if (lines == 0) continue;
+        const int64_t m1 = by_rows ? lines * t.bm : 0, n1 = by_rows ? 0 : lines * t.bn;
+        if (m1 >= M || n1 >= N) continue;
+        const Choice first{kLargest, 1, tile_time(t, lines * (by_rows ? tn : tm), static_cast<double>(ksteps))};
+        const Choice rest = choose(M - m1, N - n1, ksteps);
+        if (first.time + rest.time < time) {
+            time = first.time + rest.time;
+            best = {m1, n1, first, rest};
+        }
+    }
+    return best;
 }
 
 template <int BM, int BN, int WM, int WN, int kStages>
@@ -297,48 +380,41 @@ void launch(const TileArgs& a, bool bf16, hipStream_t stream) {
     else mx_tile_kernel<BM, BN, WM, WN, kStages, false><<<grid, 64 * WM * WN, 0, stream>>>(a);
 }
 
-}  // namespace
-
-MxPlan mx_tile_plan(int64_t M, int64_t N, int64_t K) {
-    const int64_t ksteps = mx_ksteps(K);
-    int tile = 4;
-    auto count = [&](int t) { return ((M + kTiles[t].bm - 1) / kTiles[t].bm) * ((N + kTiles[t].bn - 1) / kTiles[t].bn); };
-    while (tile > 1 && count(tile) < 200) --tile;
-    if (tile_env()) tile = tile_env();
-    int ksplit = 1;
-    const char* ks = getenv("FEATHEROPS_MX_KS");
-    const int64_t tiles = count(tile);
-    if (tiles < 128) ksplit = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(256 / tiles, ksteps / 4)));
-    if (ks && atoi(ks)) ksplit = atoi(ks);
-    size_t ws = 0;
-    if (ksplit > 1) ws = kMxCounterBytes + static_cast<size_t>(tiles) * ksplit * kTiles[tile].bm * kTiles[tile].bn * 4;
-    return {tile, ksplit, ws};
-}
-
-int mx_mm_tiles(const MxMmArgs& p, hipStream_t stream) {
-    MxPlan plan = mx_tile_plan(p.M, p.N, p.K);
-    if (plan.ws_bytes > p.ws_bytes) plan.ksplit = 1;
-    const Tile t = kTiles[plan.tile];
-    const int64_t tiles_m = (p.M + t.bm - 1) / t.bm, tiles_n = (p.N + t.bn - 1) / t.bn;
-    if (tiles_m * tiles_n * plan.ksplit > (int64_t(1) << 22)) return FEATHER_ERR_UNSUPPORTED;
-    const TileArgs a{p.a, p.a_scales, p.b, p.b_scales, p.bias, p.c, p.M, p.N, static_cast<int>(mx_ksteps(p.K)),
-                     static_cast<int>(mx_groups(p.M)), static_cast<int>(mx_groups(p.N)), static_cast<int>(tiles_m),
-                     static_cast<int>(tiles_n), plan.ksplit, 4, reinterpret_cast<uint32_t*>(p.ws),
-                     reinterpret_cast<float*>(p.ws + kMxCounterBytes)};
-    switch (plan.tile) {
+// Rows [m0, M) and columns [n0, N) of the product.
+int run(const MxMmArgs& p, Choice c, int64_t m0, int64_t n0, int64_t M, int64_t N, hipStream_t stream) {
+    const Tile& t = kTiles[c.tile];
+    if (split_bytes(M - m0, N - n0, c) > p.ws_bytes) c.ksplit = 1;
+    const int64_t tiles_m = tiles_of(M - m0, t.bm), tiles_n = tiles_of(N - n0, t.bn), ksteps = mx_ksteps(p.K);
+    if (tiles_m * tiles_n > (int64_t(1) << 22)) return FEATHER_ERR_UNSUPPORTED;
+    const int64_t a_skip = m0 / 64 * ksteps, b_skip = n0 / 64 * ksteps;
+    const TileArgs a{p.a + a_skip * 4096, p.a_scales + a_skip * 256, p.b + b_skip * 4096, p.b_scales + b_skip * 256,
+                     p.bias ? p.bias + n0 : nullptr, p.c + m0 * p.N + n0, M - m0, p.N, static_cast<int>(N - n0),
+                     static_cast<int>(ksteps), static_cast<int>(mx_groups(p.M) - m0 / 64),
+                     static_cast<int>(mx_groups(p.N) - n0 / 64), static_cast<int>(tiles_m), static_cast<int>(tiles_n),
+                     c.ksplit, 4, reinterpret_cast<uint32_t*>(p.ws), reinterpret_cast<float*>(p.ws + kMxCounterBytes)};
+    switch (c.tile) {
         case 1: launch<64, 64, 2, 2, 6>(a, p.out_bf16, stream); break;
         case 2: launch<64, 128, 2, 2, 6>(a, p.out_bf16, stream); break;
-        case 3: launch<128, 128, 2, 2, 5>(a, p.out_bf16, stream); break;
-        case 5: launch<256, 256, 2, 2, 4>(a, p.out_bf16, stream); break;
-        case 6: launch<128, 256, 2, 2, 5>(a, p.out_bf16, stream); break;
-        case 7: launch<256, 128, 2, 2, 5>(a, p.out_bf16, stream); break;
-        case 8: launch<128, 128, 2, 4, 8>(a, p.out_bf16, stream); break;
-        case 9: launch<128, 256, 2, 4, 5>(a, p.out_bf16, stream); break;
-        case 10: launch<64, 64, 2, 2, 12>(a, p.out_bf16, stream); break;
-        case 11: launch<64, 128, 2, 2, 12>(a, p.out_bf16, stream); break;
+        case 3: launch<128, 128, 2, 2, 4>(a, p.out_bf16, stream); break;
+        case 4: launch<128, 256, 2, 4, 6>(a, p.out_bf16, stream); break;
         default: launch<256, 256, 4, 2, 4>(a, p.out_bf16, stream); break;
     }
     return hipGetLastError() == hipSuccess ? FEATHER_OK : FEATHER_ERR_LAUNCH;
+}
+
+}  // namespace
+
+size_t mx_tiles_workspace(int64_t M, int64_t N, int64_t K) {
+    const Plan plan = make_plan(M, N, mx_ksteps(K));
+    if (!plan.m1 && !plan.n1) return split_bytes(M, N, plan.first);
+    return split_bytes(M - plan.m1, N - plan.n1, plan.rest);
+}
+
+int mx_mm_tiles(const MxMmArgs& p, hipStream_t stream) {
+    const Plan plan = make_plan(p.M, p.N, mx_ksteps(p.K));
+    if (!plan.m1 && !plan.n1) return run(p, plan.first, 0, 0, p.M, p.N, stream);
+    const int st = run(p, plan.first, 0, 0, plan.m1 ? plan.m1 : p.M, plan.n1 ? plan.n1 : p.N, stream);
+    return st == FEATHER_OK ? run(p, plan.rest, plan.m1, plan.n1, p.M, p.N, stream) : st;
 }
 
 }  // namespace feather

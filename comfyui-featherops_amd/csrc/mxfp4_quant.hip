@@ -3,10 +3,9 @@
 //
 // All four kernels give one wave a group of 64 rows and one step of 128 columns:
 // lane l has row l % 16 of each of the group's four row tiles and the block of 32
-// columns l / 16, the packed layout's own order, so a block's maximum needs no
-// other lane, codes leave as whole KBs and the four tiles' scales as one dword
-// per lane. The row-major side is read (written) in runs of 256 bytes per row
-// (16-bit values). HBM bound.
+// columns l / 16, the packed layout's own order, so codes leave as whole KBs and the
+// four tiles' scales as one dword per lane. Values are read and written four lanes to
+// a block (MxPieces). HBM bound.
 #include "featherops_amd.h"
 #include "mxfp4.h"
 
@@ -34,11 +33,9 @@ struct WaveTask {
         return ((group * 4 + f) * ksteps + step) * 1024 + lane * 16;
     }
     __device__ __forceinline__ int64_t scale_at(int ksteps) const { return (group * ksteps + step) * 256 + lane * 4; }
-    // how many of the lane's 32 columns exist
-    __device__ __forceinline__ int count(int cols) const {
-        const int n = cols - step * kMxStepK - kb * kMxBlock;
-        return n < 0 ? 0 : n > kMxBlock ? kMxBlock : n;
-    }
+    // the first column of the lane's pieces, and how many of their 8 values exist
+    __device__ __forceinline__ int col() const { return step * kMxStepK + mx_piece_col(lane); }
+    __device__ __forceinline__ int count(int cols) const { return max(0, min(8, cols - col())); }
 };
 
 template <int T>
@@ -49,21 +46,36 @@ __global__ __launch_bounds__(64 * kWavesPerBlock) void quantize_kernel(const uin
                                                                        int64_t groups) {
     const WaveTask t(groups, ksteps);
     if (!t.ok) return;
-    const int n = t.count(cols);
-    MxRaw<T> raw[4];
-#pragma unroll
-    for (int f = 0; f < 4; ++f) {
-        const int64_t row = t.row(f);
-        const int64_t at = row * row_bytes + (static_cast<int64_t>(t.step) * kMxStepK + t.kb * kMxBlock) * kMxElemBytes<T>;
-        raw[f].load(x + at, row < rows ? n : 0);
-    }
+    const uint8_t* at = x + static_cast<int64_t>(t.col()) * kMxElemBytes<T>;
+    // rows past the last repeat it: nothing reads what their place in the operand holds
+    auto row = [&](int f, int i) { return min(t.group * 64 + f * 16 + mx_piece_row(t.lane, i), rows - 1) * row_bytes; };
+    const int tiles = static_cast<int>(min(static_cast<int64_t>(4), (rows - t.group * 64 + 15) / 16));
+    const bool whole = (t.step + 1) * kMxStepK <= cols;
+    MxPieces<T> v[4];
     uint32_t bytes = 0u;
+    if (tiles == 4 && whole) {  // (the same for the whole wave) every load in flight at once
 #pragma unroll
-    for (int f = 0; f < 4; ++f) {
-        uint32_t s;
-        const uint4 q = raw[f].quantize(&s);
-        *reinterpret_cast<uint4*>(codes + t.code_at(f, ksteps)) = q;
-        bytes |= s << (8 * f);
+        for (int f = 0; f < 4; ++f)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[f].load(i, at + row(f, i));
+#pragma unroll
+        for (int f = 0; f < 4; ++f) {
+            uint32_t s;
+            *reinterpret_cast<uint4*>(codes + t.code_at(f, ksteps)) = v[f].quantize(t.lane, &s);
+            bytes |= s << (8 * f);
+        }
+    } else {
+        const int n = t.count(cols);
+        for (int f = 0; f < tiles; ++f) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (whole) v[0].load(i, at + row(f, i));
+                else v[0].load_part(i, at + row(f, i), n);
+            }
+            uint32_t s;
+            *reinterpret_cast<uint4*>(codes + t.code_at(f, ksteps)) = v[0].quantize(t.lane, &s);
+            bytes |= s << (8 * f);
+        }
     }
     *reinterpret_cast<uint32_t*>(scales + t.scale_at(ksteps)) = bytes;
 }
@@ -81,45 +93,42 @@ __global__ __launch_bounds__(64 * kWavesPerBlock) void dequantize_kernel(const u
                                                                          int cols, int ksteps, int64_t groups) {
     const WaveTask t(groups, ksteps);
     if (!t.ok) return;
-    const int n = t.count(cols);
-    if (n == 0) return;
     const uint32_t bytes = *reinterpret_cast<const uint32_t*>(scales + t.scale_at(ksteps));
     uint4 q[4];
 #pragma unroll
     for (int f = 0; f < 4; ++f) q[f] = *reinterpret_cast<const uint4*>(codes + t.code_at(f, ksteps));
+    const int n = t.count(cols);
 #pragma unroll
     for (int f = 0; f < 4; ++f) {
-        const int64_t row = t.row(f);
-        if (row >= rows) continue;
         const uint32_t sb = (bytes >> (8 * f)) & 255u;
-        const float s = sb == 255u ? bits_f32(0x7fc00000u) : mx_scale_f32(sb);
-        const uint32_t w[4] = {q[f].x, q[f].y, q[f].z, q[f].w};
-        float v[32];
+        const uint32_t scale = sb == 255u ? 0x7fc00000u : f32_bits(mx_scale_f32(sb));
+        const float by[4] = {bits_f32(quad_perm<kQuadLane[0]>(scale)), bits_f32(quad_perm<kQuadLane[1]>(scale)),
+                             bits_f32(quad_perm<kQuadLane[2]>(scale)), bits_f32(quad_perm<kQuadLane[3]>(scale))};
+        uint32_t w[4] = {q[f].x, q[f].y, q[f].z, q[f].w};
+        quad_transpose(w, t.lane);  // piece i: 8 codes of the block of lane 4 (l / 4) + i
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const f32x2_t a = codes_to_f32<0>(w[i], s), b = codes_to_f32<1>(w[i], s);
-            const f32x2_t c = codes_to_f32<2>(w[i], s), d = codes_to_f32<3>(w[i], s);
-            v[8 * i] = a[0], v[8 * i + 1] = a[1], v[8 * i + 2] = b[0], v[8 * i + 3] = b[1];
-            v[8 * i + 4] = c[0], v[8 * i + 5] = c[1], v[8 * i + 6] = d[0], v[8 * i + 7] = d[1];
-        }
-        uint8_t* o = out + (row * cols + static_cast<int64_t>(t.step) * kMxStepK + t.kb * kMxBlock) * kMxElemBytes<T>;
-        if (n == kMxBlock) {
+            const int64_t row = t.group * 64 + f * 16 + mx_piece_row(t.lane, i);
+            if (row >= rows || n == 0) continue;
+            const f32x2_t a = codes_to_f32<0>(w[i], by[i]), b = codes_to_f32<1>(w[i], by[i]);
+            const f32x2_t c = codes_to_f32<2>(w[i], by[i]), d = codes_to_f32<3>(w[i], by[i]);
+            const float v[8] = {a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+            uint32_t r[MxPieces<T>::kVecs * 4];
 #pragma unroll
-            for (int i = 0; i < MxRaw<T>::kVecs; ++i) {
-                uint32_t r[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    if constexpr (T == kMxF32) r[j] = f32_bits(v[4 * i + j]);
-                    else r[j] = f32x2_to_out_bits<T == kMxBf16>(v[8 * i + 2 * j], v[8 * i + 2 * j + 1]);
-                }
-                __builtin_memcpy(o + 16 * i, r, 16);
+            for (int k = 0; k < MxPieces<T>::kVecs * 4; ++k) {
+                if constexpr (T == kMxF32) r[k] = f32_bits(v[k]);
+                else r[k] = f32x2_to_out_bits<T == kMxBf16>(v[2 * k], v[2 * k + 1]);
             }
-        } else {
+            uint8_t* o = out + (row * cols + t.col()) * kMxElemBytes<T>;
+            if (n == 8) {
+                __builtin_memcpy(o, r, sizeof(r));
+            } else {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-                if (i >= n) continue;
-                if constexpr (T == kMxF32) reinterpret_cast<float*>(o)[i] = v[i];
-                else reinterpret_cast<uint16_t*>(o)[i] = f32_to_out_bits<T == kMxBf16>(v[i]);
+                for (int k = 0; k < 8; ++k) {
+                    if (k >= n) continue;
+                    if constexpr (T == kMxF32) reinterpret_cast<uint32_t*>(o)[k] = r[k];
+                    else reinterpret_cast<uint16_t*>(o)[k] = static_cast<uint16_t>(r[k >> 1] >> (16 * (k & 1)));
+                }
             }
         }
     }

@@ -1,9 +1,8 @@
 // The MXFP4 product for few rows: C (M, N) = q(A) . B^T + bias, where the call is
 // bound by streaming the weight once. 16-bit activations are quantised on the way
-// into the matrix instruction: lane l of the operand holds one block of 32 values of
-// row l % 16, so its scale and codes need no other lane and cost ~50 instructions
-// beside the 2 KB or more of weights the wave waits for; a launch of its own for
-// the quantisation would cost more than the whole product of one token.
+// into the matrix instruction (MxPieces: ~85 instructions a K step, beside the 1 to 4 KB of
+// weights that the wave waits for); a launch of its own for the quantisation would cost
+// more than that of one token's product.
 #include <algorithm>
 #include <type_traits>
 #include <utility>
@@ -28,7 +27,7 @@ __device__ __forceinline__ void unrolled(F&& f) {
 struct RowsArgs {
     const uint8_t* a;
     const uint8_t* as;
-    int64_t a_row_bytes;
+    int a_row_bytes;
     const uint8_t* b;
     const uint8_t* bs;
     const uint16_t* bias;
@@ -42,7 +41,7 @@ struct RowsArgs {
 // One step's operands of a wave: A fragments (packed, or as 16-bit values) and B fragments.
 template <int MT, int NT, int AT>
 struct Step {
-    std::conditional_t<AT == kMxPacked, uint4, MxRaw<AT == kMxBf16 ? kMxBf16 : kMxF16>> a[MT];
+    std::conditional_t<AT == kMxPacked, uint4, MxPieces<AT == kMxBf16 ? kMxBf16 : kMxF16>> a[MT];
     uint32_t as, bs;
     uint4 b[NT];
 };
@@ -52,13 +51,11 @@ struct Step {
 // through LDS in wave order. ksplit > 1: several workgroups share a strip's steps.
 template <int MT, int NT, int AT, bool kBf16>
 __global__ __launch_bounds__(64 * kWaves) void mx_rows_kernel(const RowsArgs p) {
-    constexpr int kDepth = 3;
+    constexpr int kDepth = 2;
     __shared__ __attribute__((aligned(16))) f32x4 red[kWaves][MT * NT][64];
     const int tid = threadIdx.x;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int lane = tid & 63;
-    const int lr = lane & 15;
-    const int kb = lane >> 4;
 
     // an XCD's workgroups take neighbouring strips: up to four share their scales' cache lines
     const int total = p.strips * p.ksplit;
@@ -72,29 +69,55 @@ __global__ __launch_bounds__(64 * kWaves) void mx_rows_kernel(const RowsArgs p) 
     const int k1 = static_cast<int>(static_cast<int64_t>(p.ksteps) * (q + 1) / p.ksplit);
 
     const int64_t tile0 = static_cast<int64_t>(strip) * NT;
-    const uint8_t* b = p.b + tile0 * p.ksteps * 1024 + lane * 16;
-    const uint8_t* bs = p.bs + (tile0 / 4) * p.ksteps * 256 + lane * 4;
     const int bshift = 8 * static_cast<int>(tile0 % 4);
     typedef Step<MT, NT, AT> S;
-    auto load = [&](S& s, int k) {
+    // Operands come through buffer descriptors: a step past the wave's last one reads nothing, so the loop
+    // has no branch around loads, where the compiler would wait for all of those in flight.
+    const __amdgpu_buffer_rsrc_t bres = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<uint8_t*>(p.b + tile0 * p.ksteps * 1024), 0, NT * p.ksteps * 1024, 0x00020000);
+    const __amdgpu_buffer_rsrc_t bsres = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<uint8_t*>(p.bs + (tile0 / 4) * p.ksteps * 256), 0, p.ksteps * 256, 0x00020000);
+    const __amdgpu_buffer_rsrc_t ares = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<uint8_t*>(p.a), 0, AT == kMxPacked ? MT * p.ksteps * 1024 : (p.M - 1) * p.a_row_bytes + p.K * 2, 0x00020000);
+    const __amdgpu_buffer_rsrc_t asres = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<uint8_t*>(AT == kMxPacked ? p.as : p.a), 0, AT == kMxPacked ? p.ksteps * 256 : 0, 0x00020000);
+    constexpr uint32_t kNone = 0x80000000u;  // an offset past every descriptor's end
+    uint32_t arow[MT][AT == kMxPacked ? 1 : 4];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
         if constexpr (AT == kMxPacked) {
+            arow[i][0] = i * p.ksteps * 1024 + lane * 16;
+        } else {  // rows past the last repeat it (their results are not stored)
 #pragma unroll
-            for (int i = 0; i < MT; ++i)
-                s.a[i] = *reinterpret_cast<const uint4*>(p.a + (static_cast<int64_t>(i) * p.ksteps + k) * 1024 + lane * 16);
-            s.as = *reinterpret_cast<const uint32_t*>(p.as + static_cast<int64_t>(k) * 256 + lane * 4);
-        } else {
-            const int col = k * kMxStepK + kb * kMxBlock;
-            const int n = max(0, min(kMxBlock, p.K - col));
-#pragma unroll
-            for (int i = 0; i < MT; ++i) {
-                const int row = i * 16 + lr;
-                s.a[i].load(p.a + row * p.a_row_bytes + static_cast<int64_t>(col) * 2, row < p.M ? n : 0);
-            }
+            for (int v = 0; v < 4; ++v)
+                arow[i][v] = min(i * 16 + mx_piece_row(lane, v), p.M - 1) * p.a_row_bytes + mx_piece_col(lane) * 2;
         }
+    }
+    auto load_b = [&](S& s, int k, bool have) {
 #pragma unroll
         for (int j = 0; j < NT; ++j)
-            s.b[j] = *reinterpret_cast<const uint4*>(b + (static_cast<int64_t>(j) * p.ksteps + k) * 1024);
-        s.bs = *reinterpret_cast<const uint32_t*>(bs + static_cast<int64_t>(k) * 256);
+            s.b[j] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(
+                                                   bres, have ? (j * p.ksteps + k) * 1024 + lane * 16 : kNone, 0, 0));
+        s.bs = __builtin_amdgcn_raw_buffer_load_b32(bsres, have ? k * 256 + lane * 4 : kNone, 0, 0);
+    };
+    // a step that ends within K
+    auto load = [&](S& s, int k, bool have) {
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            if constexpr (AT == kMxPacked) {
+                s.a[i] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(ares, have ? arow[i][0] + k * 1024 : kNone, 0, 0));
+            } else {
+#pragma unroll
+                for (int v = 0; v < 4; ++v)
+                    s.a[i].v[v][0] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(
+                                                                   ares, have ? arow[i][v] + k * (kMxStepK * 2) : kNone, 0, 0));
+            }
+        }
+        if constexpr (AT == kMxPacked) s.as = __builtin_amdgcn_raw_buffer_load_b32(asres, have ? k * 256 + lane * 4 : kNone, 0, 0);
+        load_b(s, k, have);
+        // the loads start here, not where the compiler would move them: beside their use, a step later
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
     };
     f32x4 acc[MT][NT];
 #pragma unroll
@@ -111,24 +134,37 @@ __global__ __launch_bounds__(64 * kWaves) void mx_rows_kernel(const RowsArgs p) 
                 a = s.a[i];
                 ascale = s.as;
             } else {
-                a = s.a[i].quantize(&ascale);
+                a = s.a[i].quantize(lane, &ascale);
             }
             unrolled<NT>([&](auto j) { acc[i][j] = mfma_mx<j, kByte>(s.b[j], a, acc[i][j], bscale, ascale); });
         });
     };
 
-    S buf[kDepth];
+    const int whole = AT == kMxPacked ? k1 : min(k1, p.K / kMxStepK);  // steps before this one end within K
+    const int first = k0 + wave;
+    if (first < whole) {
+        S buf[kDepth];
 #pragma unroll
-    for (int d = 0; d < kDepth; ++d)
-        if (k0 + wave + d * kWaves < k1) load(buf[d], k0 + wave + d * kWaves);
-    for (int k = k0 + wave; k < k1; k += kDepth * kWaves) {
+        for (int d = 0; d < kDepth; ++d) load(buf[d], first + d * kWaves, first + d * kWaves < whole);
+        for (int k = first; k < whole; k += kDepth * kWaves) {
 #pragma unroll
-        for (int d = 0; d < kDepth; ++d) {
-            const int kd = k + d * kWaves;
-            if (kd < k1) {
-                multiply(buf[d]);
-                if (kd + kDepth * kWaves < k1) load(buf[d], kd + kDepth * kWaves);
+            for (int d = 0; d < kDepth; ++d) {
+                if (k + d * kWaves < whole) multiply(buf[d]);
+                const int next = k + (kDepth + d) * kWaves;
+                load(buf[d], next, next < whole);
             }
+        }
+    }
+    if constexpr (AT != kMxPacked) {
+        if (whole < k1 && (whole - k0) % kWaves == wave) {
+            S tail;
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int v = 0; v < 4; ++v)
+                    tail.a[i].load_part(v, p.a + arow[i][v] + whole * (kMxStepK * 2), max(0, min(8, p.K - whole * kMxStepK - mx_piece_col(lane))));
+            load_b(tail, whole, true);
+            multiply(tail);
         }
     }
 #pragma unroll
@@ -207,35 +243,47 @@ void launch(const RowsArgs& a, int a_type, bool bf16, hipStream_t stream) {
     else go(std::integral_constant<int, kMxF16>{});
 }
 
-}  // namespace
+// Column tiles of a strip, and workgroups that share one's K steps.
+struct RowsPlan {
+    int nt;
+    int64_t strips, ksplit;
+    size_t ws_bytes;
+};
 
-// tile: the strip's column tiles
-MxPlan mx_rows_plan(int64_t M, int64_t N, int64_t K) {
-    const int64_t ksteps = mx_ksteps(K);
-    const int64_t tiles = (N + 15) / 16;
-    int nt = 4;
-    while (nt > 1 && (tiles + nt - 1) / nt < 256) nt /= 2;
-    const int64_t strips = (tiles + nt - 1) / nt;
-    int64_t ksplit = 1;
-    if (strips < 160) ksplit = std::max<int64_t>(1, std::min<int64_t>(256 / strips, ksteps / kWaves));
-    const int64_t mt = (M + 15) / 16;
-    size_t ws = 0;
-    if (ksplit > 1) ws = kMxCounterBytes + static_cast<size_t>(strips) * ksplit * mt * nt * 1024;
-    return {nt, static_cast<int>(ksplit), ws};
+// Strips as narrow as one round of workgroups allows, up to four tiles (us with one row and the weight
+// in HBM: N=5120 K=5120 in strips of 16 / 32 / 64 columns 9.5 / 7.0 / 8.5, N=13824 16.2 / 11.9 / 10.1,
+// N=K=4096 with 16 rows 5.9 / 6.0 / 6.8); K split where strips leave half of the CUs idle and every
+// wave keeps two steps (N=512 K=14336 9.6 -> 7.0 in four).
+RowsPlan rows_plan(int64_t M, int64_t N, int64_t K) {
+    const int64_t ksteps = mx_ksteps(K), tiles = (N + 15) / 16;
+    RowsPlan p;
+    p.nt = 1;
+    while (p.nt < 4 && (tiles + p.nt - 1) / p.nt > 256) p.nt *= 2;
+    p.strips = (tiles + p.nt - 1) / p.nt;
+    p.ksplit = std::max<int64_t>(1, std::min<int64_t>(128 / p.strips, ksteps / (2 * kWaves)));
+    p.ws_bytes = p.ksplit > 1 ? kMxCounterBytes + static_cast<size_t>(p.strips * p.ksplit * p.nt) * (M <= 16 ? 1024 : 2048) : 0;
+    return p;
 }
 
-bool mx_takes_rows(int64_t M, int64_t N, int64_t K, int a_type) { return M <= 16; }
+}  // namespace
+
+size_t mx_rows_workspace(int64_t M, int64_t N, int64_t K) { return rows_plan(M, N, K).ws_bytes; }
 
 int mx_mm_rows(const MxMmArgs& p, hipStream_t stream) {
-    MxPlan plan = mx_rows_plan(p.M, p.N, p.K);
+    if (p.a_type != kMxPacked && !mx_rows_in_reach(p.M, p.a_stride)) return FEATHER_ERR_UNSUPPORTED;
+    RowsPlan plan = rows_plan(p.M, p.N, p.K);
     if (plan.ws_bytes > p.ws_bytes) plan.ksplit = 1;
-    const int nt = plan.tile;
-    const RowsArgs a{p.a, p.a_scales, p.a_stride * 2, p.b, p.b_scales, p.bias, p.c, static_cast<int>(p.M), p.N, p.K,
-                     static_cast<int>(mx_ksteps(p.K)), static_cast<int>(((p.N + 15) / 16 + nt - 1) / nt), plan.ksplit,
-                     reinterpret_cast<uint32_t*>(p.ws), reinterpret_cast<float*>(p.ws + kMxCounterBytes)};
-    if (nt == 4) launch<1, 4>(a, p.a_type, p.out_bf16, stream);
-    else if (nt == 2) launch<1, 2>(a, p.a_type, p.out_bf16, stream);
-    else launch<1, 1>(a, p.a_type, p.out_bf16, stream);
+    const RowsArgs a{p.a, p.a_scales, p.M > 1 ? static_cast<int>(p.a_stride * 2) : 0, p.b, p.b_scales, p.bias, p.c,
+                     static_cast<int>(p.M), p.N, p.K, static_cast<int>(mx_ksteps(p.K)), static_cast<int>(plan.strips),
+                     static_cast<int>(plan.ksplit), reinterpret_cast<uint32_t*>(p.ws),
+                     reinterpret_cast<float*>(p.ws + kMxCounterBytes)};
+    auto by_strip = [&](auto mt) {
+        if (plan.nt == 4) launch<mt, 4>(a, p.a_type, p.out_bf16, stream);
+        else if (plan.nt == 2) launch<mt, 2>(a, p.a_type, p.out_bf16, stream);
+        else launch<mt, 1>(a, p.a_type, p.out_bf16, stream);
+    };
+    if (p.M <= 16) by_strip(std::integral_constant<int, 1>{});
+    else by_strip(std::integral_constant<int, 2>{});
     return hipGetLastError() == hipSuccess ? FEATHER_OK : FEATHER_ERR_LAUNCH;
 }
 

@@ -172,7 +172,7 @@ at::Tensor mxfp4_mm(const at::Tensor& a, const at::Tensor& b_codes, const at::Te
     const c10::DeviceGuard guard(a.device());
     const at::Tensor r = as_rows(a);
     const int code = a.scalar_type() == at::kHalf ? FEATHER_DTYPE_F16 : FEATHER_DTYPE_BF16;
-    if (feather_mxfp4_mm_takes_16bit(M, N, K))
+    if (feather_mxfp4_mm_takes_16bit(M, N, K, r.stride(0)))
         return run_mm(r.data_ptr(), nullptr, code, r.stride(0), b_codes, b_scales, bias, M, N, K, out_dtype);
     const Packed q = empty_packed(M, K, a);
     check_status(feather_mxfp4_quantize(r.data_ptr(), code, M, K, r.stride(0), bytes_out(q.codes), bytes_out(q.scales),

@@ -357,15 +357,16 @@ int feather_mxfp4_unprepack(const uint8_t* codes, const uint8_t* scales, uint8_t
  *   a_dtype FEATHER_DTYPE_MXFP4: a and a_scales are A (M, K) in the packed form.
  *   a_dtype F16 / BF16: a holds A's values, a_row_stride elements between rows, and
  *     is quantised on the way (the values of feather_mxfp4_quantize); a_scales is
- *     not read. Served where feather_mxfp4_mm_takes_16bit says so (few rows),
- *     FEATHER_ERR_UNSUPPORTED elsewhere: the caller quantises A and calls again.
+ *     not read. Served where feather_mxfp4_mm_takes_16bit says so (few rows, at most
+ *     2^29 elements from the first to the last), FEATHER_ERR_UNSUPPORTED elsewhere:
+ *     the caller quantises A and calls again.
  *   b, b_scales: B (N, K) in the packed form. bias: (N,) of the output type, or NULL.
  * Any M >= 0, N >= 1, K >= 1; c is contiguous, at any alignment of its type.
  * Workspace: the size below, the contract of feather_launch_scaled_mm_ws (its first
  * 64 KB zero before the first use and left zero); with less, K is not split and the
  * sums run in another order.
  */
-int feather_mxfp4_mm_takes_16bit(int64_t M, int64_t N, int64_t K);
+int feather_mxfp4_mm_takes_16bit(int64_t M, int64_t N, int64_t K, int64_t a_row_stride);
 size_t feather_mxfp4_mm_workspace_size(int64_t M, int64_t N, int64_t K, int a_dtype);
 int feather_mxfp4_mm(const void* a, const uint8_t* a_scales, int a_dtype, int64_t a_row_stride, const uint8_t* b,
                      const uint8_t* b_scales, const uint16_t* bias, uint16_t* c, int64_t M, int64_t N, int64_t K,

@@ -57,7 +57,8 @@ def test_c_entries_refuse_without_launching(lib):
     ]
     assert bad == [1] * len(bad)
     # more 16-bit rows than the product quantises itself
-    assert not lib.feather_mxfp4_mm_takes_16bit(4096, 4096, 4096)
+    assert not lib.feather_mxfp4_mm_takes_16bit(4096, 4096, 4096, 4096)
+    assert lib.feather_mxfp4_mm_takes_16bit(4, 4096, 4096, 1 << 27) and not lib.feather_mxfp4_mm_takes_16bit(4, 4096, 4096, 1 << 28)
     assert lib.feather_mxfp4_mm(P, None, 1, 4096, P, P, None, P, 4096, 4096, 4096, 1, None, 0, None) == 2
     # nothing to do
     assert lib.feather_mxfp4_quantize(None, 0, 0, 64, 64, None, None, None) == 0
