@@ -101,10 +101,12 @@ int feather_block_norm(const feather_block_norm_args* p, hipStream_t stream) {
     if (!p->x || (p->h && !p->x_out) || (!p->h && (p->gate || p->post_weight)) || (p->gate && p->gate_group <= 0) ||
         ((p->scale || p->shift) && p->mod_group <= 0) || (to_codes ? !p->codes || !p->scales || p->y : !p->y))
         return FEATHER_ERR_INVALID;
-    const NormArgs a{p->x, p->x_row_stride, p->h, p->h_row_stride, p->gate, p->gate_group, p->gate_row_stride, p->scale,
-                     p->mod_group, p->scale_row_stride, p->shift, p->shift_row_stride, p->post_weight, p->weight,
-                     p->bias, p->x_out, p->y, p->codes, p->scales, p->rows, static_cast<int>(p->cols), p->x_dtype,
-                     p->y_dtype, p->mod_dtype == FEATHER_DTYPE_F32, p->norm, p->eps, p->residual_scale};
+    auto group = [&](int64_t g) { return static_cast<uint32_t>(g < p->rows ? g : p->rows); };
+    const NormArgs a{p->x, p->x_row_stride, p->h, p->h_row_stride, p->gate, p->gate_row_stride, p->scale,
+                     p->scale_row_stride, p->shift, p->shift_row_stride, p->post_weight, p->weight, p->bias, p->x_out,
+                     p->y, p->codes, p->scales, group(p->gate_group), group(p->mod_group), p->rows,
+                     static_cast<int>(p->cols), p->x_dtype, p->y_dtype, p->mod_dtype == FEATHER_DTYPE_F32, p->norm,
+                     p->eps, p->residual_scale};
     return block_norm(a, stream);
 }
 

@@ -17,9 +17,9 @@ struct NormArgs {
     int64_t h_stride;
     // vectors of mod_f32 ? fp32 : y_type values; each may be null
     const void* gate;   // row r reads gate + r / gate_group * gate_stride
-    int64_t gate_group, gate_stride;
+    int64_t gate_stride;
     const void* scale;  // row r reads scale + r / mod_group * scale_stride
-    int64_t mod_group, scale_stride;
+    int64_t scale_stride;
     const void* shift;
     int64_t shift_stride;
     const void* post_weight;  // (cols,): h is normalised and weighted before the gate
@@ -29,7 +29,8 @@ struct NormArgs {
     void* y;                  // (rows, cols), y_type; null: codes and scales
     uint8_t* codes;           // packed MXFP4 operand
     uint8_t* scales;
-    int64_t rows;
+    uint32_t gate_group, mod_group;  // at most `rows`
+    int64_t rows;                    // below 2^31
     int cols;
     int x_type, y_type, mod_f32;  // MxType codes
     int layer;                    // 0: root mean square, 1: mean and variance

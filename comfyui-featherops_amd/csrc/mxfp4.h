@@ -65,6 +65,14 @@ __device__ __forceinline__ uint4 load16_unaligned(const void* p) {
     return v;
 }
 
+// Two fp32 -> fp16 or bf16 packed (a in the low half), round to nearest even: one instruction (a NaN keeps
+// its payload, where f32x2_to_out_bits makes a bf16 one canonical with six more).
+template <bool kBf16>
+__device__ __forceinline__ uint32_t mx_round_pair(float a, float b) {
+    if constexpr (kBf16) return f32x2_to_bf16x2_raw(a, b);
+    else return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2_t{a, b}, f16x2_t));
+}
+
 enum MxType { kMxF16 = 0, kMxBf16 = 1, kMxF32 = 2 };
 template <int T>
 constexpr int kMxElemBytes = T == kMxF32 ? 4 : 2;

@@ -261,7 +261,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mx_tile_kernel(const TileArgs
             for (int f = 0; f < 2; ++f)
 #pragma unroll
                 for (int e = 0; e < 2; ++e)
-                    o[f][e] = f32x2_to_out_bits<kBf16>(acc[i][j + f][2 * e] + bias[f][2 * e], acc[i][j + f][2 * e + 1] + bias[f][2 * e + 1]);
+                    o[f][e] = mx_round_pair<kBf16>(acc[i][j + f][2 * e] + bias[f][2 * e], acc[i][j + f][2 * e + 1] + bias[f][2 * e + 1]);
             uint32_t v[4];
 #pragma unroll
             for (int e = 0; e < 2; ++e) {

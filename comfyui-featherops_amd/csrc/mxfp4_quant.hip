@@ -117,7 +117,7 @@ __global__ __launch_bounds__(64 * kWavesPerBlock) void dequantize_kernel(const u
 #pragma unroll
             for (int k = 0; k < MxPieces<T>::kVecs * 4; ++k) {
                 if constexpr (T == kMxF32) r[k] = f32_bits(v[k]);
-                else r[k] = f32x2_to_out_bits<T == kMxBf16>(v[2 * k], v[2 * k + 1]);
+                else r[k] = mx_round_pair<T == kMxBf16>(v[2 * k], v[2 * k + 1]);
             }
             uint8_t* o = out + (row * cols + t.col()) * kMxElemBytes<T>;
             if (n == 8) {

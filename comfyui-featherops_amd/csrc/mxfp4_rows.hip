@@ -221,7 +221,7 @@ __global__ __launch_bounds__(64 * kWaves) void mx_rows_kernel(const RowsArgs p) 
             for (int i = 0; i < 4; ++i)
                 if (i < have) sum[i] += out_bits_to_f32<kBf16>(p.bias[n + i]);
         }
-        const uint32_t o[2] = {f32x2_to_out_bits<kBf16>(sum[0], sum[1]), f32x2_to_out_bits<kBf16>(sum[2], sum[3])};
+        const uint32_t o[2] = {mx_round_pair<kBf16>(sum[0], sum[1]), mx_round_pair<kBf16>(sum[2], sum[3])};
         uint16_t* c = p.c + static_cast<int64_t>(m) * p.N + n;
         if (have == 4) {
             __builtin_memcpy(c, o, 8);

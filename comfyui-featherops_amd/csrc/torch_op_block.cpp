@@ -38,12 +38,20 @@ int value_code(at::ScalarType t, const char* what) {
     return -1;
 }
 
-// t as (rows, cols) with contiguous rows, one stride between them; a view where t allows one.
-at::Tensor as_rows(const at::Tensor& t) {
+// t as rows of `cols` contiguous values with one stride between them: in place where its strides
+// allow, otherwise a copy. (A contiguous tensor, the usual case, costs no view.)
+struct Rows {
+    at::Tensor t;  // keeps the values alive until the launch
+    const void* p = nullptr;
+    int64_t n = 0, stride = 0;
+};
+
+Rows as_rows(const at::Tensor& t) {
     const int64_t cols = t.size(-1);
+    if (t.is_contiguous()) return {t, t.data_ptr(), cols ? t.numel() / cols : 0, cols};
     at::Tensor r = t.dim() == 2 ? t : t.reshape({cols ? t.numel() / cols : 0, cols});
     if ((cols > 1 && r.stride(1) != 1) || (r.size(0) > 1 && r.stride(0) < 0)) r = r.contiguous();
-    return r;
+    return {r, r.data_ptr(), r.size(0), r.stride(0)};
 }
 
 struct Packed {
@@ -81,10 +89,10 @@ std::tuple<at::Tensor, at::Tensor> quantize_mxfp4(const at::Tensor& x) {
     TORCH_CHECK(x.dim() >= 1 && x.size(-1) >= 1, "x must have at least one column");
     const int code = value_code(x.scalar_type(), "x");
     const c10::DeviceGuard guard(x.device());
-    const at::Tensor r = as_rows(x);
-    const int64_t rows = r.size(0), cols = r.size(1);
+    const Rows r = as_rows(x);
+    const int64_t rows = r.n, cols = x.size(-1);
     const Packed q = empty_packed(rows, cols, x);
-    check_status(feather_mxfp4_quantize(r.data_ptr(), code, rows, cols, r.stride(0), bytes_out(q.codes),
+    check_status(feather_mxfp4_quantize(r.p, code, rows, cols, r.stride, bytes_out(q.codes),
                                         bytes_out(q.scales), stream_of(x)),
                  "quantize_mxfp4");
     return {q.codes, q.scales};
@@ -170,12 +178,12 @@ at::Tensor mxfp4_mm(const at::Tensor& a, const at::Tensor& b_codes, const at::Te
     check_packed(b_codes, b_scales, N, K, "b");
     check_mm_out(bias, a.device(), N, out_dtype);
     const c10::DeviceGuard guard(a.device());
-    const at::Tensor r = as_rows(a);
+    const Rows r = as_rows(a);
     const int code = a.scalar_type() == at::kHalf ? FEATHER_DTYPE_F16 : FEATHER_DTYPE_BF16;
-    if (feather_mxfp4_mm_takes_16bit(M, N, K, r.stride(0)))
-        return run_mm(r.data_ptr(), nullptr, code, r.stride(0), b_codes, b_scales, bias, M, N, K, out_dtype);
+    if (feather_mxfp4_mm_takes_16bit(M, N, K, r.stride))
+        return run_mm(r.p, nullptr, code, r.stride, b_codes, b_scales, bias, M, N, K, out_dtype);
     const Packed q = empty_packed(M, K, a);
-    check_status(feather_mxfp4_quantize(r.data_ptr(), code, M, K, r.stride(0), bytes_out(q.codes), bytes_out(q.scales),
+    check_status(feather_mxfp4_quantize(r.p, code, M, K, r.stride, bytes_out(q.codes), bytes_out(q.scales),
                                         stream_of(a)),
                  "mxfp4_mm");
     return run_mm(q.codes.data_ptr(), bytes(q.scales), FEATHER_DTYPE_MXFP4, 0, b_codes, b_scales, bias, M, N, K, out_dtype);
@@ -199,13 +207,13 @@ at::Tensor mxfp4_mm_packed(const at::Tensor& a_codes, const at::Tensor& a_scales
 // share a row of t are consecutive unless t repeats along a leading dimension alone, in which
 // case it is written out.
 struct RowVectors {
-    at::Tensor t;  // keeps a copy alive until the launch
+    Rows rows;
     const void* p = nullptr;
     int64_t group = 1, stride = 0;
 };
 
 RowVectors row_vectors(const at::Tensor& x, const at::Tensor& t, at::ScalarType dtype, const char* what) {
-    const int64_t cols = x.size(-1), rows = x.numel() / cols;
+    const int64_t cols = x.size(-1);
     TORCH_CHECK(t.device() == x.device(), what, " must be on the same device as x");
     value_code(t.scalar_type(), what);
     TORCH_CHECK(t.dim() >= 1 && t.size(-1) == cols && t.dim() <= x.dim(), what, " must end in x's ", cols,
@@ -219,15 +227,13 @@ RowVectors row_vectors(const at::Tensor& x, const at::Tensor& t, at::ScalarType 
         TORCH_CHECK(n == x.size(j) || n == 1, what, " must broadcast against x");
         whole = whole && n == x.size(j);
     }
-    RowVectors r;
-    r.t = whole ? t : t.expand(x.sizes());
     if (!whole) group = 1;
-    r.t = as_rows(r.t);
-    if (r.t.scalar_type() != dtype) r.t = r.t.to(dtype);
-    r.p = r.t.data_ptr();
+    RowVectors r;
+    r.rows = t.scalar_type() == dtype ? as_rows(whole ? t : t.expand(x.sizes()))
+                                      : as_rows((whole ? t : t.expand(x.sizes())).to(dtype));
+    r.p = r.rows.p;
     r.group = group > 0 ? group : 1;
-    r.stride = r.t.size(0) > 1 ? r.t.stride(0) : 0;
-    if (rows == 0) r.stride = 0;
+    r.stride = r.rows.n > 1 ? r.rows.stride : 0;
     return r;
 }
 
@@ -265,10 +271,10 @@ NormOut run_norm(const at::Tensor& x, const OptTensor& h, const OptTensor& gate,
         if (t->has_value() && (*t)->scalar_type() != block) mods = at::kFloat;
 
     const c10::DeviceGuard guard(x.device());
-    const at::Tensor xr = as_rows(x);
-    at::Tensor hr, pw, w, b;
+    const Rows xr = as_rows(x);
+    const Rows hr = h.has_value() ? as_rows(*h) : Rows{};
+    at::Tensor pw, w, b;
     RowVectors g, sc, sh;
-    if (h.has_value()) hr = as_rows(*h);
     if (gate.has_value()) g = row_vectors(x, *gate, mods, "gate");
     if (scale.has_value()) sc = row_vectors(x, *scale, mods, "scale");
     if (shift.has_value()) sh = row_vectors(x, *shift, mods, "shift");
@@ -285,8 +291,8 @@ NormOut run_norm(const at::Tensor& x, const OptTensor& h, const OptTensor& gate,
     if (codes) out.q = empty_packed(rows, cols, x);
     else out.y = at::empty(x.sizes(), x.options().dtype(block));
     feather_block_norm_args a{};
-    a.x = xr.data_ptr();
-    a.h = h.has_value() ? hr.data_ptr() : nullptr;
+    a.x = xr.p;
+    a.h = hr.p;
     a.gate = g.p;
     a.post_weight = pw.defined() ? pw.data_ptr() : nullptr;
     a.weight = w.defined() ? w.data_ptr() : nullptr;
@@ -299,8 +305,8 @@ NormOut run_norm(const at::Tensor& x, const OptTensor& h, const OptTensor& gate,
     a.scales = codes ? bytes_out(out.q.scales) : nullptr;
     a.rows = rows;
     a.cols = cols;
-    a.x_row_stride = xr.stride(0);
-    a.h_row_stride = h.has_value() ? hr.stride(0) : 0;
+    a.x_row_stride = xr.stride;
+    a.h_row_stride = hr.stride;
     a.gate_group = g.group;
     a.gate_row_stride = g.stride;
     a.mod_group = scale.has_value() ? sc.group : sh.group;

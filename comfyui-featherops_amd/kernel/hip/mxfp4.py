@@ -58,8 +58,9 @@ def quantize_mxfp4(x: torch.Tensor) -> MXFP4Tensor:
 
 def dequantize_mxfp4(q: MXFP4Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """The values that q stands for, each rounded once to dtype (fp16, bf16 or fp32)."""
-    y = _dequantize(q.codes, q.scales, q.rows, q.cols, dtype)
-    return y if len(q.shape) == 2 else y.view(q.shape)
+    if len(q.shape) == 2:
+        return _dequantize(q.codes, q.scales, *q.shape, dtype)
+    return _dequantize(q.codes, q.scales, q.rows, q.cols, dtype).view(q.shape)
 
 
 def prepack_mxfp4(codes: torch.Tensor, scales: torch.Tensor, cols: int | None = None) -> MXFP4Tensor:
