@@ -120,8 +120,37 @@ struct MxPieces {
 #pragma unroll
         for (int k = 0; k < kVecs; ++k) v[i][k] = load16_unaligned(p + 16 * k);
     }
-    // piece i: its values [0, n), zeros beyond
-    __device__ __forceinline__ void load_part(int i, const uint8_t* p, int n) {
+    // piece i, from column col on, of a row that ends within or before it and has cols >= 8 values: loaded
+    // to end with the row and moved into place, zeros beyond
+    __device__ __forceinline__ void load_end(int i, const uint8_t* row, int col, int cols) {
+        const int from = min(col, cols - 8);
+        load(i, row + from * kMxElemBytes<T>);
+        const int by = col - from;
+        if constexpr (T == kMxF32) {
+            uint32_t w[8] = {v[i][0].x, v[i][0].y, v[i][0].z, v[i][0].w, v[i][1].x, v[i][1].y, v[i][1].z, v[i][1].w};
+#pragma unroll
+            for (int s = 4; s >= 1; s /= 2)
+#pragma unroll
+                for (int k = 0; k < 8; ++k) w[k] = by & s ? (k + s < 8 ? w[k + s] : 0u) : w[k];
+            v[i][0] = make_uint4(w[0], w[1], w[2], w[3]);
+            v[i][1] = make_uint4(w[4], w[5], w[6], w[7]);
+        } else {
+            uint32_t w[4] = {v[i][0].x, v[i][0].y, v[i][0].z, v[i][0].w};
+#pragma unroll
+            for (int s = 2; s >= 1; s /= 2)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) w[k] = by & (2 * s) ? (k + s < 4 ? w[k + s] : 0u) : w[k];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) w[k] = by & 1 ? (w[k] >> 16) | (k < 3 ? w[k + 1] << 16 : 0u) : w[k];
+            v[i][0] = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        if (by >= 8) {
+#pragma unroll
+            for (int k = 0; k < kVecs; ++k) v[i][k] = make_uint4(0u, 0u, 0u, 0u);
+        }
+    }
+    // the same for a row of fewer than 8 values: the n from p on
+    __device__ __forceinline__ void load_few(int i, const uint8_t* p, int n) {
         uint32_t w[kVecs * 4];
 #pragma unroll
         for (int k = 0; k < kVecs * 4; ++k) {

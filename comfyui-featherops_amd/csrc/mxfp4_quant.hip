@@ -6,6 +6,8 @@
 // columns l / 16, the packed layout's own order, so codes leave as whole KBs and the
 // four tiles' scales as one dword per lane. Values are read and written four lanes to
 // a block (MxPieces). HBM bound.
+#include <type_traits>
+
 #include "featherops_amd.h"
 #include "mxfp4.h"
 
@@ -38,46 +40,49 @@ struct WaveTask {
     __device__ __forceinline__ int count(int cols) const { return max(0, min(8, cols - col())); }
 };
 
-template <int T>
+// kTiles: row tiles of a wave, all four of a group where there are many rows, one where waves would be too
+// few to fill the chip (us, 154 x 4096 in bf16: ONE_US against FOUR_US).
+template <int T, int kTiles>
 __global__ __launch_bounds__(64 * kWavesPerBlock) void quantize_kernel(const uint8_t* __restrict__ x, int64_t rows,
                                                                        int cols, int64_t row_bytes,
                                                                        uint8_t* __restrict__ codes,
                                                                        uint8_t* __restrict__ scales, int ksteps,
-                                                                       int64_t groups) {
-    const WaveTask t(groups, ksteps);
-    if (!t.ok) return;
-    const uint8_t* at = x + static_cast<int64_t>(t.col()) * kMxElemBytes<T>;
+                                                                       int64_t units) {
+    const int64_t w = static_cast<int64_t>(blockIdx.x) * kWavesPerBlock + (threadIdx.x >> 6);
+    if (w >= units * ksteps) return;
+    const int64_t unit = w / ksteps;  // kTiles row tiles
+    const int step = static_cast<int>(w - unit * ksteps);
+    const int lane = threadIdx.x & 63;
+    const int64_t row0 = unit * (16 * kTiles);
+    const int col = step * kMxStepK + mx_piece_col(lane);
     // rows past the last repeat it: nothing reads what their place in the operand holds
-    auto row = [&](int f, int i) { return min(t.group * 64 + f * 16 + mx_piece_row(t.lane, i), rows - 1) * row_bytes; };
-    const int tiles = static_cast<int>(min(static_cast<int64_t>(4), (rows - t.group * 64 + 15) / 16));
-    const bool whole = (t.step + 1) * kMxStepK <= cols;
-    MxPieces<T> v[4];
-    uint32_t bytes = 0u;
-    if (tiles == 4 && whole) {  // (the same for the whole wave) every load in flight at once
+    auto row = [&](int f, int i) { return x + min(row0 + f * 16 + mx_piece_row(lane, i), rows - 1) * row_bytes; };
+    MxPieces<T> v[kTiles];
+    if ((step + 1) * kMxStepK <= cols) {  // (the same for the whole wave) every load in flight at once
 #pragma unroll
-        for (int f = 0; f < 4; ++f)
+        for (int f = 0; f < kTiles; ++f)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[f].load(i, at + row(f, i));
+            for (int i = 0; i < 4; ++i) v[f].load(i, row(f, i) + static_cast<int64_t>(col) * kMxElemBytes<T>);
+    } else if (cols >= 8) {
 #pragma unroll
-        for (int f = 0; f < 4; ++f) {
-            uint32_t s;
-            *reinterpret_cast<uint4*>(codes + t.code_at(f, ksteps)) = v[f].quantize(t.lane, &s);
-            bytes |= s << (8 * f);
-        }
+        for (int f = 0; f < kTiles; ++f)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[f].load_end(i, row(f, i), col, cols);
     } else {
-        const int n = t.count(cols);
-        for (int f = 0; f < tiles; ++f) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if (whole) v[0].load(i, at + row(f, i));
-                else v[0].load_part(i, at + row(f, i), n);
-            }
-            uint32_t s;
-            *reinterpret_cast<uint4*>(codes + t.code_at(f, ksteps)) = v[0].quantize(t.lane, &s);
-            bytes |= s << (8 * f);
-        }
+        for (int f = 0; f < kTiles; ++f)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[f].load_few(i, row(f, i), cols - col);
     }
-    *reinterpret_cast<uint32_t*>(scales + t.scale_at(ksteps)) = bytes;
+    uint32_t bytes = 0u;
+#pragma unroll
+    for (int f = 0; f < kTiles; ++f) {
+        uint32_t s;
+        *reinterpret_cast<uint4*>(codes + ((unit * kTiles + f) * ksteps + step) * 1024 + lane * 16) = v[f].quantize(lane, &s);
+        bytes |= s << (8 * f);
+    }
+    if constexpr (kTiles == 4) *reinterpret_cast<uint32_t*>(scales + (unit * ksteps + step) * 256 + lane * 4) = bytes;
+    else scales[((unit >> 2) * ksteps + step) * 256 + lane * 4 + (unit & 3)] = static_cast<uint8_t>(bytes);
 }
 
 // Two codes of byte `byte` of w as fp32, times the scale (NaN under scale 255).
@@ -184,15 +189,20 @@ int launched() { return hipGetLastError() == hipSuccess ? FEATHER_OK : FEATHER_E
 
 int mx_quantize(const void* x, int dtype, int64_t rows, int64_t cols, int64_t row_stride, uint8_t* codes,
                 uint8_t* scales, hipStream_t stream) {
-    const Grid g(rows, cols);
-    const uint8_t* xb = static_cast<const uint8_t*>(x);
-    const int c = static_cast<int>(cols);
-    if (dtype == kMxF16)
-        quantize_kernel<kMxF16><<<g.blocks, 64 * kWavesPerBlock, 0, stream>>>(xb, rows, c, row_stride * 2, codes, scales, g.ksteps, g.groups);
-    else if (dtype == kMxBf16)
-        quantize_kernel<kMxBf16><<<g.blocks, 64 * kWavesPerBlock, 0, stream>>>(xb, rows, c, row_stride * 2, codes, scales, g.ksteps, g.groups);
-    else
-        quantize_kernel<kMxF32><<<g.blocks, 64 * kWavesPerBlock, 0, stream>>>(xb, rows, c, row_stride * 4, codes, scales, g.ksteps, g.groups);
+    const int ksteps = static_cast<int>(mx_ksteps(cols));
+    auto go = [&](auto t, auto tiles) {
+        const int64_t units = (rows + 16 * tiles - 1) / (16 * tiles);
+        const unsigned blocks = static_cast<unsigned>((units * ksteps + kWavesPerBlock - 1) / kWavesPerBlock);
+        quantize_kernel<t, tiles><<<blocks, 64 * kWavesPerBlock, 0, stream>>>(
+            static_cast<const uint8_t*>(x), rows, static_cast<int>(cols), row_stride * kMxElemBytes<t>, codes, scales, ksteps, units);
+    };
+    auto by_rows = [&](auto t) {
+        if (mx_groups(rows) * ksteps < 2048) go(t, std::integral_constant<int, 1>{});
+        else go(t, std::integral_constant<int, 4>{});
+    };
+    if (dtype == kMxF16) by_rows(std::integral_constant<int, kMxF16>{});
+    else if (dtype == kMxBf16) by_rows(std::integral_constant<int, kMxBf16>{});
+    else by_rows(std::integral_constant<int, kMxF32>{});
     return launched();
 }
 

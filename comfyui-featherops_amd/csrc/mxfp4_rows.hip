@@ -161,8 +161,12 @@ __global__ __launch_bounds__(64 * kWaves) void mx_rows_kernel(const RowsArgs p) 
 #pragma unroll
             for (int i = 0; i < MT; ++i)
 #pragma unroll
-                for (int v = 0; v < 4; ++v)
-                    tail.a[i].load_part(v, p.a + arow[i][v] + whole * (kMxStepK * 2), max(0, min(8, p.K - whole * kMxStepK - mx_piece_col(lane))));
+                for (int v = 0; v < 4; ++v) {
+                    const int col = whole * kMxStepK + mx_piece_col(lane);
+                    const uint8_t* row = p.a + arow[i][v] - mx_piece_col(lane) * 2;
+                    if (p.K >= 8) tail.a[i].load_end(v, row, col, p.K);
+                    else tail.a[i].load_few(v, row + col * 2, p.K - col);
+                }
             load_b(tail, whole, true);
             multiply(tail);
         }

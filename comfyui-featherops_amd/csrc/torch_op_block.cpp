@@ -54,63 +54,70 @@ Rows as_rows(const at::Tensor& t) {
     return {r, r.data_ptr(), r.size(0), r.stride(0)};
 }
 
+// A packed operand is one uint8 tensor: its codes, then its scales (one allocation a call where two would
+// cost a microsecond more).
 struct Packed {
-    at::Tensor codes, scales;
+    at::Tensor data;
+    int64_t codes_bytes = 0;
+    uint8_t* codes() const { return static_cast<uint8_t*>(data.data_ptr()); }
+    uint8_t* scales() const { return codes() + codes_bytes; }
 };
 
+int64_t packed_units(int64_t rows, int64_t cols) { return (rows + 63) / 64 * ((cols + 127) / 128); }
+
 Packed empty_packed(int64_t rows, int64_t cols, const at::Tensor& like) {
-    const int64_t groups = (rows + 63) / 64, steps = (cols + 127) / 128;
-    const auto options = like.options().dtype(at::kByte);
-    return {at::empty({groups * 4, steps, 64, 16}, options), at::empty({groups, steps, 64, 4}, options)};
+    const int64_t units = packed_units(rows, cols);
+    return {at::empty({units * 4352}, like.options().dtype(at::kByte)), units * 4096};
 }
 
-// The packed form's shapes (see featherops_amd.h): messages name the operand.
-void check_packed(const at::Tensor& codes, const at::Tensor& scales, int64_t rows, int64_t cols, const char* what) {
-    TORCH_CHECK(codes.is_cuda() && scales.is_cuda(), what, " must be CUDA tensors");
-    TORCH_CHECK(codes.device() == scales.device(), what, " codes and scales must be on the same device");
-    TORCH_CHECK(codes.scalar_type() == at::kByte && scales.scalar_type() == at::kByte, what, " must be uint8");
-    const int64_t groups = (rows + 63) / 64, steps = (cols + 127) / 128;
-    TORCH_CHECK(codes.dim() == 4 && codes.size(0) == groups * 4 && codes.size(1) == steps && codes.size(2) == 64 &&
-                    codes.size(3) == 16 && scales.dim() == 4 && scales.size(0) == groups && scales.size(1) == steps &&
-                    scales.size(2) == 64 && scales.size(3) == 4,
-                what, " must be packed for (", rows, ", ", cols, "): codes (", groups * 4, ", ", steps,
-                ", 64, 16), scales (", groups, ", ", steps, ", 64, 4)");
-    TORCH_CHECK(codes.is_contiguous() && scales.is_contiguous(), what, " must be contiguous");
-    TORCH_CHECK(reinterpret_cast<uintptr_t>(codes.data_ptr()) % 16 == 0 &&
-                    reinterpret_cast<uintptr_t>(scales.data_ptr()) % 16 == 0,
-                what, " data pointers must be 16-byte aligned");
+Packed check_packed(const at::Tensor& data, int64_t rows, int64_t cols, const char* what) {
+    TORCH_CHECK(data.is_cuda(), what, " must be a CUDA tensor");
+    const int64_t units = packed_units(rows, cols);
+    TORCH_CHECK(data.scalar_type() == at::kByte && data.dim() == 1 && data.size(0) == units * 4352 && data.is_contiguous(),
+                what, " must be packed for (", rows, ", ", cols, "): ", units * 4352, " contiguous uint8");
+    TORCH_CHECK(reinterpret_cast<uintptr_t>(data.data_ptr()) % 16 == 0, what, " data pointer must be 16-byte aligned");
+    return {data, units * 4096};
+}
+
+int64_t rows_of(at::IntArrayRef shape) {
+    int64_t n = 1;
+    for (size_t i = 0; i + 1 < shape.size(); ++i) n *= shape[i];
+    return n;
+}
+// shape with its last dimension replaced
+at::DimVector with_last(at::IntArrayRef shape, int64_t n) {
+    at::DimVector v(shape.begin(), shape.end());
+    v.back() = n;
+    return v;
 }
 
 const uint8_t* bytes(const at::Tensor& t) { return static_cast<const uint8_t*>(t.data_ptr()); }
-uint8_t* bytes_out(const at::Tensor& t) { return static_cast<uint8_t*>(t.data_ptr()); }
 
-std::tuple<at::Tensor, at::Tensor> quantize_mxfp4(const at::Tensor& x) {
+at::Tensor quantize_mxfp4(const at::Tensor& x) {
     TORCH_CHECK(x.is_cuda(), "x must be a CUDA tensor");
     TORCH_CHECK(x.dim() >= 1 && x.size(-1) >= 1, "x must have at least one column");
     const int code = value_code(x.scalar_type(), "x");
     const c10::DeviceGuard guard(x.device());
     const Rows r = as_rows(x);
-    const int64_t rows = r.n, cols = x.size(-1);
-    const Packed q = empty_packed(rows, cols, x);
-    check_status(feather_mxfp4_quantize(r.p, code, rows, cols, r.stride, bytes_out(q.codes),
-                                        bytes_out(q.scales), stream_of(x)),
+    const Packed q = empty_packed(r.n, x.size(-1), x);
+    check_status(feather_mxfp4_quantize(r.p, code, r.n, x.size(-1), r.stride, q.codes(), q.scales(), stream_of(x)),
                  "quantize_mxfp4");
-    return {q.codes, q.scales};
+    return q.data;
 }
 
-at::Tensor dequantize_mxfp4(const at::Tensor& codes, const at::Tensor& scales, int64_t rows, int64_t cols,
-                            at::ScalarType dtype) {
-    TORCH_CHECK(rows >= 0 && cols >= 1, "rows must not be negative, cols must be positive");
-    check_packed(codes, scales, rows, cols, "q");
+at::Tensor dequantize_mxfp4(const at::Tensor& data, at::IntArrayRef shape, at::ScalarType dtype) {
+    TORCH_CHECK(!shape.empty() && shape.back() >= 1, "q must have at least one column");
+    const int64_t rows = rows_of(shape), cols = shape.back();
+    const Packed q = check_packed(data, rows, cols, "q");
     const int code = value_code(dtype, "dtype");
-    const c10::DeviceGuard guard(codes.device());
-    const at::Tensor out = at::empty({rows, cols}, codes.options().dtype(dtype));
-    check_status(feather_mxfp4_dequantize(bytes(codes), bytes(scales), out.data_ptr(), code, rows, cols, stream_of(codes)),
+    const c10::DeviceGuard guard(data.device());
+    const at::Tensor out = at::empty(shape, data.options().dtype(dtype));
+    check_status(feather_mxfp4_dequantize(q.codes(), q.scales(), out.data_ptr(), code, rows, cols, stream_of(data)),
                  "dequantize_mxfp4");
     return out;
 }
 
-std::tuple<at::Tensor, at::Tensor> prepack_mxfp4(const at::Tensor& codes, const at::Tensor& scales, int64_t cols) {
+at::Tensor prepack_mxfp4(const at::Tensor& codes, const at::Tensor& scales, int64_t cols) {
     TORCH_CHECK(codes.is_cuda() && scales.is_cuda(), "codes and scales must be CUDA tensors");
     TORCH_CHECK(codes.device() == scales.device(), "codes and scales must be on the same device");
     TORCH_CHECK(codes.element_size() == 1 && scales.element_size() == 1, "codes and scales must be 1-byte types");
@@ -120,22 +127,20 @@ std::tuple<at::Tensor, at::Tensor> prepack_mxfp4(const at::Tensor& codes, const 
                 "codes must be (rows, ", blocks * 16, ") and scales (rows, ", blocks, ") for ", cols, " columns");
     const c10::DeviceGuard guard(codes.device());
     const at::Tensor c = codes.contiguous(), s = scales.contiguous();
-    const int64_t rows = c.size(0);
-    const auto options = codes.options().dtype(at::kByte);
-    const Packed q = empty_packed(rows, cols, at::empty({0}, options));
-    check_status(feather_mxfp4_prepack(bytes(c), bytes(s), bytes_out(q.codes), bytes_out(q.scales), rows, cols, stream_of(c)),
+    const Packed q = empty_packed(c.size(0), cols, c);
+    check_status(feather_mxfp4_prepack(bytes(c), bytes(s), q.codes(), q.scales(), c.size(0), cols, stream_of(c)),
                  "prepack_mxfp4");
-    return {q.codes, q.scales};
+    return q.data;
 }
 
-std::tuple<at::Tensor, at::Tensor> unprepack_mxfp4(const at::Tensor& codes, const at::Tensor& scales, int64_t rows,
-                                                   int64_t cols) {
+std::tuple<at::Tensor, at::Tensor> unprepack_mxfp4(const at::Tensor& data, int64_t rows, int64_t cols) {
     TORCH_CHECK(rows >= 0 && cols >= 1, "rows must not be negative, cols must be positive");
-    check_packed(codes, scales, rows, cols, "q");
-    const c10::DeviceGuard guard(codes.device());
+    const Packed q = check_packed(data, rows, cols, "q");
+    const c10::DeviceGuard guard(data.device());
     const int64_t blocks = (cols + 31) / 32;
-    const at::Tensor c = at::empty({rows, blocks * 16}, codes.options()), s = at::empty({rows, blocks}, codes.options());
-    check_status(feather_mxfp4_unprepack(bytes(codes), bytes(scales), bytes_out(c), bytes_out(s), rows, cols, stream_of(codes)),
+    const at::Tensor c = at::empty({rows, blocks * 16}, data.options()), s = at::empty({rows, blocks}, data.options());
+    check_status(feather_mxfp4_unprepack(q.codes(), q.scales(), static_cast<uint8_t*>(c.data_ptr()),
+                                         static_cast<uint8_t*>(s.data_ptr()), rows, cols, stream_of(data)),
                  "unprepack_mxfp4");
     return {c, s};
 }
@@ -150,15 +155,16 @@ void check_mm_out(const OptTensor& bias, const at::Device& dev, int64_t N, at::S
     }
 }
 
-at::Tensor run_mm(const void* a, const uint8_t* a_scales, int a_dtype, int64_t a_stride, const at::Tensor& b_codes,
-                  const at::Tensor& b_scales, const OptTensor& bias, int64_t M, int64_t N, int64_t K,
-                  at::ScalarType out_dtype) {
-    const hipStream_t stream = stream_of(b_codes);
-    const at::Tensor c = at::empty({M, N}, b_codes.options().dtype(out_dtype));
+// C of the given shape (its leading dimensions are A's rows)
+at::Tensor run_mm(const void* a, const uint8_t* a_scales, int a_dtype, int64_t a_stride, const Packed& b,
+                  const OptTensor& bias, at::IntArrayRef shape, int64_t K, at::ScalarType out_dtype) {
+    const hipStream_t stream = stream_of(b.data);
+    const int64_t M = rows_of(shape), N = shape.back();
+    const at::Tensor c = at::empty(shape, b.data.options().dtype(out_dtype));
     const size_t ws_bytes = feather_mxfp4_mm_workspace_size(M, N, K, a_dtype);
     at::Tensor ws;
-    if (ws_bytes) ws = feather::workspace_for(b_codes.device(), stream, ws_bytes);
-    check_status(feather_mxfp4_mm(a, a_scales, a_dtype, a_stride, bytes(b_codes), bytes(b_scales),
+    if (ws_bytes) ws = feather::workspace_for(b.data.device(), stream, ws_bytes);
+    check_status(feather_mxfp4_mm(a, a_scales, a_dtype, a_stride, b.codes(), b.scales(),
                                   bias.has_value() ? static_cast<const uint16_t*>(bias->data_ptr()) : nullptr,
                                   static_cast<uint16_t*>(c.data_ptr()), M, N, K,
                                   out_dtype == at::kBFloat16 ? FEATHER_DTYPE_BF16 : FEATHER_DTYPE_F16,
@@ -167,38 +173,37 @@ at::Tensor run_mm(const void* a, const uint8_t* a_scales, int a_dtype, int64_t a
     return c;
 }
 
-at::Tensor mxfp4_mm(const at::Tensor& a, const at::Tensor& b_codes, const at::Tensor& b_scales, int64_t N,
-                    const OptTensor& bias, at::ScalarType out_dtype) {
+at::Tensor mxfp4_mm(const at::Tensor& a, const at::Tensor& b, int64_t N, int64_t K, const OptTensor& bias,
+                    std::optional<at::ScalarType> dtype) {
     TORCH_CHECK(a.is_cuda(), "a must be a CUDA tensor");
     TORCH_CHECK(a.scalar_type() == at::kHalf || a.scalar_type() == at::kBFloat16, "a must be float16 or bfloat16");
-    TORCH_CHECK(a.dim() == 2 && a.size(1) >= 1, "a must be 2D with at least one column");
-    TORCH_CHECK(N >= 1, "N must be positive");
-    TORCH_CHECK(b_codes.device() == a.device(), "b must be on the same device as a");
-    const int64_t M = a.size(0), K = a.size(1);
-    check_packed(b_codes, b_scales, N, K, "b");
+    TORCH_CHECK(N >= 1 && K >= 1, "b must have at least one row and one column");
+    TORCH_CHECK(a.dim() >= 1 && a.size(-1) == K, "a must have b's ", K, " columns");
+    TORCH_CHECK(b.device() == a.device(), "b must be on the same device as a");
+    const at::ScalarType out_dtype = dtype.value_or(a.scalar_type());
+    const Packed w = check_packed(b, N, K, "b");
     check_mm_out(bias, a.device(), N, out_dtype);
     const c10::DeviceGuard guard(a.device());
     const Rows r = as_rows(a);
+    const at::DimVector shape = with_last(a.sizes(), N);
     const int code = a.scalar_type() == at::kHalf ? FEATHER_DTYPE_F16 : FEATHER_DTYPE_BF16;
-    if (feather_mxfp4_mm_takes_16bit(M, N, K, r.stride))
-        return run_mm(r.p, nullptr, code, r.stride, b_codes, b_scales, bias, M, N, K, out_dtype);
-    const Packed q = empty_packed(M, K, a);
-    check_status(feather_mxfp4_quantize(r.p, code, M, K, r.stride, bytes_out(q.codes), bytes_out(q.scales),
-                                        stream_of(a)),
-                 "mxfp4_mm");
-    return run_mm(q.codes.data_ptr(), bytes(q.scales), FEATHER_DTYPE_MXFP4, 0, b_codes, b_scales, bias, M, N, K, out_dtype);
+    if (feather_mxfp4_mm_takes_16bit(r.n, N, K, r.stride))
+        return run_mm(r.p, nullptr, code, r.stride, w, bias, shape, K, out_dtype);
+    const Packed q = empty_packed(r.n, K, a);
+    check_status(feather_mxfp4_quantize(r.p, code, r.n, K, r.stride, q.codes(), q.scales(), stream_of(a)), "mxfp4_mm");
+    return run_mm(q.codes(), q.scales(), FEATHER_DTYPE_MXFP4, 0, w, bias, shape, K, out_dtype);
 }
 
-at::Tensor mxfp4_mm_packed(const at::Tensor& a_codes, const at::Tensor& a_scales, int64_t M, int64_t K,
-                           const at::Tensor& b_codes, const at::Tensor& b_scales, int64_t N, const OptTensor& bias,
-                           at::ScalarType out_dtype) {
-    TORCH_CHECK(M >= 0 && N >= 1 && K >= 1, "M must not be negative, N and K must be positive");
-    check_packed(a_codes, a_scales, M, K, "a");
-    check_packed(b_codes, b_scales, N, K, "b");
-    TORCH_CHECK(b_codes.device() == a_codes.device(), "b must be on the same device as a");
-    check_mm_out(bias, a_codes.device(), N, out_dtype);
-    const c10::DeviceGuard guard(a_codes.device());
-    return run_mm(a_codes.data_ptr(), bytes(a_scales), FEATHER_DTYPE_MXFP4, 0, b_codes, b_scales, bias, M, N, K, out_dtype);
+at::Tensor mxfp4_mm_packed(const at::Tensor& a, at::IntArrayRef a_shape, const at::Tensor& b, int64_t N, int64_t K,
+                           const OptTensor& bias, at::ScalarType out_dtype) {
+    TORCH_CHECK(N >= 1 && K >= 1, "b must have at least one row and one column");
+    TORCH_CHECK(!a_shape.empty() && a_shape.back() == K, "a must have b's ", K, " columns");
+    const Packed q = check_packed(a, rows_of(a_shape), K, "a");
+    const Packed w = check_packed(b, N, K, "b");
+    TORCH_CHECK(b.device() == a.device(), "b must be on the same device as a");
+    check_mm_out(bias, a.device(), N, out_dtype);
+    const c10::DeviceGuard guard(a.device());
+    return run_mm(q.codes(), q.scales(), FEATHER_DTYPE_MXFP4, 0, w, bias, with_last(a_shape, N), K, out_dtype);
 }
 
 // ---- norms ----
@@ -301,8 +306,8 @@ NormOut run_norm(const at::Tensor& x, const OptTensor& h, const OptTensor& gate,
     a.shift = sh.p;
     a.x_out = out.stream.defined() ? out.stream.data_ptr() : nullptr;
     a.y = codes ? nullptr : out.y.data_ptr();
-    a.codes = codes ? bytes_out(out.q.codes) : nullptr;
-    a.scales = codes ? bytes_out(out.q.scales) : nullptr;
+    a.codes = codes ? out.q.codes() : nullptr;
+    a.scales = codes ? out.q.scales() : nullptr;
     a.rows = rows;
     a.cols = cols;
     a.x_row_stride = xr.stride;
@@ -327,11 +332,9 @@ at::Tensor modulated_norm(const at::Tensor& x, const OptTensor& weight, const Op
     return run_norm(x, {}, {}, {}, weight, bias, scale, shift, layer, eps, 1.0, out_dtype, false).y;
 }
 
-std::tuple<at::Tensor, at::Tensor> modulated_norm_mxfp4(const at::Tensor& x, const OptTensor& weight,
-                                                        const OptTensor& bias, const OptTensor& scale,
-                                                        const OptTensor& shift, bool layer, double eps) {
-    const NormOut o = run_norm(x, {}, {}, {}, weight, bias, scale, shift, layer, eps, 1.0, {}, true);
-    return {o.q.codes, o.q.scales};
+at::Tensor modulated_norm_mxfp4(const at::Tensor& x, const OptTensor& weight, const OptTensor& bias,
+                                const OptTensor& scale, const OptTensor& shift, bool layer, double eps) {
+    return run_norm(x, {}, {}, {}, weight, bias, scale, shift, layer, eps, 1.0, {}, true).q.data;
 }
 
 std::tuple<at::Tensor, at::Tensor> gated_residual_norm(const at::Tensor& x, const at::Tensor& h, const OptTensor& gate,
@@ -343,45 +346,42 @@ std::tuple<at::Tensor, at::Tensor> gated_residual_norm(const at::Tensor& x, cons
     return {o.stream, o.y};
 }
 
-std::tuple<at::Tensor, at::Tensor, at::Tensor> gated_residual_norm_mxfp4(
-    const at::Tensor& x, const at::Tensor& h, const OptTensor& gate, const OptTensor& post_weight,
-    const OptTensor& weight, const OptTensor& bias, const OptTensor& scale, const OptTensor& shift, bool layer,
-    double eps, double residual_scale) {
+std::tuple<at::Tensor, at::Tensor> gated_residual_norm_mxfp4(const at::Tensor& x, const at::Tensor& h,
+                                                             const OptTensor& gate, const OptTensor& post_weight,
+                                                             const OptTensor& weight, const OptTensor& bias,
+                                                             const OptTensor& scale, const OptTensor& shift, bool layer,
+                                                             double eps, double residual_scale) {
     const NormOut o = run_norm(x, h, gate, post_weight, weight, bias, scale, shift, layer, eps, residual_scale, {}, true);
-    return {o.stream, o.q.codes, o.q.scales};
+    return {o.stream, o.q.data};
 }
 
 // ---- fake tensors ----
 
-std::tuple<at::Tensor, at::Tensor> quantize_mxfp4_meta(const at::Tensor& x) {
-    const Packed q = empty_packed(x.numel() / x.size(-1), x.size(-1), x);
-    return {q.codes, q.scales};
+at::Tensor quantize_mxfp4_meta(const at::Tensor& x) { return empty_packed(x.numel() / x.size(-1), x.size(-1), x).data; }
+at::Tensor dequantize_mxfp4_meta(const at::Tensor& data, at::IntArrayRef shape, at::ScalarType dtype) {
+    return at::empty(shape, data.options().dtype(dtype));
 }
-at::Tensor dequantize_mxfp4_meta(const at::Tensor& codes, const at::Tensor&, int64_t rows, int64_t cols, at::ScalarType dtype) {
-    return at::empty({rows, cols}, codes.options().dtype(dtype));
+at::Tensor prepack_mxfp4_meta(const at::Tensor& codes, const at::Tensor&, int64_t cols) {
+    return empty_packed(codes.size(0), cols, codes).data;
 }
-std::tuple<at::Tensor, at::Tensor> prepack_mxfp4_meta(const at::Tensor& codes, const at::Tensor&, int64_t cols) {
-    const Packed q = empty_packed(codes.size(0), cols, codes);
-    return {q.codes, q.scales};
-}
-std::tuple<at::Tensor, at::Tensor> unprepack_mxfp4_meta(const at::Tensor& codes, const at::Tensor&, int64_t rows, int64_t cols) {
+std::tuple<at::Tensor, at::Tensor> unprepack_mxfp4_meta(const at::Tensor& data, int64_t rows, int64_t cols) {
     const int64_t blocks = (cols + 31) / 32;
-    return {at::empty({rows, blocks * 16}, codes.options()), at::empty({rows, blocks}, codes.options())};
+    return {at::empty({rows, blocks * 16}, data.options()), at::empty({rows, blocks}, data.options())};
 }
-at::Tensor mxfp4_mm_meta(const at::Tensor& a, const at::Tensor&, const at::Tensor&, int64_t N, const OptTensor&,
-                         at::ScalarType out_dtype) {
-    return at::empty({a.size(0), N}, a.options().dtype(out_dtype));
+at::Tensor mxfp4_mm_meta(const at::Tensor& a, const at::Tensor&, int64_t N, int64_t, const OptTensor&,
+                         std::optional<at::ScalarType> dtype) {
+    return at::empty(with_last(a.sizes(), N), a.options().dtype(dtype.value_or(a.scalar_type())));
 }
-at::Tensor mxfp4_mm_packed_meta(const at::Tensor& a_codes, const at::Tensor&, int64_t M, int64_t, const at::Tensor&,
-                                const at::Tensor&, int64_t N, const OptTensor&, at::ScalarType out_dtype) {
-    return at::empty({M, N}, a_codes.options().dtype(out_dtype));
+at::Tensor mxfp4_mm_packed_meta(const at::Tensor& a, at::IntArrayRef a_shape, const at::Tensor&, int64_t N, int64_t,
+                                const OptTensor&, at::ScalarType out_dtype) {
+    return at::empty(with_last(a_shape, N), a.options().dtype(out_dtype));
 }
 at::Tensor modulated_norm_meta(const at::Tensor& x, const OptTensor&, const OptTensor&, const OptTensor&, const OptTensor&,
                                bool, double, std::optional<at::ScalarType> out_dtype) {
     return at::empty(x.sizes(), x.options().dtype(out_dtype.value_or(x.scalar_type())));
 }
-std::tuple<at::Tensor, at::Tensor> modulated_norm_mxfp4_meta(const at::Tensor& x, const OptTensor&, const OptTensor&,
-                                                             const OptTensor&, const OptTensor&, bool, double) {
+at::Tensor modulated_norm_mxfp4_meta(const at::Tensor& x, const OptTensor&, const OptTensor&, const OptTensor&,
+                                     const OptTensor&, bool, double) {
     return quantize_mxfp4_meta(x);
 }
 std::tuple<at::Tensor, at::Tensor> gated_residual_norm_meta(const at::Tensor& x, const at::Tensor& h, const OptTensor&,
@@ -390,33 +390,32 @@ std::tuple<at::Tensor, at::Tensor> gated_residual_norm_meta(const at::Tensor& x,
                                                             std::optional<at::ScalarType>) {
     return {at::empty(x.sizes(), x.options()), at::empty(x.sizes(), h.options())};
 }
-std::tuple<at::Tensor, at::Tensor, at::Tensor> gated_residual_norm_mxfp4_meta(
-    const at::Tensor& x, const at::Tensor&, const OptTensor&, const OptTensor&, const OptTensor&, const OptTensor&,
-    const OptTensor&, const OptTensor&, bool, double, double) {
-    const auto [codes, scales] = quantize_mxfp4_meta(x);
-    return {at::empty(x.sizes(), x.options()), codes, scales};
+std::tuple<at::Tensor, at::Tensor> gated_residual_norm_mxfp4_meta(const at::Tensor& x, const at::Tensor&,
+                                                                  const OptTensor&, const OptTensor&, const OptTensor&,
+                                                                  const OptTensor&, const OptTensor&, const OptTensor&,
+                                                                  bool, double, double) {
+    return {at::empty(x.sizes(), x.options()), quantize_mxfp4_meta(x)};
 }
 
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(feather_ops, m) {
-    m.def("quantize_mxfp4(Tensor x) -> (Tensor, Tensor)");
-    m.def("dequantize_mxfp4(Tensor codes, Tensor scales, int rows, int cols, ScalarType dtype) -> Tensor");
-    m.def("prepack_mxfp4(Tensor codes, Tensor scales, int cols) -> (Tensor, Tensor)");
-    m.def("unprepack_mxfp4(Tensor codes, Tensor scales, int rows, int cols) -> (Tensor, Tensor)");
-    m.def("mxfp4_mm(Tensor a, Tensor b_codes, Tensor b_scales, int N, Tensor? bias, ScalarType out_dtype) -> Tensor");
-    m.def("mxfp4_mm_packed(Tensor a_codes, Tensor a_scales, int M, int K, Tensor b_codes, Tensor b_scales, int N, "
-          "Tensor? bias, ScalarType out_dtype) -> Tensor");
+    m.def("quantize_mxfp4(Tensor x) -> Tensor");
+    m.def("dequantize_mxfp4(Tensor data, int[] shape, ScalarType dtype) -> Tensor");
+    m.def("prepack_mxfp4(Tensor codes, Tensor scales, int cols) -> Tensor");
+    m.def("unprepack_mxfp4(Tensor data, int rows, int cols) -> (Tensor, Tensor)");
+    m.def("mxfp4_mm(Tensor a, Tensor b, int N, int K, Tensor? bias, ScalarType? out_dtype) -> Tensor");
+    m.def("mxfp4_mm_packed(Tensor a, int[] a_shape, Tensor b, int N, int K, Tensor? bias, ScalarType out_dtype) -> Tensor");
     m.def("modulated_norm(Tensor x, Tensor? weight, Tensor? bias, Tensor? scale, Tensor? shift, bool layer, float eps, "
           "ScalarType? out_dtype) -> Tensor");
     m.def("modulated_norm_mxfp4(Tensor x, Tensor? weight, Tensor? bias, Tensor? scale, Tensor? shift, bool layer, "
-          "float eps) -> (Tensor, Tensor)");
+          "float eps) -> Tensor");
     m.def("gated_residual_norm(Tensor x, Tensor h, Tensor? gate, Tensor? post_weight, Tensor? weight, Tensor? bias, "
           "Tensor? scale, Tensor? shift, bool layer, float eps, float residual_scale, ScalarType? out_dtype) -> "
           "(Tensor, Tensor)");
     m.def("gated_residual_norm_mxfp4(Tensor x, Tensor h, Tensor? gate, Tensor? post_weight, Tensor? weight, "
           "Tensor? bias, Tensor? scale, Tensor? shift, bool layer, float eps, float residual_scale) -> "
-          "(Tensor, Tensor, Tensor)");
+          "(Tensor, Tensor)");
 }
 
 TORCH_LIBRARY_IMPL(feather_ops, CUDA, m) {

@@ -14,6 +14,7 @@ All of it runs in libfeatherops_amd.so on torch's current stream; there is no ot
 
 from __future__ import annotations
 
+import math
 from typing import NamedTuple
 
 import torch
@@ -31,10 +32,10 @@ _mm_packed = _ops.mxfp4_mm_packed.default
 
 
 class MXFP4Tensor(NamedTuple):
-    """A tensor in MXFP4, blocks along its last dimension, in the packed layout."""
+    """A tensor in MXFP4, blocks along its last dimension, in the packed layout: `data` (uint8) holds the
+    codes and, behind them, the scales."""
 
-    codes: torch.Tensor
-    scales: torch.Tensor
+    data: torch.Tensor
     shape: tuple
 
     @property
@@ -43,24 +44,30 @@ class MXFP4Tensor(NamedTuple):
 
     @property
     def rows(self) -> int:
-        n = 1
-        for d in self.shape[:-1]:
-            n *= d
-        return n
+        return math.prod(self.shape[:-1])
+
+    @property
+    def codes(self) -> torch.Tensor:
+        """(4 * groups, steps, 64, 16) view of the codes: include/featherops_amd.h."""
+        groups, steps = (self.rows + 63) // 64, (self.cols + 127) // 128
+        return self.data[:groups * steps * 4096].view(groups * 4, steps, 64, 16)
+
+    @property
+    def scales(self) -> torch.Tensor:
+        """(groups, steps, 64, 4) view of the scales."""
+        groups, steps = (self.rows + 63) // 64, (self.cols + 127) // 128
+        return self.data[groups * steps * 4096:].view(groups, steps, 64, 4)
 
 
 def quantize_mxfp4(x: torch.Tensor) -> MXFP4Tensor:
     """x (..., cols), fp16, bf16 or fp32, quantised along its last dimension; any number of columns
     (a last block shorter than 32 counts as continued by zeros)."""
-    codes, scales = _quantize(x)
-    return MXFP4Tensor(codes, scales, tuple(x.shape))
+    return MXFP4Tensor(_quantize(x), tuple(x.shape))
 
 
 def dequantize_mxfp4(q: MXFP4Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """The values that q stands for, each rounded once to dtype (fp16, bf16 or fp32)."""
-    if len(q.shape) == 2:
-        return _dequantize(q.codes, q.scales, *q.shape, dtype)
-    return _dequantize(q.codes, q.scales, q.rows, q.cols, dtype).view(q.shape)
+    return _dequantize(q.data, q.shape, dtype)
 
 
 def prepack_mxfp4(codes: torch.Tensor, scales: torch.Tensor, cols: int | None = None) -> MXFP4Tensor:
@@ -68,13 +75,12 @@ def prepack_mxfp4(codes: torch.Tensor, scales: torch.Tensor, cols: int | None = 
     half, and e8m0 scales (rows, blocks) in the packed layout. cols: the number of columns where it
     is not blocks * 32 (the codes beyond it must be zero)."""
     cols = codes.shape[-1] * 2 if cols is None else cols
-    packed, packed_scales = _prepack(codes, scales, cols)
-    return MXFP4Tensor(packed, packed_scales, (codes.shape[0], cols))
+    return MXFP4Tensor(_prepack(codes, scales, cols), (codes.shape[0], cols))
 
 
 def unprepack_mxfp4(q: MXFP4Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """The row-major codes and scales of q (prepack_mxfp4's arguments)."""
-    return _unprepack(q.codes, q.scales, q.rows, q.cols)
+    return _unprepack(q.data, q.rows, q.cols)
 
 
 def mxfp4_mm(a: torch.Tensor | MXFP4Tensor, w: MXFP4Tensor, bias: torch.Tensor | None = None,
@@ -87,12 +93,5 @@ def mxfp4_mm(a: torch.Tensor | MXFP4Tensor, w: MXFP4Tensor, bias: torch.Tensor |
     result is rounded once."""
     N, K = w.shape
     if isinstance(a, MXFP4Tensor):
-        if a.shape[-1] != K:
-            raise RuntimeError(f"a has {a.shape[-1]} columns, w {K}")
-        y = _mm_packed(a.codes, a.scales, a.rows, K, w.codes, w.scales, N, bias, out_dtype or torch.bfloat16)
-        return y if len(a.shape) == 2 else y.view(*a.shape[:-1], N)
-    if a.dim() < 1 or a.shape[-1] != K:
-        raise RuntimeError(f"a must have w's {K} columns, got {tuple(a.shape)}")
-    if a.dim() == 2:
-        return _mm(a, w.codes, w.scales, N, bias, out_dtype or a.dtype)
-    return _mm(a.reshape(-1, K), w.codes, w.scales, N, bias, out_dtype or a.dtype).view(*a.shape[:-1], N)
+        return _mm_packed(a.data, a.shape, w.data, N, K, bias, out_dtype or torch.bfloat16)
+    return _mm(a, w.data, N, K, bias, out_dtype)

@@ -50,8 +50,7 @@ def modulated_norm(x: torch.Tensor, *, weight: torch.Tensor | None = None, bias:
                    eps: float = 1e-6, out_dtype: torch.dtype | str | None = None) -> torch.Tensor | MXFP4Tensor:
     """norm(x) * weight + bias, then * (1 + scale) + shift, in one pass over x."""
     if out_dtype == "mxfp4":
-        codes, scales = _modulated_mxfp4(x, weight, bias, scale, shift, _is_layer(kind), eps)
-        return MXFP4Tensor(codes, scales, tuple(x.shape))
+        return MXFP4Tensor(_modulated_mxfp4(x, weight, bias, scale, shift, _is_layer(kind), eps), tuple(x.shape))
     return _modulated(x, weight, bias, scale, shift, _is_layer(kind), eps, out_dtype)
 
 
@@ -64,7 +63,6 @@ def gated_residual_norm(x: torch.Tensor, h: torch.Tensor, gate: torch.Tensor | N
     """(x, y): the block's output h on the residual stream x, and the norm of the sum before it is
     rounded, in one pass over x and h."""
     if out_dtype == "mxfp4":
-        stream, codes, scales = _gated_mxfp4(x, h, gate, post_weight, weight, bias, scale, shift, _is_layer(kind), eps,
-                                             residual_scale)
-        return stream, MXFP4Tensor(codes, scales, tuple(x.shape))
+        stream, y = _gated_mxfp4(x, h, gate, post_weight, weight, bias, scale, shift, _is_layer(kind), eps, residual_scale)
+        return stream, MXFP4Tensor(y, tuple(x.shape))
     return _gated(x, h, gate, post_weight, weight, bias, scale, shift, _is_layer(kind), eps, residual_scale, out_dtype)

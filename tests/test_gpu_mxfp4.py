@@ -261,13 +261,15 @@ def test_refusals(mx, cuda):
         (lambda: mx.dequantize_mxfp4(w, torch.float64), "float16, bfloat16 or float32"),
         (lambda: mx.dequantize_mxfp4(w._replace(shape=(80, 64))), "packed for"),
         (lambda: mx.mxfp4_mm(x.float(), w), "float16 or bfloat16"),
-        (lambda: mx.mxfp4_mm(x[:, :32], w), "64 columns"),
+        (lambda: mx.mxfp4_mm(x[:, :32], w), "b's 64 columns"),
         (lambda: mx.mxfp4_mm(mx.quantize_mxfp4(x[:, :32]), w), "columns"),
         (lambda: mx.mxfp4_mm(x, w, torch.zeros(8, device=cuda)), "output's dtype"),
         (lambda: mx.mxfp4_mm(x, w, torch.zeros(9, dtype=x.dtype, device=cuda)), "N (8) elements"),
         (lambda: mx.mxfp4_mm(x, w, None, torch.float32), "out_dtype"),
-        (lambda: mx.mxfp4_mm(x, w._replace(codes=w.codes.cpu())), "device"),
-        (lambda: mx.mxfp4_mm(x, w._replace(codes=w.codes.transpose(2, 3).contiguous().transpose(2, 3))), "contiguous"),
+        (lambda: mx.mxfp4_mm(x, w._replace(data=w.data.cpu())), "device"),
+        (lambda: mx.mxfp4_mm(x, w._replace(data=w.data.repeat_interleave(2)[::2])), "contiguous"),
+        (lambda: mx.mxfp4_mm(x, w._replace(data=w.data[:-1])), "packed for"),
+        (lambda: mx.mxfp4_mm(x, w._replace(data=torch.cat((w.data[:8], w.data))[8:])), "aligned"),
         (lambda: mx.prepack_mxfp4(w.codes.view(-1, 16)[:8], w.scales.view(-1, 1)[:9]), "rows"),
         (lambda: mx.prepack_mxfp4(torch.zeros(8, 32, dtype=torch.uint8, device=cuda),
                                   torch.zeros(8, 2, dtype=torch.uint8, device=cuda), 65), "for 65 columns"),
