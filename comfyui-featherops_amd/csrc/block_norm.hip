@@ -276,7 +276,7 @@ __global__ __launch_bounds__(kOneWave ? 256 : 1024, V == 1 ? 8 : 4) void norm_ke
     }
     normalise(s, sums[2]);
     // (this row's place in the packed operand; the columns' place in it is the thread's)
-    uint8_t* row_codes = kCodes ? p.codes + (row >> 4) * ksteps * 1024 + (row & 15) * 16 : nullptr;
+    uint8_t* row_codes = kCodes ? p.codes + ((row >> 6) * ksteps * 4 + ((row >> 4) & 3)) * 1024 + (row & 15) * 16 : nullptr;
     uint8_t* row_scales = kCodes ? p.scales + (row >> 6) * ksteps * 256 + (row & 15) * 4 + ((row >> 4) & 3) : nullptr;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
@@ -333,7 +333,7 @@ __global__ __launch_bounds__(kOneWave ? 256 : 1024, V == 1 ? 8 : 4) void norm_ke
             o = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(o, y[4], y[5], q, 2);
             o = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(o, y[6], y[7], q, 3);
             if (c < ksteps * kMxStepK) {
-                *reinterpret_cast<uint32_t*>(row_codes + c / kMxBlock * 256 + c % kMxBlock / 2) = o;
+                *reinterpret_cast<uint32_t*>(row_codes + c / kMxStepK * 4096 + c % kMxStepK / kMxBlock * 256 + c % kMxBlock / 2) = o;
                 if (c % kMxBlock == 0) row_scales[c / kMxBlock * 64] = static_cast<uint8_t>(sb);
             }
         }

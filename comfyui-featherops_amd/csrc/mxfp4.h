@@ -14,12 +14,13 @@
 //
 // Packed layout, the operand order of the block-scaled 16x16x128 MFMA, for R
 // rows and K columns, ksteps = ceil(K / 128), groups = ceil(R / 64):
-//   codes  [4 * groups][ksteps][64][16 bytes]: lane l of row tile t and step s
-//          holds row 16 t + l % 16, columns 128 s + 32 (l / 16) .. + 31
-//   scales [groups][ksteps][64][4]: byte f of lane l belongs to row tile
-//          4 g + f of that lane's row and block
-// so a wave's operand load is one contiguous KB and the scales of four row tiles
-// are one dword per lane, selected by the instruction. Columns beyond K are zero
+//   codes  [groups][ksteps][4][64][16 bytes]: lane l of row tile f of group g and
+//          step s holds row 64 g + 16 f + l % 16, columns 128 s + 32 (l / 16) .. + 31
+//   scales [groups][ksteps][64][4]: byte f of lane l belongs to that row and block
+// so a wave's operand load is one contiguous KB, the scales of four row tiles are one
+// dword per lane, selected by the instruction, and the row tiles that a workgroup reads
+// at one step are runs of 4 KB: with the steps of a row tile next to each other instead,
+// row tiles lie ksteps KB apart and a step's reads fall on few of the L2's channels (LAYOUT_US). Columns beyond K are zero
 // codes under scale 2^-127; rows beyond R may hold anything (no row's result
 // depends on another row).
 #pragma once

@@ -31,6 +31,14 @@ __device__ __forceinline__ void dma4_lds(const void* sbase, uint32_t voff, uint3
         : "memory");
 }
 
+// A wave-uniform pointer in scalar registers, as the copies take it.
+__device__ __forceinline__ const uint8_t* scalar_pointer(const uint8_t* p) {
+    const uint64_t v = reinterpret_cast<uint64_t>(p);
+    const uint64_t lo = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(v)));
+    const uint64_t hi = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(v >> 32)));
+    return reinterpret_cast<const uint8_t*>(hi << 32 | lo);
+}
+
 struct TileArgs {
     const uint8_t* a;
     const uint8_t* as;
@@ -107,7 +115,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mx_tile_kernel(const TileArgs
         const bool is_a = j < BM / 16;
         const int f = is_a ? j : j - BM / 16;
         const int64_t g = is_a ? min(static_cast<int>(m0 / 64) + f / 4, p.a_groups - 1) : min(n0 / 64 + f / 4, p.b_groups - 1);
-        src[i] = (is_a ? p.a : p.b) + ((g * 4 + f % 4) * p.ksteps + k0) * 1024;
+        src[i] = scalar_pointer((is_a ? p.a : p.b) + ((g * p.ksteps + k0) * 4 + f % 4) * 1024);
         dst[i] = lds + j * 1024;
     }
 #pragma unroll
@@ -115,12 +123,12 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mx_tile_kernel(const TileArgs
         const int j = min(i * kWaves + wave, kScaleCopies - 1);
         const bool is_a = j < kGroupsM;
         const int64_t g = is_a ? min(static_cast<int>(m0 / 64) + j, p.a_groups - 1) : min(n0 / 64 + j - kGroupsM, p.b_groups - 1);
-        src[kCodes + i] = (is_a ? p.as : p.bs) + (g * p.ksteps + k0) * 256;
+        src[kCodes + i] = scalar_pointer((is_a ? p.as : p.bs) + (g * p.ksteps + k0) * 256);
         dst[kCodes + i] = lds + kScaleBase + j * 256;
     }
     // (the step in the lane's offset, one instruction for all copies, not in each copy's address)
     auto copy = [&](auto i, int step, int slot_bytes) {
-        if constexpr (i < kCodes) dma16_lds(src[i], lane * 16 + step * 1024, dst[i] + slot_bytes);
+        if constexpr (i < kCodes) dma16_lds(src[i], lane * 16 + step * 4096, dst[i] + slot_bytes);
         else dma4_lds(src[i], lane * 4 + step * 256, dst[i] + slot_bytes);
     };
 

@@ -32,7 +32,7 @@ struct WaveTask {
     }
     __device__ __forceinline__ int64_t row(int f) const { return group * 64 + f * 16 + lr; }
     __device__ __forceinline__ int64_t code_at(int f, int ksteps) const {
-        return ((group * 4 + f) * ksteps + step) * 1024 + lane * 16;
+        return ((group * ksteps + step) * 4 + f) * 1024 + lane * 16;
     }
     __device__ __forceinline__ int64_t scale_at(int ksteps) const { return (group * ksteps + step) * 256 + lane * 4; }
     // the first column of the lane's pieces, and how many of their 8 values exist
@@ -78,7 +78,8 @@ __global__ __launch_bounds__(64 * kWavesPerBlock) void quantize_kernel(const uin
 #pragma unroll
     for (int f = 0; f < kTiles; ++f) {
         uint32_t s;
-        *reinterpret_cast<uint4*>(codes + ((unit * kTiles + f) * ksteps + step) * 1024 + lane * 16) = v[f].quantize(lane, &s);
+        const int64_t tile = unit * kTiles + f;
+        *reinterpret_cast<uint4*>(codes + (((tile >> 2) * ksteps + step) * 4 + (tile & 3)) * 1024 + lane * 16) = v[f].quantize(lane, &s);
         bytes |= s << (8 * f);
     }
     if constexpr (kTiles == 4) *reinterpret_cast<uint32_t*>(scales + (unit * ksteps + step) * 256 + lane * 4) = bytes;

@@ -74,11 +74,12 @@ __global__ __launch_bounds__(64 * kWaves) void mx_rows_kernel(const RowsArgs p) 
     // Operands come through buffer descriptors: a step past the wave's last one reads nothing, so the loop
     // has no branch around loads, where the compiler would wait for all of those in flight.
     const __amdgpu_buffer_rsrc_t bres = __builtin_amdgcn_make_buffer_rsrc(
-        const_cast<uint8_t*>(p.b + tile0 * p.ksteps * 1024), 0, NT * p.ksteps * 1024, 0x00020000);
+        const_cast<uint8_t*>(p.b + (tile0 / 4 * p.ksteps * 4 + tile0 % 4) * 1024), 0,
+        (p.ksteps * 4 - static_cast<int>(tile0 % 4)) * 1024, 0x00020000);
     const __amdgpu_buffer_rsrc_t bsres = __builtin_amdgcn_make_buffer_rsrc(
         const_cast<uint8_t*>(p.bs + (tile0 / 4) * p.ksteps * 256), 0, p.ksteps * 256, 0x00020000);
     const __amdgpu_buffer_rsrc_t ares = __builtin_amdgcn_make_buffer_rsrc(
-        const_cast<uint8_t*>(p.a), 0, AT == kMxPacked ? MT * p.ksteps * 1024 : (p.M - 1) * p.a_row_bytes + p.K * 2, 0x00020000);
+        const_cast<uint8_t*>(p.a), 0, AT == kMxPacked ? p.ksteps * 4096 : (p.M - 1) * p.a_row_bytes + p.K * 2, 0x00020000);
     const __amdgpu_buffer_rsrc_t asres = __builtin_amdgcn_make_buffer_rsrc(
         const_cast<uint8_t*>(AT == kMxPacked ? p.as : p.a), 0, AT == kMxPacked ? p.ksteps * 256 : 0, 0x00020000);
     constexpr uint32_t kNone = 0x80000000u;  // an offset past every descriptor's end
@@ -86,7 +87,7 @@ __global__ __launch_bounds__(64 * kWaves) void mx_rows_kernel(const RowsArgs p) 
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
         if constexpr (AT == kMxPacked) {
-            arow[i][0] = i * p.ksteps * 1024 + lane * 16;
+            arow[i][0] = i * 1024 + lane * 16;
         } else {  // rows past the last repeat it (their results are not stored)
 #pragma unroll
             for (int v = 0; v < 4; ++v)
@@ -97,7 +98,7 @@ __global__ __launch_bounds__(64 * kWaves) void mx_rows_kernel(const RowsArgs p) 
 #pragma unroll
         for (int j = 0; j < NT; ++j)
             s.b[j] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(
-                                                   bres, have ? (j * p.ksteps + k) * 1024 + lane * 16 : kNone, 0, 0));
+                                                   bres, have ? (k * 4 + j) * 1024 + lane * 16 : kNone, 0, 0));
         s.bs = __builtin_amdgcn_raw_buffer_load_b32(bsres, have ? k * 256 + lane * 4 : kNone, 0, 0);
     };
     // a step that ends within K
@@ -105,7 +106,7 @@ __global__ __launch_bounds__(64 * kWaves) void mx_rows_kernel(const RowsArgs p) 
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
             if constexpr (AT == kMxPacked) {
-                s.a[i] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(ares, have ? arow[i][0] + k * 1024 : kNone, 0, 0));
+                s.a[i] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(ares, have ? arow[i][0] + k * 4096 : kNone, 0, 0));
             } else {
 #pragma unroll
                 for (int v = 0; v < 4; ++v)

@@ -48,9 +48,9 @@ class MXFP4Tensor(NamedTuple):
 
     @property
     def codes(self) -> torch.Tensor:
-        """(4 * groups, steps, 64, 16) view of the codes: include/featherops_amd.h."""
+        """(groups, steps, 4, 64, 16) view of the codes: include/featherops_amd.h."""
         groups, steps = (self.rows + 63) // 64, (self.cols + 127) // 128
-        return self.data[:groups * steps * 4096].view(groups * 4, steps, 64, 16)
+        return self.data[:groups * steps * 4096].view(groups, steps, 4, 64, 16)
 
     @property
     def scales(self) -> torch.Tensor:

@@ -327,8 +327,8 @@ int feather_dequantize_e5m2(const uint8_t* packed, const float* scale, void* out
  * Row-major form (checkpoints), blocks = ceil(cols / 32): codes (rows, blocks * 16)
  * bytes, the earlier value of a pair in the low half; scales (rows, blocks).
  * Packed form (operands), steps = ceil(cols / 128), groups = ceil(rows / 64):
- *   codes  [4 * groups][steps][64][16]: row r, column k in byte (k % 32) / 2 of
- *          [r / 16][k / 128][16 * (k % 128 / 32) + r % 16]
+ *   codes  [groups][steps][4][64][16]: row r, column k in byte (k % 32) / 2 of
+ *          [r / 64][k / 128][r / 16 % 4][16 * (k % 128 / 32) + r % 16]
  *   scales [groups][steps][64][4]: that block's in byte r / 16 % 4 of
  *          [r / 64][k / 128][16 * (k % 128 / 32) + r % 16]
  * Buffers of the packed form are 16-byte aligned. rows <= 2^30, cols < 2^24.

@@ -92,12 +92,12 @@ def test_splits_fit_their_counters(lib):
 def test_fake_tensors(mx, nm):
     x = torch.empty(3, 5, 200, dtype=torch.bfloat16, device="meta")
     q = mx.quantize_mxfp4(x)
-    assert q.codes.shape == (4, 2, 64, 16) and q.scales.shape == (1, 2, 64, 4) and q.shape == (3, 5, 200)
+    assert q.codes.shape == (1, 2, 4, 64, 16) and q.scales.shape == (1, 2, 64, 4) and q.shape == (3, 5, 200)
     assert (q.rows, q.cols) == (15, 200)
     assert mx.dequantize_mxfp4(q, torch.float32).shape == (3, 5, 200)
     w = mx.prepack_mxfp4(torch.empty(70, 112, dtype=torch.uint8, device="meta"),
                          torch.empty(70, 7, dtype=torch.uint8, device="meta"), 200)
-    assert w.codes.shape == (8, 2, 64, 16) and w.shape == (70, 200)
+    assert w.codes.shape == (2, 2, 4, 64, 16) and w.shape == (70, 200)
     assert [t.shape for t in mx.unprepack_mxfp4(w)] == [(70, 112), (70, 7)]
     assert mx.mxfp4_mm(x, w).shape == (3, 5, 70) and mx.mxfp4_mm(q, w).dtype == torch.bfloat16
     s, y = nm.gated_residual_norm(x.float(), x, x[0, 0])

@@ -120,10 +120,10 @@ def test_prepack_layout_and_back(mx, cuda, rows, cols):
     r, b = np.meshgrid(np.arange(rows), np.arange(blocks), indexing="ij")
     packed, packed_scales = q.codes.cpu().numpy(), q.scales.cpu().numpy()
     lane = 16 * (b % 4) + r % 16
-    np.testing.assert_array_equal(packed[r // 16, b // 4, lane], codes.reshape(rows, blocks, 16))
+    np.testing.assert_array_equal(packed[r // 64, b // 4, r // 16 % 4, lane], codes.reshape(rows, blocks, 16))
     np.testing.assert_array_equal(packed_scales[r // 64, b // 4, lane, r // 16 % 4], scales)
     # steps are padded with zero codes
-    assert not packed[:, blocks // 4:][:, :, 16 * (blocks % 4):].any() or blocks % 4 == 0
+    assert not packed[:, blocks // 4:, :, 16 * (blocks % 4):].any() or blocks % 4 == 0
 
 
 def operands(mx, cuda, M, N, K, dtype, seed):
@@ -205,7 +205,9 @@ def test_product_keeps_rows_apart(mx, cuda, M):
     y = mx.mxfp4_mm(x, q, bias)
     check_product(y, x, w, bias, "non-finite")
     a = mx.quantize_mxfp4(x)
-    a.codes.view(-1, a.codes.shape[1], 4, 16, 16)[-(-M // 16):] = 0xFF
+    codes = a.codes.view(*a.codes.shape[:3], 4, 16, 16)
+    codes[-1, :, M % 64 // 16, :, M % 16:] = 0xFF
+    codes[-1, :, M % 64 // 16 + 1:] = 0xFF
     a.scales.view(-1, a.scales.shape[1], 4, 16, 4)[-1, :, :, M % 16:, M % 64 // 16] = 0xFF
     if M % 64 // 16 < 3:
         a.scales.view(-1, a.scales.shape[1], 4, 16, 4)[-1, :, :, :, M % 64 // 16 + 1:] = 0xFF
