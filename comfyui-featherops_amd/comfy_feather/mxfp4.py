@@ -1,0 +1,120 @@
+"""Linear replacement with a 4-bit weight (no counterpart in the reference).
+
+`mxfp4_ops(out_dtype, excluded_names)` returns an operations class for ComfyUI's `custom_operations`
+hook, the 4-bit sibling of `feather_ops`. Its `Linear`:
+  * at state-dict load quantizes the weight to packed MXFP4 on the GPU, or lays out one that the
+    checkpoint holds in MXFP4 already (uint8 codes (N, blocks * 16) with uint8 `weight_scale` (N, blocks)),
+    unless the layer is excluded or 1-wide;
+  * in forward runs mxfp4_mm with the bias; activations in fp16 or bf16 (fp32 is cast to bf16), or an
+    MXFP4Tensor that a norm left in 4 bits (kernel.hip.norm, out_dtype="mxfp4"), and applies basic LoRA
+    patches as a separate pass over activations that are not in 4 bits;
+  * converts the weight back for a merge (convert_weight) and takes the merged one (set_weight).
+
+Inside ComfyUI it subclasses comfy.ops.manual_cast; without it the stand-in of `ops.py`.
+"""
+
+from __future__ import annotations
+
+import torch
+import torch.nn.functional as F
+from torch import nn
+
+from ..kernel.hip.mxfp4 import MXFP4Tensor, dequantize_mxfp4, mxfp4_mm, prepack_mxfp4, quantize_mxfp4, unprepack_mxfp4
+from .lora import apply_lora_patches
+from .ops import cast_bias_weight, manual_cast, run_every_op, uncast_bias_weight
+
+
+def _on_gpu(t: torch.Tensor) -> torch.Tensor:
+    return t if t.is_cuda else t.to("cuda")
+
+
+def mxfp4_ops(out_dtype=torch.bfloat16, excluded_names=()):
+    excluded_names = tuple(excluded_names)
+
+    class MXFP4Ops(manual_cast):
+        _excluded_names = excluded_names
+        _out_dtype = out_dtype
+
+        class Linear(manual_cast.Linear):
+            def __init__(self, *args, **kwargs):
+                super().__init__(*args, **kwargs)
+                self.excluded_names = MXFP4Ops._excluded_names
+                self.out_dtype = MXFP4Ops._out_dtype
+                self.mx_weight: MXFP4Tensor | None = None
+
+            def _load_from_state_dict(self, state_dict, prefix, local_metadata, strict, missing_keys,
+                                      unexpected_keys, error_msgs):
+                weight = state_dict.pop(prefix + "weight", None)
+                bias = state_dict.pop(prefix + "bias", None)
+                scales = state_dict.pop(prefix + "weight_scale", None)
+                if weight is None:
+                    missing_keys.append(prefix + "weight")
+                elif scales is not None and weight.dtype == torch.uint8:
+                    self._hold(prepack_mxfp4(_on_gpu(weight), _on_gpu(scales), self.in_features))
+                elif (any(x in prefix for x in self.excluded_names) or weight.ndim == 1 or self.in_features == 1
+                      or self.out_features == 1):
+                    self.mx_weight = None
+                    self.weight = nn.Parameter(weight, requires_grad=False)
+                else:
+                    self._hold(quantize_mxfp4(_on_gpu(weight)))
+                self.bias = None if bias is None else nn.Parameter(bias.to(self.out_dtype), requires_grad=False)
+
+            def _hold(self, weight: MXFP4Tensor) -> None:
+                if weight.shape != (self.out_features, self.in_features):
+                    raise ValueError(f"expected a ({self.out_features}, {self.in_features}) weight, got {weight.shape}")
+                self.mx_weight = weight
+                self.weight = None
+
+            def _save_to_state_dict(self, destination, prefix, keep_vars):
+                super()._save_to_state_dict(destination, prefix, keep_vars)
+                if self.mx_weight is not None:
+                    destination[prefix + "weight"], destination[prefix + "weight_scale"] = unprepack_mxfp4(self.mx_weight)
+
+            def _apply(self, fn, recurse=True):
+                super()._apply(fn, recurse)
+                if self.mx_weight is not None:  # bytes: moved between devices, never cast
+                    moved = fn(self.mx_weight.data)
+                    self.mx_weight = self.mx_weight._replace(data=moved if moved.dtype == torch.uint8
+                                                             else self.mx_weight.data.to(moved.device))
+                return self
+
+            def convert_weight(self, weight=None, inplace=False, **kwargs):
+                if self.mx_weight is None:
+                    return self.weight if weight is None else weight
+                return dequantize_mxfp4(self.mx_weight, self.out_dtype)
+
+            def set_weight(self, weight, inplace_update=False, seed=None, return_weight=False, **kwargs):
+                if self.mx_weight is None:
+                    weight = weight.to(self.weight.dtype)
+                    if return_weight:
+                        return weight
+                    self.weight = nn.Parameter(weight, requires_grad=False)
+                    return None
+                quantized = quantize_mxfp4(_on_gpu(weight))
+                if return_weight:
+                    return quantized
+                assert inplace_update is False
+                self._hold(quantized)
+                return None
+
+            def forward(self, x: torch.Tensor | MXFP4Tensor) -> torch.Tensor:
+                run_every_op()
+                if self.mx_weight is None:
+                    weight, bias, offload_stream = cast_bias_weight(self, x, offloadable=True)
+                    y = F.linear(x, weight, bias)
+                    uncast_bias_weight(self, weight, bias, offload_stream)
+                    return y
+                bias = self.bias
+                if isinstance(x, MXFP4Tensor):
+                    if self.weight_function:
+                        raise NotImplementedError("LoRA patches need activations in 16 bits")
+                    return mxfp4_mm(x, self.mx_weight, bias, self.out_dtype)
+                dtype = x.dtype
+                if dtype == torch.float32:
+                    x = x.to(torch.bfloat16)
+                y = mxfp4_mm(x, self.mx_weight, bias, self.out_dtype)
+                if self.weight_function:
+                    y = apply_lora_patches(x, y, self.weight_function)
+                return y if y.dtype == dtype else y.to(dtype)
+
+    return MXFP4Ops

@@ -12,10 +12,10 @@ using namespace feather;
 constexpr int64_t kMaxCols = int64_t(1) << 24;
 constexpr int64_t kMaxRows = int64_t(1) << 30;
 
-// rows and cols of an MXFP4 tensor; the layout kernels give one wave 64 x 128 values and a grid
-// holds fewer than 2^32 threads
+// rows and cols of an MXFP4 tensor; the layout kernels give one wave at least 16 x 128 values and a
+// grid holds fewer than 2^32 threads
 bool mx_sizes_ok(int64_t rows, int64_t cols) {
-    return rows >= 0 && cols > 0 && rows <= kMaxRows && cols < kMaxCols && mx_groups(rows) * mx_ksteps(cols) < (int64_t(1) << 25);
+    return rows >= 0 && cols > 0 && rows <= kMaxRows && cols < kMaxCols && mx_groups(rows) * mx_ksteps(cols) < (int64_t(1) << 23);
 }
 bool value_type(int t) { return t == FEATHER_DTYPE_F16 || t == FEATHER_DTYPE_BF16 || t == FEATHER_DTYPE_F32; }
 bool mm_sizes_ok(int64_t M, int64_t N, int64_t K) { return mx_sizes_ok(M, K) && N > 0 && mx_sizes_ok(N, K); }

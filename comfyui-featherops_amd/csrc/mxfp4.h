@@ -19,8 +19,8 @@
 //   scales [groups][ksteps][64][4]: byte f of lane l belongs to that row and block
 // so a wave's operand load is one contiguous KB, the scales of four row tiles are one
 // dword per lane, selected by the instruction, and the row tiles that a workgroup reads
-// at one step are runs of 4 KB: with the steps of a row tile next to each other instead,
-// row tiles lie ksteps KB apart and a step's reads fall on few of the L2's channels (LAYOUT_US). Columns beyond K are zero
+// at one step are runs of 4 KB (with the steps of a row tile next to each other instead,
+// M=333 N=K=5120 takes 12.7 us for 12.2). Columns beyond K are zero
 // codes under scale 2^-127; rows beyond R may hold anything (no row's result
 // depends on another row).
 #pragma once

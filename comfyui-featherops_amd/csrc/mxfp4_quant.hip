@@ -1,11 +1,11 @@
 // MXFP4 quantisation and its layouts: row-major values <-> packed operands, and
 // the row-major codes of checkpoints <-> packed operands. Formats in mxfp4.h.
 //
-// All four kernels give one wave a group of 64 rows and one step of 128 columns:
-// lane l has row l % 16 of each of the group's four row tiles and the block of 32
-// columns l / 16, the packed layout's own order, so codes leave as whole KBs and the
-// four tiles' scales as one dword per lane. Values are read and written four lanes to
-// a block (MxPieces). HBM bound.
+// All four kernels give one wave rows of one step of 128 columns, a row tile of 16 or a
+// group of four: lane l has row l % 16 of a tile and the block of 32 columns l / 16, the
+// packed layout's own order, so a tile's codes are one KB. Values are read and written four
+// lanes to a block (MxPieces). HBM bound: 13824 x 5120 in bf16 quantised at 5.6 TB/s (31.8 us),
+// read back at 6.6 (27.1 us; the codes come from the memory-side cache).
 #include <type_traits>
 
 #include "featherops_amd.h"
@@ -40,50 +40,39 @@ struct WaveTask {
     __device__ __forceinline__ int count(int cols) const { return max(0, min(8, cols - col())); }
 };
 
-// kTiles: row tiles of a wave, all four of a group where there are many rows, one where waves would be too
-// few to fill the chip (us, 154 x 4096 in bf16: ONE_US against FOUR_US).
-template <int T, int kTiles>
+// A wave quantises one row tile of one step: the other kernels' four tiles a wave leave too few waves to fill the
+// chip below some thousand rows (154 x 4096 in bf16 2.5 against 3.3 us, 1003 x 3211 in fp16 3.8 against 6.7) and
+// gain little above (13824 x 5120 31.8 against 31.2).
+template <int T>
 __global__ __launch_bounds__(64 * kWavesPerBlock) void quantize_kernel(const uint8_t* __restrict__ x, int64_t rows,
                                                                        int cols, int64_t row_bytes,
                                                                        uint8_t* __restrict__ codes,
                                                                        uint8_t* __restrict__ scales, int ksteps,
-                                                                       int64_t units) {
+                                                                       int64_t tiles) {
     const int64_t w = static_cast<int64_t>(blockIdx.x) * kWavesPerBlock + (threadIdx.x >> 6);
-    if (w >= units * ksteps) return;
-    const int64_t unit = w / ksteps;  // kTiles row tiles
-    const int step = static_cast<int>(w - unit * ksteps);
+    if (w >= tiles * ksteps) return;
+    const int64_t tile = w / ksteps;
+    const int step = static_cast<int>(w - tile * ksteps);
     const int lane = threadIdx.x & 63;
-    const int64_t row0 = unit * (16 * kTiles);
     const int col = step * kMxStepK + mx_piece_col(lane);
     // rows past the last repeat it: nothing reads what their place in the operand holds
-    auto row = [&](int f, int i) { return x + min(row0 + f * 16 + mx_piece_row(lane, i), rows - 1) * row_bytes; };
-    MxPieces<T> v[kTiles];
-    if ((step + 1) * kMxStepK <= cols) {  // (the same for the whole wave) every load in flight at once
+    auto row = [&](int i) { return x + min(tile * 16 + mx_piece_row(lane, i), rows - 1) * row_bytes; };
+    MxPieces<T> v;
+    if ((step + 1) * kMxStepK <= cols) {  // (the same for the whole wave, as are the others)
 #pragma unroll
-        for (int f = 0; f < kTiles; ++f)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[f].load(i, row(f, i) + static_cast<int64_t>(col) * kMxElemBytes<T>);
+        for (int i = 0; i < 4; ++i) v.load(i, row(i) + static_cast<int64_t>(col) * kMxElemBytes<T>);
     } else if (cols >= 8) {
 #pragma unroll
-        for (int f = 0; f < kTiles; ++f)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[f].load_end(i, row(f, i), col, cols);
+        for (int i = 0; i < 4; ++i) v.load_end(i, row(i), col, cols);
     } else {
 #pragma unroll
-        for (int f = 0; f < kTiles; ++f)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[f].load_few(i, row(f, i), cols - col);
+        for (int i = 0; i < 4; ++i) v.load_few(i, row(i) + static_cast<int64_t>(col) * kMxElemBytes<T>, cols - col);
     }
-    uint32_t bytes = 0u;
-#pragma unroll
-    for (int f = 0; f < kTiles; ++f) {
-        uint32_t s;
-        const int64_t tile = unit * kTiles + f;
-        *reinterpret_cast<uint4*>(codes + (((tile >> 2) * ksteps + step) * 4 + (tile & 3)) * 1024 + lane * 16) = v[f].quantize(lane, &s);
-        bytes |= s << (8 * f);
-    }
-    if constexpr (kTiles == 4) *reinterpret_cast<uint32_t*>(scales + (unit * ksteps + step) * 256 + lane * 4) = bytes;
-    else scales[((unit >> 2) * ksteps + step) * 256 + lane * 4 + (unit & 3)] = static_cast<uint8_t>(bytes);
+    uint32_t scale;
+    const uint4 q = v.quantize(lane, &scale);
+    const int64_t unit = (tile >> 2) * ksteps + step;
+    *reinterpret_cast<uint4*>(codes + (unit * 4 + (tile & 3)) * 1024 + lane * 16) = q;
+    scales[unit * 256 + lane * 4 + (tile & 3)] = static_cast<uint8_t>(scale);
 }
 
 // Two codes of byte `byte` of w as fp32, times the scale (NaN under scale 255).
@@ -191,19 +180,16 @@ int launched() { return hipGetLastError() == hipSuccess ? FEATHER_OK : FEATHER_E
 int mx_quantize(const void* x, int dtype, int64_t rows, int64_t cols, int64_t row_stride, uint8_t* codes,
                 uint8_t* scales, hipStream_t stream) {
     const int ksteps = static_cast<int>(mx_ksteps(cols));
-    auto go = [&](auto t, auto tiles) {
-        const int64_t units = (rows + 16 * tiles - 1) / (16 * tiles);
-        const unsigned blocks = static_cast<unsigned>((units * ksteps + kWavesPerBlock - 1) / kWavesPerBlock);
-        quantize_kernel<t, tiles><<<blocks, 64 * kWavesPerBlock, 0, stream>>>(
-            static_cast<const uint8_t*>(x), rows, static_cast<int>(cols), row_stride * kMxElemBytes<t>, codes, scales, ksteps, units);
+    const int64_t tiles = (rows + 15) / 16;
+    const unsigned blocks = static_cast<unsigned>((tiles * ksteps + kWavesPerBlock - 1) / kWavesPerBlock);
+    auto go = [&](auto t) {
+        quantize_kernel<t><<<blocks, 64 * kWavesPerBlock, 0, stream>>>(static_cast<const uint8_t*>(x), rows,
+                                                                       static_cast<int>(cols), row_stride * kMxElemBytes<t>,
+                                                                       codes, scales, ksteps, tiles);
     };
-    auto by_rows = [&](auto t) {
-        if (mx_groups(rows) * ksteps < 2048) go(t, std::integral_constant<int, 1>{});
-        else go(t, std::integral_constant<int, 4>{});
-    };
-    if (dtype == kMxF16) by_rows(std::integral_constant<int, kMxF16>{});
-    else if (dtype == kMxBf16) by_rows(std::integral_constant<int, kMxBf16>{});
-    else by_rows(std::integral_constant<int, kMxF32>{});
+    if (dtype == kMxF16) go(std::integral_constant<int, kMxF16>{});
+    else if (dtype == kMxBf16) go(std::integral_constant<int, kMxBf16>{});
+    else go(std::integral_constant<int, kMxF32>{});
     return launched();
 }
 
