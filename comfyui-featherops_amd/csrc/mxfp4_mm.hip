@@ -21,7 +21,18 @@ __device__ __forceinline__ void unrolled(F&& f) {
     unrolled_impl(std::make_integer_sequence<int, N>{}, f);
 }
 
-// 4 bytes per lane from sbase + voff into LDS at lds_addr + 4 * lane (dma16_lds for dwords).
+// dma16_lds, and the same for 4 bytes per lane, with an offset that the instruction adds to both addresses:
+// copies a KB apart in LDS share one M0.
+template <int kOffset>
+__device__ __forceinline__ void dma16_lds_at(const void* sbase, uint32_t voff, uint32_t lds_addr) {
+    static_assert(kOffset >= 0 && kOffset < 4096, "instruction offset");
+    asm volatile(
+        "s_nop 0\n\t"
+        "global_load_lds_dwordx4 %0, %1 offset:%3"
+        :
+        : "v"(voff), "s"(sbase), "{m0}"(lds_addr), "n"(kOffset)
+        : "memory");
+}
 __device__ __forceinline__ void dma4_lds(const void* sbase, uint32_t voff, uint32_t lds_addr) {
     asm volatile(
         "s_nop 0\n\t"
@@ -61,7 +72,7 @@ struct TileArgs {
 // per lane and 64 rows) are copied from HBM into a ring of kStages LDS buffers; a
 // fragment is one contiguous KB in HBM, in LDS and in the wave's ds_read_b128, so
 // there is no swizzle and no bank conflict. Every iteration waits for the stage
-// after the one it multiplies, issues the copies of the stage kStages ahead into the
+// after the one it multiplies, issues the copies of the stage kStages - 1 ahead into the
 // buffer it has emptied, and reads the next stage's fragments into the other half
 // of its fragment registers under this stage's MFMAs. Copies past the last step
 // repeat it, so the wait counts are constants.
@@ -72,12 +83,13 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mx_tile_kernel(const TileArgs
     constexpr int FM = TM / 16, FN = TN / 16;  // its fragments
     constexpr int kGroupsM = BM / 64, kGroupsN = BN / 64;
     constexpr int kCodeCopies = (BM + BN) / 16, kScaleCopies = kGroupsM + kGroupsN;
-    constexpr int kCodes = (kCodeCopies + kWaves - 1) / kWaves, kScales = (kScaleCopies + kWaves - 1) / kWaves;
-    constexpr int kPerWave = kCodes + kScales;  // copies of a stage by every wave (surplus ones repeat the last)
+    constexpr int kCodes = kCodeCopies / kWaves, kScales = (kScaleCopies + kWaves - 1) / kWaves;
+    constexpr int kPerWave = kCodes + kScales;  // copies of a stage by every wave (surplus scales repeat the last)
     constexpr int kStageBytes = kCodeCopies * 1024 + kScaleCopies * 256;
     constexpr int kScaleBase = kCodeCopies * 1024;
     constexpr int SM = (FM + 3) / 4, SN = (FN + 3) / 4;  // scale dwords of the wave's rows and columns
-    static_assert(kStages * kStageBytes <= 160 * 1024, "LDS");
+    static_assert(kStages * kStageBytes <= 160 * 1024 && kStages % 2 == 0, "LDS");
+    static_assert(kCodeCopies % kWaves == 0 && kCodes <= 4, "copies");
     static_assert((kStages - 1) * kPerWave < 64, "vmcnt range");
     static_assert(FM % 2 == 0 && FN % 2 == 0 && (FM % 4 == 0 || FM == 2) && (FN % 4 == 0 || FN == 2), "scale bytes");
     __shared__ __attribute__((aligned(1024))) uint8_t smem[kStages * kStageBytes];
@@ -107,16 +119,16 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mx_tile_kernel(const TileArgs
 
     // This wave's copies: their addresses at step k0. Groups of 64 rows past an operand's end read its last one.
     const uint8_t* src[kPerWave];
-    uint32_t dst[kPerWave];
     const uint32_t lds = lds_addr_of(smem);
+    const uint32_t code_dst = lds + wave * (kCodes * 1024);
+    uint32_t scale_dst[kScales];
 #pragma unroll
     for (int i = 0; i < kCodes; ++i) {
-        const int j = min(i * kWaves + wave, kCodeCopies - 1);
+        const int j = wave * kCodes + i;
         const bool is_a = j < BM / 16;
         const int f = is_a ? j : j - BM / 16;
         const int64_t g = is_a ? min(static_cast<int>(m0 / 64) + f / 4, p.a_groups - 1) : min(n0 / 64 + f / 4, p.b_groups - 1);
-        src[i] = scalar_pointer((is_a ? p.a : p.b) + ((g * p.ksteps + k0) * 4 + f % 4) * 1024);
-        dst[i] = lds + j * 1024;
+        src[i] = scalar_pointer((is_a ? p.a : p.b) + ((g * p.ksteps + k0) * 4 + f % 4) * 1024 - i * 1024);  // (see copy)
     }
 #pragma unroll
     for (int i = 0; i < kScales; ++i) {
@@ -124,12 +136,12 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mx_tile_kernel(const TileArgs
         const bool is_a = j < kGroupsM;
         const int64_t g = is_a ? min(static_cast<int>(m0 / 64) + j, p.a_groups - 1) : min(n0 / 64 + j - kGroupsM, p.b_groups - 1);
         src[kCodes + i] = scalar_pointer((is_a ? p.as : p.bs) + (g * p.ksteps + k0) * 256);
-        dst[kCodes + i] = lds + kScaleBase + j * 256;
+        scale_dst[i] = lds + kScaleBase + j * 256;
     }
     // (the step in the lane's offset, one instruction for all copies, not in each copy's address)
-    auto copy = [&](auto i, int step, int slot_bytes) {
-        if constexpr (i < kCodes) dma16_lds(src[i], lane * 16 + step * 4096, dst[i] + slot_bytes);
-        else dma4_lds(src[i], lane * 4 + step * 256, dst[i] + slot_bytes);
+    auto copy = [&](auto i, int step, int slot) {
+        if constexpr (i < kCodes) dma16_lds_at<i * 1024>(src[i], lane * 16 + step * 4096, code_dst + slot * kStageBytes);
+        else dma4_lds(src[i], lane * 4 + step * 256, scale_dst[i - kCodes] + slot * kStageBytes);
     };
 
     struct Frags {
@@ -140,11 +152,9 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mx_tile_kernel(const TileArgs
     auto read = [&](auto r, Frags& f, const uint8_t* base) {
         if constexpr (r < SN) {
             f.sb[r] = *reinterpret_cast<const uint32_t*>(base + kScaleBase + (kGroupsM + wn * TN / 64 + r) * 256 + lane * 4);
-            if constexpr (FN == 2) f.sb[r] >>= 16 * (wn % 2);
         } else if constexpr (r < SN + SM) {
             constexpr int i = r - SN;
             f.sa[i] = *reinterpret_cast<const uint32_t*>(base + kScaleBase + (wm * TM / 64 + i) * 256 + lane * 4);
-            if constexpr (FM == 2) f.sa[i] >>= 16 * (wm % 2);
         } else if constexpr (r < SN + SM + FN) {
             constexpr int i = r - SN - SM;
             f.b[i] = *reinterpret_cast<const uint4*>(base + (BM / 16 + wn * FN + i) * 1024 + lane * 16);
@@ -159,27 +169,30 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mx_tile_kernel(const TileArgs
     for (int i = 0; i < FM; ++i)
 #pragma unroll
         for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    // (half a group's scales are moved down where they are used: beside the read they would wait for it)
     auto multiply = [&](auto n, const Frags& f) {
         constexpr int i = n / FN, j = n % FN;
-        acc[i][j] = mfma_mx<j % 4, i % 4>(f.b[j], f.a[i], acc[i][j], f.sb[j / 4], f.sa[i / 4]);
+        const uint32_t sb = FN == 2 ? f.sb[0] >> (16 * (wn % 2)) : f.sb[j / 4];
+        const uint32_t sa = FM == 2 ? f.sa[0] >> (16 * (wm % 2)) : f.sa[i / 4];
+        acc[i][j] = mfma_mx<j % 4, i % 4>(f.b[j], f.a[i], acc[i][j], sb, sa);
     };
 
 #pragma unroll
-    for (int s = 0; s < kStages - 1; ++s) unrolled<kPerWave>([&](auto i) { copy(i, min(s, steps - 1), s * kStageBytes); });
+    for (int s = 0; s < kStages - 1; ++s) unrolled<kPerWave>([&](auto i) { copy(i, min(s, steps - 1), s); });
     Frags f0, f1;
     wait_vmcnt<(kStages - 2) * kPerWave>();
     stage_barrier();
     unrolled<kReads>([&](auto r) { read(r, f0, smem); });
-    int slot = 0;  // of the step being multiplied, in bytes as are the others
-    // One step. The copies and the next step's reads are pinned between the MFMAs, all of them in the
+    // One step, in ring buffer `slot`. The loop below goes round the ring, so that buffers' addresses are
+    // constants (256 x 256: 70.9 -> 68.5 us at M 4096, N = K = 5120; the small tiles the same).
+    // The copies and the next step's reads are pinned between the MFMAs, all of them in the
     // first three quarters: left alone, the compiler reads each fragment into the registers of the one
     // just used up, after its last MFMA, and every step waits for LDS with the matrix cores idle.
     constexpr int kMfmas = FM * FN, kOps = kPerWave + kReads, kOver = kMfmas >= 8 ? kMfmas * 3 / 4 : kMfmas;
-    auto iterate = [&](int k, const Frags& now, Frags& next) {
-        const int after = slot == (kStages - 1) * kStageBytes ? 0 : slot + kStageBytes;
-        const int free_slot = slot == 0 ? (kStages - 1) * kStageBytes : slot - kStageBytes;
+    auto iterate = [&](auto slot, int k, const Frags& now, Frags& next) {
+        constexpr int kAfter = (slot + 1) % kStages, kFree = (slot + kStages - 1) % kStages;
         const int ahead = min(k + kStages - 1, steps - 1);
-        const uint8_t* base = smem + after;
+        const uint8_t* base = smem + kAfter * kStageBytes;
         // Stage k + 1 has landed; the buffer of stage k - 1 is free: the MFMAs of that step, which are
         // issued, waited for its reads. The reads of stage k may still be under way.
         wait_vmcnt<(kStages - 3) * kPerWave>();
@@ -190,19 +203,19 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mx_tile_kernel(const TileArgs
             unrolled<last - first>([&](auto o) {
                 // the copies in even steps among the reads
                 constexpr int op = first + o, copies = (op + 1) * kPerWave / kOps, before = op * kPerWave / kOps;
-                if constexpr (copies > before) copy(std::integral_constant<int, before>{}, ahead, free_slot);
+                if constexpr (copies > before) copy(std::integral_constant<int, before>{}, ahead, kFree);
                 else read(std::integral_constant<int, op - before>{}, next, base);
             });
             __builtin_amdgcn_sched_barrier(0);
         });
-        slot = after;
     };
-    int k = 0;
-    for (; k + 1 < steps; k += 2) {
-        iterate(k, f0, f1);
-        iterate(k + 1, f1, f0);
+    for (int k = 0; k < steps; k += kStages) {
+        unrolled<kStages>([&](auto slot) {
+            if (k + slot >= steps) return;
+            if constexpr (slot % 2 == 0) iterate(slot, k + slot, f0, f1);
+            else iterate(slot, k + slot, f1, f0);
+        });
     }
-    if (k < steps) unrolled<kMfmas>([&](auto n) { multiply(n, f0); });
     wait_vmcnt<0>();
 
     const int lm = lane & 15;
@@ -306,7 +319,7 @@ constexpr Tile kTiles[] = {
     {64, 128, 2, 3.7, 0.16, 0.23, 0.37, 0},
     {128, 128, 2, 4.5, 0.27, 0.36, 0.58, 0},
     {128, 256, 1, 5.4, 0.38, 0.57, 0, 0},
-    {256, 256, 1, 6.7, 0.55, 0.93, 0, 0},
+    {256, 256, 1, 6.7, 0.47, 0.93, 0, 0},
 };
 constexpr int kNumTiles = 6, kLargest = 5;
 constexpr int kCus = 256;
