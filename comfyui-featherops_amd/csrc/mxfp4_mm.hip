@@ -1,5 +1,12 @@
 // C (M, N) = A (M, K) . B (N, K)^T + bias with both operands packed MXFP4
 // (mxfp4.h), on the block-scaled 16x16x128 MFMA with fp32 accumulators.
+//
+// Bounds, measured (MI355X, packed operands, weights from HBM):
+//   one row of the largest tile on every CU and more: the matrix cores at the clock that the power allows. The
+//   instruction alone sustains 6.4 to 7.1 PFLOP/s; (16384, 5120, 13824) runs at 5.0, (32768, 13824, 5120) at 4.4,
+//   of which the stores of a tile, 128 KB a CU that no other tile's work covers, take 11%.
+//   up to some hundred rows: the operands' way from HBM through one workgroup's ring, 50 to 60 GB/s a CU, in one
+//   round of workgroups: (154, 10240, 4096) 11.2 us with 22 MB of weights, (1024, 5120, 5120) 21.5 us.
 #include <algorithm>
 #include <type_traits>
 #include <utility>
@@ -323,6 +330,10 @@ constexpr Tile kTiles[] = {
 };
 constexpr int kNumTiles = 6, kLargest = 5;
 constexpr int kCus = 256;
+// Tile rows the raster walks at a time: an XCD's 32 workgroups of the largest tile then cover about as many rows
+// as columns. 4, 6, 8 at (32768, 13824, 5120): 1095, 1050, 1113 us; (2048, 5120, 5120) in 64 x 128 tiles: 46.7,
+// 43.0, 44.9; M = 1024 the same within 2%.
+constexpr int kRasterRows = 6;
 
 int64_t tiles_of(int64_t n, int t) { return (n + t - 1) / t; }
 
@@ -412,7 +423,7 @@ int run(const MxMmArgs& p, Choice c, int64_t m0, int64_t n0, int64_t M, int64_t 
                      p.bias ? p.bias + n0 : nullptr, p.c + m0 * p.N + n0, M - m0, p.N, static_cast<int>(N - n0),
                      static_cast<int>(ksteps), static_cast<int>(mx_groups(p.M) - m0 / 64),
                      static_cast<int>(mx_groups(p.N) - n0 / 64), static_cast<int>(tiles_m), static_cast<int>(tiles_n),
-                     c.ksplit, 4, reinterpret_cast<uint32_t*>(p.ws), reinterpret_cast<float*>(p.ws + kMxCounterBytes)};
+                     c.ksplit, kRasterRows, reinterpret_cast<uint32_t*>(p.ws), reinterpret_cast<float*>(p.ws + kMxCounterBytes)};
     switch (c.tile) {
         case 1: launch<64, 64, 2, 2, 6>(a, p.out_bf16, stream); break;
         case 2: launch<64, 128, 2, 2, 6>(a, p.out_bf16, stream); break;

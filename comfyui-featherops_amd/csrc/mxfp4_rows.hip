@@ -2,7 +2,9 @@
 // bound by streaming the weight once. 16-bit activations are quantised on the way
 // into the matrix instruction (MxPieces: ~85 instructions a K step, beside the 1 to 4 KB of
 // weights that the wave waits for); a launch of its own for the quantisation would cost
-// more than that of one token's product.
+// more than that of one token's product. One row and N = 13824, K = 5120 (37.6 MB) takes 8.7 us
+// on the GPU, 4.3 TB/s with the launch; 16 rows and N = K = 4096 (8.9 MB) 6.0 us, of which some
+// 3 are the launch, the first load's way and the join of the eight waves.
 #include <algorithm>
 #include <type_traits>
 #include <utility>
