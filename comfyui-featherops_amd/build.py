@@ -102,7 +102,7 @@ def build_torch_ops() -> Path:
     with ThreadPoolExecutor(max_workers=len(sources)) as ex:
         list(ex.map(lambda so: _run([*cmd, "-c", str(so[0]), "-o", str(so[1])]), zip(sources, objects)))
     tmp = OPS_LIB_PATH.with_suffix(".so.tmp")
-    _run([cmd[0], "-shared", *map(str, objects), f"-L{torch_lib}", "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch",
+    _run([cmd[0], "-shared", *map(str, objects), f"-L{torch_lib}", "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_hip", "-ltorch",
           f"-L{LIB_DIR}", "-lfeatherops_amd", "-Wl,-rpath,$ORIGIN", "-o", str(tmp)])
     os.replace(tmp, OPS_LIB_PATH)
     return OPS_LIB_PATH

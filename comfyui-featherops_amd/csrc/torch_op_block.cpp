@@ -8,6 +8,7 @@
 // stream of the first tensor's device. Views whose rows have one stride are read in
 // place, others are made contiguous first.
 #include <ATen/ATen.h>
+#include <ATen/hip/EmptyTensor.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/library.h>
@@ -36,6 +37,12 @@ int value_code(at::ScalarType t, const char* what) {
         default: TORCH_CHECK(false, what, " must be float16, bfloat16 or float32, got ", t);
     }
     return -1;
+}
+
+// at::empty on `like`'s device; on the GPU without another round through the dispatcher.
+at::Tensor empty_on(const at::Tensor& like, at::IntArrayRef shape, at::ScalarType dtype) {
+    if (!like.is_cuda()) return at::empty(shape, like.options().dtype(dtype));
+    return at::Tensor(at::detail::empty_cuda(shape, dtype, like.device(), std::nullopt));
 }
 
 // t as rows of `cols` contiguous values with one stride between them: in place where its strides
@@ -67,7 +74,7 @@ int64_t packed_units(int64_t rows, int64_t cols) { return (rows + 63) / 64 * ((c
 
 Packed empty_packed(int64_t rows, int64_t cols, const at::Tensor& like) {
     const int64_t units = packed_units(rows, cols);
-    return {at::empty({units * 4352}, like.options().dtype(at::kByte)), units * 4096};
+    return {empty_on(like, {units * 4352}, at::kByte), units * 4096};
 }
 
 Packed check_packed(const at::Tensor& data, int64_t rows, int64_t cols, const char* what) {
@@ -111,7 +118,7 @@ at::Tensor dequantize_mxfp4(const at::Tensor& data, at::IntArrayRef shape, at::S
     const Packed q = check_packed(data, rows, cols, "q");
     const int code = value_code(dtype, "dtype");
     const c10::DeviceGuard guard(data.device());
-    const at::Tensor out = at::empty(shape, data.options().dtype(dtype));
+    const at::Tensor out = empty_on(data, shape, dtype);
     check_status(feather_mxfp4_dequantize(q.codes(), q.scales(), out.data_ptr(), code, rows, cols, stream_of(data)),
                  "dequantize_mxfp4");
     return out;
@@ -160,7 +167,7 @@ at::Tensor run_mm(const void* a, const uint8_t* a_scales, int a_dtype, int64_t a
                   const OptTensor& bias, at::IntArrayRef shape, int64_t K, at::ScalarType out_dtype) {
     const hipStream_t stream = stream_of(b.data);
     const int64_t M = rows_of(shape), N = shape.back();
-    const at::Tensor c = at::empty(shape, b.data.options().dtype(out_dtype));
+    const at::Tensor c = empty_on(b.data, shape, out_dtype);
     const size_t ws_bytes = feather_mxfp4_mm_workspace_size(M, N, K, a_dtype);
     at::Tensor ws;
     if (ws_bytes) ws = feather::workspace_for(b.data.device(), stream, ws_bytes);
@@ -292,9 +299,9 @@ NormOut run_norm(const at::Tensor& x, const OptTensor& h, const OptTensor& gate,
     if (bias.has_value()) b = column_vector(x, *bias, mods, "bias");
 
     NormOut out;
-    if (h.has_value()) out.stream = at::empty(x.sizes(), x.options());
+    if (h.has_value()) out.stream = empty_on(x, x.sizes(), x.scalar_type());
     if (codes) out.q = empty_packed(rows, cols, x);
-    else out.y = at::empty(x.sizes(), x.options().dtype(block));
+    else out.y = empty_on(x, x.sizes(), block);
     feather_block_norm_args a{};
     a.x = xr.p;
     a.h = hr.p;
