@@ -316,17 +316,17 @@ struct Tile {
     double base;  // us of a launch with next to no K
     double lo, one, two, three;  // us per K step: few workgroups, one, two, three on every CU
 };
-// Tiles of the plan (ids 1..) and their measured times: MI355X, packed operands, weights from HBM,
-// M 64 .. 32768, N 2317 .. 13824, K 640 .. 14336. Small tiles fill the chip where there are few rows;
-// large ones read each operand fewer times (a CU takes ~50 GB/s per tile from beyond its L2 whatever the
-// ring's depth), and at 256 x 256 the matrix cores are the bound.
+// Tiles of the plan (ids 1..) and their times, MI355X, packed operands. The constants are those with which the
+// pick came nearest to the fastest of all tiles and splits, over 330 shapes (M 33 .. 6000, N 256 .. 16384, K 256 ..
+// 16384), each with the weight in HBM and in the caches: 1.4% and 1.3% above it in the geometric mean, 21% and 18% at
+// most. Small tiles fill the chip where there are few rows; large ones read each operand fewer times.
 constexpr Tile kTiles[] = {
     {0, 0, 0, 0, 0, 0, 0, 0},
-    {64, 64, 3, 3.2, 0.15, 0.20, 0.29, 0.345},
-    {64, 128, 2, 3.7, 0.16, 0.23, 0.37, 0},
-    {128, 128, 2, 4.5, 0.27, 0.36, 0.58, 0},
-    {128, 256, 1, 5.4, 0.38, 0.57, 0, 0},
-    {256, 256, 1, 6.7, 0.47, 0.93, 0, 0},
+    {64, 64, 3, 4.1, 0.12, 0.16, 0.35, 0.42},
+    {64, 128, 2, 4.2, 0.176, 0.23, 0.37, 0},
+    {128, 128, 2, 4.1, 0.316, 0.36, 0.57, 0},
+    {128, 256, 1, 5.4, 0.38, 0.54, 0, 0},
+    {256, 256, 1, 6.4, 0.49, 0.93, 0, 0},
 };
 constexpr int kNumTiles = 6, kLargest = 5;
 constexpr int kCus = 256;
@@ -364,7 +364,7 @@ Choice choose(int64_t M, int64_t N, int64_t ksteps) {
             // arrival counters' 64 KB); it costs the exchange of the partial sums
             if (ks > 1 && (ksteps / ks < 8 || tiles * ks > kCus * t.per_cu)) break;
             double time = tile_time(t, tiles * ks, static_cast<double>((ksteps + ks - 1) / ks));
-            if (ks > 1) time += 0.8 + static_cast<double>(tiles * ks) * t.bm * t.bn * 8 / 5e6;
+            if (ks > 1) time += 1.2 + static_cast<double>(tiles * ks) * t.bm * t.bn * 8 / 4.6e6;
             if (time < best.time) best = {id, ks, time};
         }
     }
