@@ -4,7 +4,8 @@
 hook, the 4-bit sibling of `feather_ops`. Its `Linear`:
   * at state-dict load quantizes the weight to packed MXFP4 on the GPU, or lays out one that the
     checkpoint holds in MXFP4 already (uint8 codes (N, blocks * 16) with uint8 `weight_scale` (N, blocks)),
-    unless the layer is excluded or 1-wide;
+    unless the layer is excluded or 1-wide. A `weight_scale` or `scale_weight` beside a weight in floating
+    point (fp8 checkpoints, one scale or one per row) is multiplied in first;
   * in forward runs mxfp4_mm with the bias; activations in fp16 or bf16 (fp32 is cast to bf16), or an
     MXFP4Tensor that a norm left in 4 bits (kernel.hip.norm, out_dtype="mxfp4"), and applies basic LoRA
     patches as a separate pass over activations that are not in 4 bits;
@@ -28,6 +29,16 @@ def _on_gpu(t: torch.Tensor) -> torch.Tensor:
     return t if t.is_cuda else t.to("cuda")
 
 
+def _scaled(weight: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
+    """The fp32 values that a checkpoint's weight and its scale (one, or one per row) stand for."""
+    scale = scale.to(device=weight.device, dtype=torch.float32)
+    if scale.numel() == 1:
+        scale = scale.reshape(())
+    elif weight.ndim != 2 or scale.shape != (weight.shape[0], 1):
+        raise ValueError(f"weight scale must be one number or ({weight.shape[0]}, 1), got {tuple(scale.shape)}")
+    return weight.to(torch.float32) * scale
+
+
 def mxfp4_ops(out_dtype=torch.bfloat16, excluded_names=()):
     excluded_names = tuple(excluded_names)
 
@@ -47,6 +58,8 @@ def mxfp4_ops(out_dtype=torch.bfloat16, excluded_names=()):
                 weight = state_dict.pop(prefix + "weight", None)
                 bias = state_dict.pop(prefix + "bias", None)
                 scales = state_dict.pop(prefix + "weight_scale", None)
+                if scales is None:
+                    scales = state_dict.pop(prefix + "scale_weight", None)
                 if weight is None:
                     missing_keys.append(prefix + "weight")
                 elif scales is not None and weight.dtype == torch.uint8:
@@ -54,9 +67,16 @@ def mxfp4_ops(out_dtype=torch.bfloat16, excluded_names=()):
                 elif (any(x in prefix for x in self.excluded_names) or weight.ndim == 1 or self.in_features == 1
                       or self.out_features == 1):
                     self.mx_weight = None
+                    if scales is not None:  # (an 8-bit float cannot hold the product: the layer's type does)
+                        weight = _scaled(weight, scales).to(weight.dtype if weight.element_size() > 1 else self.out_dtype)
                     self.weight = nn.Parameter(weight, requires_grad=False)
                 else:
-                    self._hold(quantize_mxfp4(_on_gpu(weight)))
+                    weight = _on_gpu(weight)
+                    if scales is not None:
+                        weight = _scaled(weight, scales)
+                    elif weight.element_size() == 1 and weight.is_floating_point():  # (8-bit floats: bf16 holds all of their values)
+                        weight = weight.to(torch.bfloat16)
+                    self._hold(quantize_mxfp4(weight))
                 self.bias = None if bias is None else nn.Parameter(bias.to(self.out_dtype), requires_grad=False)
 
             def _hold(self, weight: MXFP4Tensor) -> None:

@@ -1,0 +1,44 @@
+"""How weights and biases get into the MXFP4 Linear and out of it, on the GPU."""
+
+import importlib
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+F8 = torch.float8_e4m3fn
+
+
+@pytest.fixture(scope="module")
+def mx(pkg):
+    return importlib.import_module("featherops_amd.kernel.hip.mxfp4")
+
+
+@pytest.fixture(scope="module")
+def ops(pkg):
+    return importlib.import_module("featherops_amd.comfy_feather.mxfp4").mxfp4_ops
+
+
+def load(ops, state, n, k, out=torch.bfloat16):
+    with torch.device("meta"):
+        linear = ops(out).Linear(k, n, bias="bias" in state)
+    top = torch.nn.Module()
+    top.add_module("up", linear)
+    top.load_state_dict({"up." + key: v for key, v in state.items()})
+    return linear
+
+
+def some(*shape, dtype=torch.bfloat16, seed=0, std=1.0):
+    return (torch.randn(*shape, generator=torch.Generator().manual_seed(seed)) * std).to(dtype)
+
+
+@pytest.mark.parametrize("where", ["cpu", "cuda"])
+@pytest.mark.parametrize("dtype", [F8, torch.bfloat16, torch.float32])
+def test_scaled_checkpoint(ops, mx, cuda, dtype, where):
+    """One scale, and one per row: the layer's weight is the quantised product."""
+    weight = some(70, 200, dtype=dtype)
+    x = some(5, 200, seed=1).to(cuda)
+    for scale in (torch.tensor(0.003), some(70, 1, dtype=torch.float32, seed=2).abs()):
+        linear = load(ops, {"weight": weight.to(where), "weight_scale": scale.to(where)}, 70, 200)
+        want = mx.quantize_mxfp4((weight.float() * scale).to(cuda))
+        assert torch.equal(linear(x), mx.mxfp4_mm(x, want))

@@ -1,0 +1,75 @@
+"""CPU tests of the MXFP4 Linear's bookkeeping, with the library's kernels replaced by stand-ins that record what they
+are given. No kernel runs."""
+
+import importlib
+
+import pytest
+import torch
+
+
+@pytest.fixture(scope="module")
+def layer_module(pkg):
+    return importlib.import_module("featherops_amd.comfy_feather.mxfp4")
+
+
+@pytest.fixture
+def seen(layer_module, monkeypatch):
+    """What quantize_mxfp4 was given, in order; its result is a packed operand of zeros."""
+    given = []
+
+    def quantize(x):
+        given.append(x)
+        rows, cols = x.shape
+        data = torch.zeros(-(-rows // 64) * -(-cols // 128) * 4352, dtype=torch.uint8)
+        return layer_module.MXFP4Tensor(data, tuple(x.shape))
+
+    monkeypatch.setattr(layer_module, "quantize_mxfp4", quantize)
+    monkeypatch.setattr(layer_module, "_on_gpu", lambda t: t)
+    return given
+
+
+def load(layer_module, state, n, k, out=torch.bfloat16, excluded=(), strict=True):
+    with torch.device("meta"):
+        linear = layer_module.mxfp4_ops(out, excluded).Linear(k, n, bias="bias" in state)
+    top = torch.nn.Module()
+    top.add_module("up", linear)
+    top.load_state_dict({"up." + key: v for key, v in state.items()}, strict=strict)
+    return linear
+
+
+F8 = torch.float8_e4m3fn
+
+
+@pytest.mark.parametrize("key", ["weight_scale", "scale_weight"])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32, F8, torch.float8_e5m2])
+def test_checkpoint_scale_reaches_the_quantiser(layer_module, seen, key, dtype):
+    g = torch.Generator().manual_seed(0)
+    weight = torch.randn(5, 64, generator=g).to(dtype)
+    for scale in (torch.tensor(0.0125), torch.tensor([0.0125]), torch.rand(5, 1, generator=g)):
+        load(layer_module, {"weight": weight, key: scale}, 5, 64)
+        assert torch.equal(seen.pop(), weight.float() * scale)  # as the 8-bit layer: in fp32, one rounding
+
+
+@pytest.mark.parametrize("dtype", [F8, torch.float8_e5m2])
+def test_unscaled_fp8_weight(layer_module, seen, dtype):
+    weight = torch.randn(4, 64, generator=torch.Generator().manual_seed(1)).to(dtype)
+    load(layer_module, {"weight": weight}, 4, 64)
+    assert torch.equal(seen.pop().float(), weight.float())
+
+
+def test_scale_of_an_excluded_layer(layer_module, seen):
+    weight, scale = torch.randn(4, 64, generator=torch.Generator().manual_seed(2)), torch.tensor(0.25)
+    for dtype, held in ((F8, torch.bfloat16), (torch.float16, torch.float16), (torch.float32, torch.float32)):
+        linear = load(layer_module, {"weight": weight.to(dtype), "weight_scale": scale}, 4, 64, excluded=("up",))
+        assert linear.weight.dtype == held
+        assert torch.equal(linear.weight.data.float(), weight.to(dtype).float() * scale)  # (a power of two: exact)
+    linear = load(layer_module, {"weight": weight.half()}, 4, 64, excluded=("up",))
+    assert torch.equal(linear.weight.data, weight.half()) and not seen
+
+
+def test_scale_refusals(layer_module, seen):
+    weight = torch.zeros(4, 64, dtype=torch.bfloat16)
+    for scale in (torch.ones(4), torch.ones(1, 64), torch.ones(3, 1), torch.ones(4, 2)):
+        with pytest.raises(ValueError, match="weight scale must be"):
+            load(layer_module, {"weight": weight, "weight_scale": scale}, 4, 64)
+    assert not seen
