@@ -11,6 +11,9 @@ hook, the 4-bit sibling of `feather_ops`. Its `Linear`:
     patches as a separate pass over activations that are not in 4 bits;
   * converts the weight back for a merge (convert_weight) and takes the merged one (set_weight).
 
+A quantized layer's `weight` parameter is its packed operand (uint8, codes and scales), so that whatever moves, sizes or
+backs up parameters finds it; `mx_weight` is the same as an MXFP4Tensor, None for a layer that is not quantized.
+
 Inside ComfyUI it subclasses comfy.ops.manual_cast; without it the stand-in of `ops.py`.
 """
 
@@ -51,7 +54,11 @@ def mxfp4_ops(out_dtype=torch.bfloat16, excluded_names=()):
                 super().__init__(*args, **kwargs)
                 self.excluded_names = MXFP4Ops._excluded_names
                 self.out_dtype = MXFP4Ops._out_dtype
-                self.mx_weight: MXFP4Tensor | None = None
+                self.is_quantized = False
+
+            @property
+            def mx_weight(self) -> MXFP4Tensor | None:
+                return MXFP4Tensor(self.weight, (self.out_features, self.in_features)) if self.is_quantized else None
 
             def _load_from_state_dict(self, state_dict, prefix, local_metadata, strict, missing_keys,
                                       unexpected_keys, error_msgs):
@@ -66,7 +73,7 @@ def mxfp4_ops(out_dtype=torch.bfloat16, excluded_names=()):
                     self._hold(prepack_mxfp4(_on_gpu(weight), _on_gpu(scales), self.in_features))
                 elif (any(x in prefix for x in self.excluded_names) or weight.ndim == 1 or self.in_features == 1
                       or self.out_features == 1):
-                    self.mx_weight = None
+                    self.is_quantized = False
                     if scales is not None:  # (an 8-bit float cannot hold the product: the layer's type does)
                         weight = _scaled(weight, scales).to(weight.dtype if weight.element_size() > 1 else self.out_dtype)
                     self.weight = nn.Parameter(weight, requires_grad=False)
@@ -82,29 +89,39 @@ def mxfp4_ops(out_dtype=torch.bfloat16, excluded_names=()):
             def _hold(self, weight: MXFP4Tensor) -> None:
                 if weight.shape != (self.out_features, self.in_features):
                     raise ValueError(f"expected a ({self.out_features}, {self.in_features}) weight, got {weight.shape}")
-                self.mx_weight = weight
-                self.weight = None
+                self.is_quantized = True
+                self.weight = nn.Parameter(weight.data, requires_grad=False)
 
             def _save_to_state_dict(self, destination, prefix, keep_vars):
                 super()._save_to_state_dict(destination, prefix, keep_vars)
-                if self.mx_weight is not None:
+                if self.is_quantized:
                     destination[prefix + "weight"], destination[prefix + "weight_scale"] = unprepack_mxfp4(self.mx_weight)
 
             def _apply(self, fn, recurse=True):
-                super()._apply(fn, recurse)
-                if self.mx_weight is not None:  # bytes: moved between devices, never cast
-                    moved = fn(self.mx_weight.data)
-                    self.mx_weight = self.mx_weight._replace(data=moved if moved.dtype == torch.uint8
-                                                             else self.mx_weight.data.to(moved.device))
-                return self
+                def keep_bytes(t):  # the packed operand is moved between devices, never cast
+                    moved = fn(t)
+                    return moved if t.dtype != torch.uint8 or moved.dtype == torch.uint8 else t.to(moved.device)
+
+                return super()._apply(keep_bytes, recurse)
 
             def convert_weight(self, weight=None, inplace=False, **kwargs):
-                if self.mx_weight is None:
+                """The values, in the layer's output dtype, of `weight`: a packed operand as `weight` and `mx_weight`
+                hold it and set_weight(return_weight=True) returns it; by default the layer's own."""
+                if not self.is_quantized:
                     return self.weight if weight is None else weight
-                return dequantize_mxfp4(self.mx_weight, self.out_dtype)
+                shape = (self.out_features, self.in_features)
+                if weight is None:
+                    weight = self.weight
+                if not isinstance(weight, MXFP4Tensor):
+                    if not isinstance(weight, torch.Tensor) or weight.dtype != torch.uint8 or weight.ndim != 1:
+                        raise TypeError(f"expected a packed MXFP4 weight, got {getattr(weight, 'dtype', type(weight).__name__)}")
+                    weight = MXFP4Tensor(weight, shape)
+                if weight.shape != shape:
+                    raise ValueError(f"expected a {shape} weight, got {weight.shape}")
+                return dequantize_mxfp4(weight, self.out_dtype)
 
             def set_weight(self, weight, inplace_update=False, seed=None, return_weight=False, **kwargs):
-                if self.mx_weight is None:
+                if not self.is_quantized:
                     weight = weight.to(self.weight.dtype)
                     if return_weight:
                         return weight
@@ -119,7 +136,7 @@ def mxfp4_ops(out_dtype=torch.bfloat16, excluded_names=()):
 
             def forward(self, x: torch.Tensor | MXFP4Tensor) -> torch.Tensor:
                 run_every_op()
-                if self.mx_weight is None:
+                if not self.is_quantized:
                     weight, bias, offload_stream = cast_bias_weight(self, x, offloadable=True)
                     y = F.linear(x, weight, bias)
                     uncast_bias_weight(self, weight, bias, offload_stream)

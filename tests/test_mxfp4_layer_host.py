@@ -73,3 +73,40 @@ def test_scale_refusals(layer_module, seen):
         with pytest.raises(ValueError, match="weight scale must be"):
             load(layer_module, {"weight": weight, "weight_scale": scale}, 4, 64)
     assert not seen
+
+
+@pytest.fixture
+def codec(layer_module, seen, monkeypatch):
+    """Dequantisation that marks its result with the operand's first byte."""
+    monkeypatch.setattr(layer_module, "dequantize_mxfp4",
+                        lambda q, dtype: torch.full(q.shape, float(q.data[0]), dtype=dtype, device="cpu"))
+
+
+def test_weight_is_the_packed_operand(layer_module, seen):
+    """Whatever reads, sizes, moves or restores a parameter finds the packed bytes."""
+    linear = load(layer_module, {"weight": torch.zeros(70, 200)}, 70, 200)
+    assert isinstance(linear.weight, torch.nn.Parameter) and dict(linear.named_parameters())["weight"] is linear.weight
+    assert linear.weight.dtype == torch.uint8 and linear.weight.shape == (2 * 2 * 4352,) and not linear.weight.requires_grad
+    assert linear.mx_weight.shape == (70, 200) and linear.mx_weight.data.data_ptr() == linear.weight.data_ptr()
+    backup = linear.weight.detach().clone()
+    backup[0] = 7
+    linear.weight = torch.nn.Parameter(backup, requires_grad=False)
+    assert linear.mx_weight.data[0] == 7
+    for cast in (lambda m: m.to(torch.float16), lambda m: m.half(), lambda m: m.float(), lambda m: m.type(torch.float64)):
+        cast(linear)
+        assert linear.weight.dtype == torch.uint8 and linear.weight[0] == 7
+    assert linear.to("meta").weight.device.type == "meta"
+
+
+def test_convert_weight_converts_its_argument(layer_module, codec):
+    linear = load(layer_module, {"weight": torch.zeros(4, 64)}, 4, 64)
+    new = linear.set_weight(torch.ones(4, 64), return_weight=True)
+    new.data[0] = 3
+    for weight, first in ((new, 3), (new.data, 3), (linear.weight, 0), (linear.mx_weight, 0), (None, 0)):
+        values = linear.convert_weight(weight)
+        assert values.dtype == torch.bfloat16 and values.shape == (4, 64) and (values == first).all()
+    for other in (torch.zeros(4, 64), torch.zeros(4, 64, dtype=torch.uint8), "weight"):
+        with pytest.raises(TypeError, match="packed MXFP4 weight"):
+            linear.convert_weight(other)
+    with pytest.raises(ValueError, match="expected a"):
+        linear.convert_weight(new._replace(shape=(64, 4)))
