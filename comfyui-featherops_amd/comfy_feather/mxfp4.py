@@ -12,7 +12,9 @@ hook, the 4-bit sibling of `feather_ops`. Its `Linear`:
   * converts the weight back for a merge (convert_weight) and takes the merged one (set_weight).
 
 A quantized layer's `weight` parameter is its packed operand (uint8, codes and scales), so that whatever moves, sizes or
-backs up parameters finds it; `mx_weight` is the same as an MXFP4Tensor, None for a layer that is not quantized.
+backs up parameters finds it; `mx_weight` is the same as an MXFP4Tensor, None for a layer that is not quantized. The
+layer may lie in host memory: conversions run on the GPU and their results come back to where the weight is. A
+state dict holds the row-major codes and scales, a copy of the weight's size for as long as the dict lives.
 
 Inside ComfyUI it subclasses comfy.ops.manual_cast; without it the stand-in of `ops.py`.
 """
@@ -29,7 +31,7 @@ from .ops import cast_bias_weight, manual_cast, run_every_op, uncast_bias_weight
 
 
 def _on_gpu(t: torch.Tensor) -> torch.Tensor:
-    return t if t.is_cuda else t.to("cuda")
+    return t if t.is_cuda or t.is_meta else t.to("cuda")
 
 
 def _scaled(weight: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
@@ -92,10 +94,16 @@ def mxfp4_ops(out_dtype=torch.bfloat16, excluded_names=()):
                 self.is_quantized = True
                 self.weight = nn.Parameter(weight.data, requires_grad=False)
 
+            def _operand(self, data: torch.Tensor) -> MXFP4Tensor:
+                """A packed operand's bytes, wherever they lie, for the kernels."""
+                return MXFP4Tensor(_on_gpu(data), (self.out_features, self.in_features))
+
             def _save_to_state_dict(self, destination, prefix, keep_vars):
                 super()._save_to_state_dict(destination, prefix, keep_vars)
                 if self.is_quantized:
-                    destination[prefix + "weight"], destination[prefix + "weight_scale"] = unprepack_mxfp4(self.mx_weight)
+                    codes = unprepack_mxfp4(self._operand(self.weight))
+                    for name, t in zip(("weight", "weight_scale"), codes):
+                        destination[prefix + name] = t.to(self.weight.device)
 
             def _apply(self, fn, recurse=True):
                 def keep_bytes(t):  # the packed operand is moved between devices, never cast
@@ -109,16 +117,15 @@ def mxfp4_ops(out_dtype=torch.bfloat16, excluded_names=()):
                 hold it and set_weight(return_weight=True) returns it; by default the layer's own."""
                 if not self.is_quantized:
                     return self.weight if weight is None else weight
-                shape = (self.out_features, self.in_features)
                 if weight is None:
                     weight = self.weight
-                if not isinstance(weight, MXFP4Tensor):
-                    if not isinstance(weight, torch.Tensor) or weight.dtype != torch.uint8 or weight.ndim != 1:
-                        raise TypeError(f"expected a packed MXFP4 weight, got {getattr(weight, 'dtype', type(weight).__name__)}")
-                    weight = MXFP4Tensor(weight, shape)
-                if weight.shape != shape:
-                    raise ValueError(f"expected a {shape} weight, got {weight.shape}")
-                return dequantize_mxfp4(weight, self.out_dtype)
+                if isinstance(weight, MXFP4Tensor):
+                    if weight.shape != (self.out_features, self.in_features):
+                        raise ValueError(f"expected a ({self.out_features}, {self.in_features}) weight, got {weight.shape}")
+                    weight = weight.data
+                if not isinstance(weight, torch.Tensor) or weight.dtype != torch.uint8 or weight.ndim != 1:
+                    raise TypeError(f"expected a packed MXFP4 weight, got {getattr(weight, 'dtype', type(weight).__name__)}")
+                return dequantize_mxfp4(self._operand(weight), self.out_dtype).to(weight.device)
 
             def set_weight(self, weight, inplace_update=False, seed=None, return_weight=False, **kwargs):
                 if not self.is_quantized:
@@ -131,7 +138,7 @@ def mxfp4_ops(out_dtype=torch.bfloat16, excluded_names=()):
                 if return_weight:
                     return quantized
                 assert inplace_update is False
-                self._hold(quantized)
+                self._hold(quantized._replace(data=quantized.data.to(self.weight.device)))
                 return None
 
             def forward(self, x: torch.Tensor | MXFP4Tensor) -> torch.Tensor:

@@ -42,3 +42,23 @@ def test_scaled_checkpoint(ops, mx, cuda, dtype, where):
         linear = load(ops, {"weight": weight.to(where), "weight_scale": scale.to(where)}, 70, 200)
         want = mx.quantize_mxfp4((weight.float() * scale).to(cuda))
         assert torch.equal(linear(x), mx.mxfp4_mm(x, want))
+
+
+def test_layer_in_host_memory(ops, mx, cuda):
+    """Saved, converted and given a merged weight where it lies, with the values of the layer on the GPU."""
+    weight = some(70, 200)
+    here, off = load(ops, {"weight": weight}, 70, 200), load(ops, {"weight": weight}, 70, 200).to("cpu")
+    assert off.weight.device.type == "cpu" and here.weight.is_cuda
+    want = here.state_dict()
+    for name, t in off.state_dict().items():
+        assert t.device.type == "cpu" and want[name].is_cuda and torch.equal(t, want[name].cpu())
+    again = load(ops, off.state_dict(), 70, 200).state_dict()  # (a packed operand's bytes beyond its rows are not specified)
+    assert all(torch.equal(again[name], want[name]) for name in want)
+    values = off.convert_weight(off.weight)
+    assert values.device.type == "cpu" and torch.equal(values, here.convert_weight().cpu())
+    merged = values + some(70, 200, seed=3, std=0.02)
+    assert torch.equal(off.convert_weight(off.set_weight(merged, return_weight=True)).cpu(),
+                       mx.dequantize_mxfp4(mx.quantize_mxfp4(merged.to(cuda))).cpu())
+    off.set_weight(merged)
+    here.set_weight(merged.to(cuda))
+    assert off.weight.device.type == "cpu" and torch.equal(off.state_dict()["weight"], here.state_dict()["weight"].cpu())

@@ -110,3 +110,28 @@ def test_convert_weight_converts_its_argument(layer_module, codec):
             linear.convert_weight(other)
     with pytest.raises(ValueError, match="expected a"):
         linear.convert_weight(new._replace(shape=(64, 4)))
+
+
+def test_conversions_of_a_layer_in_host_memory(layer_module, codec, monkeypatch):
+    """The kernels get the operand on the GPU (here: another device than the layer's), results come back from it."""
+    there = []
+
+    def on_gpu(t):
+        there.append(t)
+        return t
+
+    def unprepack(q):
+        return torch.zeros(4, 32, dtype=torch.uint8), torch.zeros(4, 2, dtype=torch.uint8)
+
+    monkeypatch.setattr(layer_module, "_on_gpu", on_gpu)
+    monkeypatch.setattr(layer_module, "unprepack_mxfp4", unprepack)
+    linear = load(layer_module, {"weight": torch.zeros(4, 64)}, 4, 64)
+    for convert in (linear.state_dict, lambda: linear.convert_weight(linear.weight)):
+        there.clear()
+        convert()
+        assert any(t is linear.weight for t in there)
+
+
+def test_layer_without_storage(layer_module, seen):
+    state = load(layer_module, {"weight": torch.zeros(4, 64)}, 4, 64).to("meta").state_dict()
+    assert {k: (t.shape, t.device.type) for k, t in state.items()} == {"weight": ((4, 32), "meta"), "weight_scale": ((4, 2), "meta")}
