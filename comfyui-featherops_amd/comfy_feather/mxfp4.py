@@ -86,7 +86,10 @@ def mxfp4_ops(out_dtype=torch.bfloat16, excluded_names=()):
                     elif weight.element_size() == 1 and weight.is_floating_point():  # (8-bit floats: bf16 holds all of their values)
                         weight = weight.to(torch.bfloat16)
                     self._hold(quantize_mxfp4(weight))
-                self.bias = None if bias is None else nn.Parameter(bias.to(self.out_dtype), requires_grad=False)
+                if bias is not None:  # (beside a packed weight, which is on the GPU)
+                    bias = nn.Parameter(bias.to(device=self.weight.device if self.is_quantized else None, dtype=self.out_dtype),
+                                        requires_grad=False)
+                self.bias = bias
 
             def _hold(self, weight: MXFP4Tensor) -> None:
                 if weight.shape != (self.out_features, self.in_features):
@@ -148,17 +151,34 @@ def mxfp4_ops(out_dtype=torch.bfloat16, excluded_names=()):
                     y = F.linear(x, weight, bias)
                     uncast_bias_weight(self, weight, bias, offload_stream)
                     return y
-                bias = self.bias
                 if isinstance(x, MXFP4Tensor):
                     if self.weight_function:
                         raise NotImplementedError("LoRA patches need activations in 16 bits")
-                    return mxfp4_mm(x, self.mx_weight, bias, self.out_dtype)
+                    return self._product(x, x.data)
                 dtype = x.dtype
                 if dtype == torch.float32:
                     x = x.to(torch.bfloat16)
-                y = mxfp4_mm(x, self.mx_weight, bias, self.out_dtype)
+                y = self._product(x, x)
                 if self.weight_function:
                     y = apply_lora_patches(x, y, self.weight_function)
                 return y if y.dtype == dtype else y.to(dtype)
+
+            def _product(self, x: torch.Tensor | MXFP4Tensor, data: torch.Tensor) -> torch.Tensor:
+                weight, bias = self.weight, self.bias
+                shape = (self.out_features, self.in_features)
+                device = data.device
+                if weight.device == device and (bias is None or bias.device == device and bias.dtype == self.out_dtype):
+                    return mxfp4_mm(x, MXFP4Tensor(weight, shape), bias, self.out_dtype)
+                # an offloaded layer: no patch is applied to the packed weight on its way
+                saved_weight_function = self.weight_function
+                self.weight_function = []
+                try:
+                    weight, bias, offload_stream = cast_bias_weight(self, data, dtype=torch.uint8,
+                                                                    bias_dtype=self.out_dtype, offloadable=True)
+                finally:
+                    self.weight_function = saved_weight_function
+                y = mxfp4_mm(x, MXFP4Tensor(weight, shape), bias, self.out_dtype)
+                uncast_bias_weight(self, weight, bias, offload_stream)
+                return y
 
     return MXFP4Ops

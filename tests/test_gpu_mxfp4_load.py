@@ -62,3 +62,18 @@ def test_layer_in_host_memory(ops, mx, cuda):
     off.set_weight(merged)
     here.set_weight(merged.to(cuda))
     assert off.weight.device.type == "cpu" and torch.equal(off.state_dict()["weight"], here.state_dict()["weight"].cpu())
+
+
+@pytest.mark.parametrize("out", [torch.bfloat16, torch.float16])
+def test_cpu_checkpoint_and_offloaded_layer(ops, mx, cuda, out):
+    """A layer from a checkpoint in host memory runs as it is, and so does one that was moved back there."""
+    weight, bias = some(70, 200), some(70, seed=4)
+    x = some(5, 200, seed=1).to(cuda)
+    q = mx.quantize_mxfp4(x)
+    want = mx.mxfp4_mm(x, mx.quantize_mxfp4(weight.to(cuda)), bias.to(cuda, out), out)
+    linear = load(ops, {"weight": weight, "bias": bias}, 70, 200, out)
+    assert linear.weight.is_cuda and linear.bias.is_cuda
+    for move in (lambda m: m, lambda m: m.to("cpu"), lambda m: m.to(cuda), lambda m: m.to(torch.float16), lambda m: m.to(torch.bfloat16)):
+        move(linear)
+        assert torch.equal(linear(x), want.to(x.dtype)) and torch.equal(linear(q), want)
+        assert linear.weight.device == linear.bias.device

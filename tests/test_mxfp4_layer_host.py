@@ -135,3 +135,37 @@ def test_conversions_of_a_layer_in_host_memory(layer_module, codec, monkeypatch)
 def test_layer_without_storage(layer_module, seen):
     state = load(layer_module, {"weight": torch.zeros(4, 64)}, 4, 64).to("meta").state_dict()
     assert {k: (t.shape, t.device.type) for k, t in state.items()} == {"weight": ((4, 32), "meta"), "weight_scale": ((4, 2), "meta")}
+
+
+@pytest.fixture
+def product(layer_module, monkeypatch):
+    """Stands for mxfp4_mm: the operands it was given, a result of zeros."""
+    calls = []
+
+    def mm(a, w, bias=None, out_dtype=None):
+        calls.append((a, w, bias))
+        return torch.zeros(*a.shape[:-1], w.shape[0], dtype=out_dtype, device=w.data.device)
+
+    monkeypatch.setattr(layer_module, "mxfp4_mm", mm)
+    return calls
+
+
+def test_offloaded_layer_comes_to_the_activations(layer_module, seen, product):
+    """Weight and bias elsewhere than the activations (here: those on the meta device) are brought to them for the call;
+    a bias of another type, as .to(float16) leaves it, is cast."""
+    linear = load(layer_module, {"weight": torch.zeros(4, 64), "bias": torch.ones(4)}, 4, 64)
+    for x in (torch.zeros(3, 64, dtype=torch.bfloat16, device="meta"),
+              layer_module.MXFP4Tensor(torch.zeros(4352, dtype=torch.uint8, device="meta"), (3, 64))):
+        linear(x)
+        _, weight, bias = product.pop()
+        assert weight.data.device.type == bias.device.type == "meta" and weight.shape == (4, 64)
+        assert linear.weight.device.type == linear.bias.device.type == "cpu"
+    linear.to(torch.float16)
+    linear(torch.zeros(3, 64, dtype=torch.float16))
+    assert product[-1][2].dtype == torch.bfloat16 and product[-1][1].data is linear.weight
+    linear.to(torch.bfloat16)
+    linear(torch.zeros(3, 64, dtype=torch.bfloat16))
+    assert product[-1][1].data is linear.weight and product[-1][2] is linear.bias
+    plain = load(layer_module, {"weight": torch.zeros(4, 64)}, 4, 64)
+    plain(torch.zeros(3, 64, dtype=torch.bfloat16, device="meta"))
+    assert product[-1][1].data.device.type == "meta" and product[-1][2] is None
