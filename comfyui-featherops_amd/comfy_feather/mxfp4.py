@@ -167,9 +167,10 @@ def mxfp4_ops(out_dtype=torch.bfloat16, excluded_names=()):
                 weight, bias = self.weight, self.bias
                 shape = (self.out_features, self.in_features)
                 device = data.device
-                if weight.device == device and (bias is None or bias.device == device and bias.dtype == self.out_dtype):
+                if weight.device == device and (bias is None or (bias.device == device and bias.dtype == self.out_dtype
+                                                                 and not self.bias_function)):
                     return mxfp4_mm(x, MXFP4Tensor(weight, shape), bias, self.out_dtype)
-                # an offloaded layer: no patch is applied to the packed weight on its way
+                # an offloaded layer, or a patched bias: no patch is applied to the packed weight on its way
                 saved_weight_function = self.weight_function
                 self.weight_function = []
                 try:

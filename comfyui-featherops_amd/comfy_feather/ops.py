@@ -61,6 +61,9 @@ else:
             bias_dtype = bias_dtype or bias.dtype
             if bias.device != input.device or bias.dtype != bias_dtype:
                 bias = bias.to(device=input.device, dtype=bias_dtype)
+        if bias is not None:
+            for f in getattr(s, "bias_function", ()):
+                bias = f(bias)
         return weight, bias, None
 
     def uncast_bias_weight(s, weight, bias, offload_stream) -> None:

@@ -169,3 +169,14 @@ def test_offloaded_layer_comes_to_the_activations(layer_module, seen, product):
     plain = load(layer_module, {"weight": torch.zeros(4, 64)}, 4, 64)
     plain(torch.zeros(3, 64, dtype=torch.bfloat16, device="meta"))
     assert product[-1][1].data.device.type == "meta" and product[-1][2] is None
+
+
+def test_bias_patches(layer_module, seen, product):
+    """bias_function runs on the bias in the output's type, in order, and leaves the stored one as it is."""
+    linear = load(layer_module, {"weight": torch.zeros(4, 64), "bias": torch.ones(4)}, 4, 64)
+    linear.bias_function = [lambda b: b + 1, lambda b: b * 3]
+    linear(torch.zeros(3, 64, dtype=torch.bfloat16))
+    assert torch.equal(product[-1][2], torch.full((4,), 6, dtype=torch.bfloat16)) and (linear.bias == 1).all()
+    linear.bias_function = []
+    linear(torch.zeros(3, 64, dtype=torch.bfloat16))
+    assert product[-1][2] is linear.bias
