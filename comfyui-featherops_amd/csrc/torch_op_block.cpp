@@ -70,7 +70,10 @@ struct Packed {
     uint8_t* scales() const { return codes() + codes_bytes; }
 };
 
-int64_t packed_units(int64_t rows, int64_t cols) { return (rows + 63) / 64 * ((cols + 127) / 128); }
+template <class Int>
+Int packed_units(const Int& rows, const Int& cols) {
+    return (rows + 63) / 64 * ((cols + 127) / 128);
+}
 
 Packed empty_packed(int64_t rows, int64_t cols, const at::Tensor& like) {
     const int64_t units = packed_units(rows, cols);
@@ -86,14 +89,16 @@ Packed check_packed(const at::Tensor& data, int64_t rows, int64_t cols, const ch
     return {data, units * 4096};
 }
 
-int64_t rows_of(at::IntArrayRef shape) {
-    int64_t n = 1;
-    for (size_t i = 0; i + 1 < shape.size(); ++i) n *= shape[i];
+template <class Int>
+Int rows_of(c10::ArrayRef<Int> shape) {
+    Int n = 1;
+    for (size_t i = 0; i + 1 < shape.size(); ++i) n = n * shape[i];
     return n;
 }
 // shape with its last dimension replaced
-at::DimVector with_last(at::IntArrayRef shape, int64_t n) {
-    at::DimVector v(shape.begin(), shape.end());
+template <class Int>
+c10::SmallVector<Int, at::kDimVectorStaticSize> with_last(c10::ArrayRef<Int> shape, const Int& n) {
+    c10::SmallVector<Int, at::kDimVectorStaticSize> v(shape.begin(), shape.end());
     v.back() = n;
     return v;
 }
@@ -364,55 +369,66 @@ std::tuple<at::Tensor, at::Tensor> gated_residual_norm_mxfp4(const at::Tensor& x
 
 // ---- fake tensors ----
 
-at::Tensor quantize_mxfp4_meta(const at::Tensor& x) { return empty_packed(x.numel() / x.size(-1), x.size(-1), x).data; }
-at::Tensor dequantize_mxfp4_meta(const at::Tensor& data, at::IntArrayRef shape, at::ScalarType dtype) {
-    return at::empty(shape, data.options().dtype(dtype));
+at::Tensor values_meta(c10::SymIntArrayRef shape, const at::Tensor& like, at::ScalarType dtype) {
+    return at::empty_symint(shape, like.options().dtype(dtype));
 }
-at::Tensor prepack_mxfp4_meta(const at::Tensor& codes, const at::Tensor&, int64_t cols) {
-    return empty_packed(codes.size(0), cols, codes).data;
+at::Tensor packed_meta(const c10::SymInt& rows, const c10::SymInt& cols, const at::Tensor& like) {
+    return values_meta({packed_units(rows, cols) * 4352}, like, at::kByte);
 }
-std::tuple<at::Tensor, at::Tensor> unprepack_mxfp4_meta(const at::Tensor& data, int64_t rows, int64_t cols) {
-    const int64_t blocks = (cols + 31) / 32;
-    return {at::empty({rows, blocks * 16}, data.options()), at::empty({rows, blocks}, data.options())};
+
+at::Tensor quantize_mxfp4_meta(const at::Tensor& x) {
+    return packed_meta(rows_of(x.sym_sizes()), x.sym_size(-1), x);
 }
-at::Tensor mxfp4_mm_meta(const at::Tensor& a, const at::Tensor&, int64_t N, int64_t, const OptTensor&,
+at::Tensor dequantize_mxfp4_meta(const at::Tensor& data, c10::SymIntArrayRef shape, at::ScalarType dtype) {
+    return values_meta(shape, data, dtype);
+}
+at::Tensor prepack_mxfp4_meta(const at::Tensor& codes, const at::Tensor& scales, c10::SymInt cols) {
+    return packed_meta(codes.sym_size(0), cols, codes);
+}
+std::tuple<at::Tensor, at::Tensor> unprepack_mxfp4_meta(const at::Tensor& data, c10::SymInt rows, c10::SymInt cols) {
+    const c10::SymInt blocks = (cols + 31) / 32;
+    return {values_meta({rows, blocks * 16}, data, at::kByte), values_meta({rows, blocks}, data, at::kByte)};
+}
+at::Tensor mxfp4_mm_meta(const at::Tensor& a, const at::Tensor& b, c10::SymInt N, c10::SymInt K, const OptTensor& bias,
                          std::optional<at::ScalarType> dtype) {
-    return at::empty(with_last(a.sizes(), N), a.options().dtype(dtype.value_or(a.scalar_type())));
+    return values_meta(with_last(a.sym_sizes(), N), a, dtype.value_or(a.scalar_type()));
 }
-at::Tensor mxfp4_mm_packed_meta(const at::Tensor& a, at::IntArrayRef a_shape, const at::Tensor&, int64_t N, int64_t,
-                                const OptTensor&, at::ScalarType out_dtype) {
-    return at::empty(with_last(a_shape, N), a.options().dtype(out_dtype));
+at::Tensor mxfp4_mm_packed_meta(const at::Tensor& a, c10::SymIntArrayRef a_shape, const at::Tensor& b, c10::SymInt N,
+                                c10::SymInt K, const OptTensor& bias, at::ScalarType out_dtype) {
+    return values_meta(with_last(a_shape, N), a, out_dtype);
 }
-at::Tensor modulated_norm_meta(const at::Tensor& x, const OptTensor&, const OptTensor&, const OptTensor&, const OptTensor&,
-                               bool, double, std::optional<at::ScalarType> out_dtype) {
-    return at::empty(x.sizes(), x.options().dtype(out_dtype.value_or(x.scalar_type())));
+at::Tensor modulated_norm_meta(const at::Tensor& x, const OptTensor& weight, const OptTensor& bias, const OptTensor& scale,
+                               const OptTensor& shift, bool, double, std::optional<at::ScalarType> out_dtype) {
+    return values_meta(x.sym_sizes(), x, out_dtype.value_or(x.scalar_type()));
 }
-at::Tensor modulated_norm_mxfp4_meta(const at::Tensor& x, const OptTensor&, const OptTensor&, const OptTensor&,
-                                     const OptTensor&, bool, double) {
+at::Tensor modulated_norm_mxfp4_meta(const at::Tensor& x, const OptTensor& weight, const OptTensor& bias,
+                                     const OptTensor& scale, const OptTensor& shift, bool, double) {
     return quantize_mxfp4_meta(x);
 }
-std::tuple<at::Tensor, at::Tensor> gated_residual_norm_meta(const at::Tensor& x, const at::Tensor& h, const OptTensor&,
-                                                            const OptTensor&, const OptTensor&, const OptTensor&,
-                                                            const OptTensor&, const OptTensor&, bool, double, double,
-                                                            std::optional<at::ScalarType>) {
-    return {at::empty(x.sizes(), x.options()), at::empty(x.sizes(), h.options())};
+std::tuple<at::Tensor, at::Tensor> gated_residual_norm_meta(const at::Tensor& x, const at::Tensor& h, const OptTensor& gate,
+                                                            const OptTensor& post_weight, const OptTensor& weight,
+                                                            const OptTensor& bias, const OptTensor& scale,
+                                                            const OptTensor& shift, bool, double, double,
+                                                            std::optional<at::ScalarType> out_dtype) {
+    return {values_meta(x.sym_sizes(), x, x.scalar_type()), values_meta(x.sym_sizes(), x, h.scalar_type())};
 }
-std::tuple<at::Tensor, at::Tensor> gated_residual_norm_mxfp4_meta(const at::Tensor& x, const at::Tensor&,
-                                                                  const OptTensor&, const OptTensor&, const OptTensor&,
-                                                                  const OptTensor&, const OptTensor&, const OptTensor&,
-                                                                  bool, double, double) {
-    return {at::empty(x.sizes(), x.options()), quantize_mxfp4_meta(x)};
+std::tuple<at::Tensor, at::Tensor> gated_residual_norm_mxfp4_meta(const at::Tensor& x, const at::Tensor& h,
+                                                                  const OptTensor& gate, const OptTensor& post_weight,
+                                                                  const OptTensor& weight, const OptTensor& bias,
+                                                                  const OptTensor& scale, const OptTensor& shift, bool,
+                                                                  double, double) {
+    return {values_meta(x.sym_sizes(), x, x.scalar_type()), quantize_mxfp4_meta(x)};
 }
 
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(feather_ops, m) {
     m.def("quantize_mxfp4(Tensor x) -> Tensor");
-    m.def("dequantize_mxfp4(Tensor data, int[] shape, ScalarType dtype) -> Tensor");
-    m.def("prepack_mxfp4(Tensor codes, Tensor scales, int cols) -> Tensor");
-    m.def("unprepack_mxfp4(Tensor data, int rows, int cols) -> (Tensor, Tensor)");
-    m.def("mxfp4_mm(Tensor a, Tensor b, int N, int K, Tensor? bias, ScalarType? out_dtype) -> Tensor");
-    m.def("mxfp4_mm_packed(Tensor a, int[] a_shape, Tensor b, int N, int K, Tensor? bias, ScalarType out_dtype) -> Tensor");
+    m.def("dequantize_mxfp4(Tensor data, SymInt[] shape, ScalarType dtype) -> Tensor");
+    m.def("prepack_mxfp4(Tensor codes, Tensor scales, SymInt cols) -> Tensor");
+    m.def("unprepack_mxfp4(Tensor data, SymInt rows, SymInt cols) -> (Tensor, Tensor)");
+    m.def("mxfp4_mm(Tensor a, Tensor b, SymInt N, SymInt K, Tensor? bias, ScalarType? out_dtype) -> Tensor");
+    m.def("mxfp4_mm_packed(Tensor a, SymInt[] a_shape, Tensor b, SymInt N, SymInt K, Tensor? bias, ScalarType out_dtype) -> Tensor");
     m.def("modulated_norm(Tensor x, Tensor? weight, Tensor? bias, Tensor? scale, Tensor? shift, bool layer, float eps, "
           "ScalarType? out_dtype) -> Tensor");
     m.def("modulated_norm_mxfp4(Tensor x, Tensor? weight, Tensor? bias, Tensor? scale, Tensor? shift, bool layer, "
