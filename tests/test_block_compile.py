@@ -1,4 +1,5 @@
-"""The MXFP4 operators and the block norms on fake tensors: compiled once for any number of tokens. No kernel runs."""
+"""The MXFP4 operators and the block norms on fake tensors: compiled once for any number of tokens, and refusing what the
+kernels refuse. No kernel runs."""
 
 import importlib
 
@@ -74,3 +75,41 @@ def test_names_are_all():
             return lambda *a, **k: None
 
     assert list(calls(Any(), Any())) == NAMES
+
+
+def test_fake_tensors_are_checked(mx, nm):
+    """What the kernels refuse does not trace."""
+    x, v = meta(4, 64), meta(64)
+    w = mx.quantize_mxfp4(meta(8, 64))
+    q = mx.quantize_mxfp4(x)
+    for call, message in [
+        (lambda: mx.quantize_mxfp4(meta(4, 0)), "at least one column"),
+        (lambda: mx.quantize_mxfp4(meta()), "at least one column"),
+        (lambda: mx.quantize_mxfp4(meta(4, 64, dtype=torch.float64)), "float16, bfloat16 or float32"),
+        (lambda: mx.dequantize_mxfp4(q, torch.float64), "float16, bfloat16 or float32"),
+        (lambda: mx.dequantize_mxfp4(q._replace(shape=(4, 0))), "at least one column"),
+        (lambda: mx.dequantize_mxfp4(q._replace(shape=(65, 64))), "packed for"),
+        (lambda: mx.unprepack_mxfp4(q._replace(shape=(65, 64))), "packed for"),
+        (lambda: mx.prepack_mxfp4(meta(4, 32, dtype=torch.uint8), meta(5, 2, dtype=torch.uint8)), "rows"),
+        (lambda: mx.prepack_mxfp4(meta(4, 32), meta(4, 2)), "1-byte"),
+        (lambda: mx.mxfp4_mm(meta(4, 64, dtype=F32), w), "float16 or bfloat16"),
+        (lambda: mx.mxfp4_mm(meta(4, 32), w), "b's 64 columns"),
+        (lambda: mx.mxfp4_mm(x, w, v), "elements"),
+        (lambda: mx.mxfp4_mm(x, w, None, F32), "out_dtype"),
+        (lambda: mx.mxfp4_mm(x, w._replace(shape=(70, 64))), "packed for"),
+        (lambda: mx.mxfp4_mm(q._replace(shape=(4, 32)), w), "columns"),
+        (lambda: mx.mxfp4_mm(q._replace(shape=(65, 64)), w), "packed for"),
+        (lambda: nm.modulated_norm(meta(4, 0)), "columns"),
+        (lambda: nm.modulated_norm(meta(4, 0), out_dtype="mxfp4"), "columns"),
+        (lambda: nm.modulated_norm(meta(4, 16385)), "16384 columns"),
+        (lambda: nm.modulated_norm(meta(4, 64, dtype=torch.float64)), "float16, bfloat16 or float32"),
+        (lambda: nm.modulated_norm(x, out_dtype=F16), "block's dtype"),
+        (lambda: nm.modulated_norm(x, weight=v[:63]), "64 columns"),
+        (lambda: nm.modulated_norm(x, scale=meta(3, 64)), "broadcast"),
+        (lambda: nm.gated_residual_norm(x, meta(3, 64)), "shape"),
+        (lambda: nm.gated_residual_norm(x, x.to(F16)), "block's dtype"),
+        (lambda: nm.gated_residual_norm(x, x, out_dtype=F32), "h's dtype"),
+        (lambda: nm.gated_residual_norm(x, meta(5, 64), out_dtype="mxfp4"), "shape"),
+    ]:
+        with pytest.raises(RuntimeError, match=message):
+            call()
