@@ -106,7 +106,7 @@ int feather_block_norm(const feather_block_norm_args* p, hipStream_t stream) {
                      p->scale_row_stride, p->shift, p->shift_row_stride, p->post_weight, p->weight, p->bias, p->x_out,
                      p->y, p->codes, p->scales, group(p->gate_group), group(p->mod_group), p->rows,
                      static_cast<int>(p->cols), p->x_dtype, p->y_dtype, p->mod_dtype == FEATHER_DTYPE_F32, p->norm,
-                     p->eps, p->residual_scale};
+                     p->eps, p->residual_scale, 0};
     return block_norm(a, stream);
 }
 

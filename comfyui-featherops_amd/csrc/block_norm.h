@@ -35,6 +35,7 @@ struct NormArgs {
     int x_type, y_type, mod_f32;  // MxType codes
     int layer;                    // 0: root mean square, 1: mean and variance
     float eps, residual_scale;
+    int64_t row0;  // first row of this launch, a multiple of 128: set by block_norm
 };
 
 int block_norm(const NormArgs& p, hipStream_t stream);

@@ -149,6 +149,7 @@ __global__ __launch_bounds__(kOneWave ? 256 : 1024, V == 1 ? 8 : 4) void norm_ke
     } else {
         row = kOneWave ? static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6) : blockIdx.x;
     }
+    row += p.row0;
     if (row >= p.rows) return;  // (whole rows: no thread of a row that takes part leaves)
 
     // vector i of this thread: the columns it stands for, where it lies, and how many of its values another
@@ -342,8 +343,12 @@ __global__ __launch_bounds__(kOneWave ? 256 : 1024, V == 1 ? 8 : 4) void norm_ke
     }
 }
 
+// Rows of one launch: a grid holds fewer than 2^32 threads, and a row takes up to 1024.
+constexpr int64_t kLaunchRows = int64_t(1) << 21;
+
+// Rows [p.row0, p.row0 + rows).
 template <int TX, int TY, bool kModF32, int V>
-int launch(const NormArgs& p, int threads, hipStream_t stream) {
+int launch_rows(const NormArgs& p, int64_t rows, int threads, hipStream_t stream) {
     const int ksteps = static_cast<int>(mx_ksteps(p.cols));
     typedef std::integral_constant<bool, true> Yes;
     typedef std::integral_constant<bool, false> No;
@@ -352,7 +357,7 @@ int launch(const NormArgs& p, int threads, hipStream_t stream) {
             <<<static_cast<unsigned>(blocks), block_threads, 0, stream>>>(p, ksteps);
     };
     if (threads == 64) {
-        const int64_t blocks = (p.rows + 3) / 4;
+        const int64_t blocks = (rows + 3) / 4;
         if constexpr (V == 1) {
             if (p.cols < 8) {
                 if (p.codes) go(Yes{}, Yes{}, Yes{}, blocks, 256);
@@ -363,11 +368,19 @@ int launch(const NormArgs& p, int threads, hipStream_t stream) {
         if (p.codes) go(Yes{}, Yes{}, No{}, blocks, 256);
         else go(Yes{}, No{}, No{}, blocks, 256);
     } else if (p.codes) {
-        go(No{}, Yes{}, No{}, (p.rows + 127) / 128 * 128, threads);  // whole rounds of 16 rows on each XCD
+        go(No{}, Yes{}, No{}, (rows + 127) / 128 * 128, threads);  // whole rounds of 16 rows on each XCD
     } else {
-        go(No{}, No{}, No{}, p.rows, threads);
+        go(No{}, No{}, No{}, rows, threads);
     }
     return hipGetLastError() == hipSuccess ? FEATHER_OK : FEATHER_ERR_LAUNCH;
+}
+
+template <int TX, int TY, bool kModF32, int V>
+int launch(NormArgs p, int threads, hipStream_t stream) {
+    int st = FEATHER_OK;
+    for (p.row0 = 0; p.row0 < p.rows && st == FEATHER_OK; p.row0 += kLaunchRows)
+        st = launch_rows<TX, TY, kModF32, V>(p, std::min(kLaunchRows, p.rows - p.row0), threads, stream);
+    return st;
 }
 
 template <int TX, int TY, bool kModF32>

@@ -374,7 +374,7 @@ int feather_mxfp4_mm(const void* a, const uint8_t* a_scales, int a_dtype, int64_
                      int output_dtype, void* workspace, size_t workspace_bytes, hipStream_t stream);
 
 /*
- * The norms around a block, one pass over (rows, cols), cols <= 16384:
+ * The norms around a block, one pass over (rows, cols), rows <= 2^30, cols <= 16384:
  *   h' = post_weight ? norm(h) * post_weight : h
  *   s  = residual_scale * x + gate * h'   (fp32; s = x where h is NULL), x_out = s
  *   y  = norm(s) * weight + bias;  y = y * (1 + scale) + shift
