@@ -10,7 +10,7 @@
 // HBM bound: x and h are read once and stay in registers (8 values a vector, V
 // vectors a thread) over the reductions; the variance is a second sum over the centred
 // registers, so a large mean costs no digits. A workgroup owns a row; rows of up to
-// 512 V values are one wave's, four to a workgroup, and meet no barrier. Measured, with gate, scale
+// 512 values are one wave's, four to a workgroup, and meet no barrier. Measured, with gate, scale
 // and shift: 8192 x 5120 with an fp32 stream 99 us (5.1 TB/s; a copy runs at 4.5 to 4.8), 4096 x 5120 in
 // bf16 33.5 us (5.0 TB/s), with MXFP4 out 27.6 us (5.1), one row of 5120 3.1 us.
 #include <algorithm>
@@ -356,21 +356,23 @@ int launch_rows(const NormArgs& p, int64_t rows, int threads, hipStream_t stream
         norm_kernel<TX, TY, kModF32, V, one_wave, codes, tiny>
             <<<static_cast<unsigned>(blocks), block_threads, 0, stream>>>(p, ksteps);
     };
-    if (threads == 64) {
-        const int64_t blocks = (rows + 3) / 4;
-        if constexpr (V == 1) {
+    bool one_wave = false;
+    if constexpr (V == 1) {  // (two vectors a thread: only rows of five waves or more, see pick)
+        one_wave = threads == 64;
+        if (one_wave) {
+            const int64_t blocks = (rows + 3) / 4;
             if (p.cols < 8) {
                 if (p.codes) go(Yes{}, Yes{}, Yes{}, blocks, 256);
                 else go(Yes{}, No{}, Yes{}, blocks, 256);
-                return hipGetLastError() == hipSuccess ? FEATHER_OK : FEATHER_ERR_LAUNCH;
+            } else {
+                if (p.codes) go(Yes{}, Yes{}, No{}, blocks, 256);
+                else go(Yes{}, No{}, No{}, blocks, 256);
             }
         }
-        if (p.codes) go(Yes{}, Yes{}, No{}, blocks, 256);
-        else go(Yes{}, No{}, No{}, blocks, 256);
-    } else if (p.codes) {
-        go(No{}, Yes{}, No{}, (rows + 127) / 128 * 128, threads);  // whole rounds of 16 rows on each XCD
-    } else {
-        go(No{}, No{}, No{}, rows, threads);
+    }
+    if (!one_wave) {
+        if (p.codes) go(No{}, Yes{}, No{}, (rows + 127) / 128 * 128, threads);  // whole rounds of 16 rows on each XCD
+        else go(No{}, No{}, No{}, rows, threads);
     }
     return hipGetLastError() == hipSuccess ? FEATHER_OK : FEATHER_ERR_LAUNCH;
 }
