@@ -73,6 +73,15 @@ size_t feather_mxfp4_mm_workspace_size(int64_t M, int64_t N, int64_t K, int a_dt
     return M <= kMxFewRows ? mx_rows_workspace(M, N, K) : mx_tiles_workspace(M, N, K);
 }
 
+int feather_mxfp4_mm_plan(int64_t M, int64_t N, int64_t K, int64_t* plan) {
+    if (!mm_sizes_ok(M, N, K) || !plan) return FEATHER_ERR_INVALID;
+    for (int i = 0; i < 8; ++i) plan[i] = 0;
+    if (M == 0) return FEATHER_OK;
+    if (M <= kMxFewRows) mx_rows_parts(M, N, K, plan);
+    else mx_tiles_parts(M, N, K, plan);
+    return FEATHER_OK;
+}
+
 int feather_mxfp4_mm(const void* a, const uint8_t* a_scales, int a_dtype, int64_t a_row_stride, const uint8_t* b,
                      const uint8_t* b_scales, const uint16_t* bias, uint16_t* c, int64_t M, int64_t N, int64_t K,
                      int output_dtype, void* workspace, size_t workspace_bytes, hipStream_t stream) {

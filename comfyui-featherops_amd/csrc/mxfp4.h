@@ -277,5 +277,8 @@ size_t mx_rows_workspace(int64_t M, int64_t N, int64_t K);
 size_t mx_tiles_workspace(int64_t M, int64_t N, int64_t K);
 int mx_mm_rows(const MxMmArgs& p, hipStream_t stream);
 int mx_mm_tiles(const MxMmArgs& p, hipStream_t stream);
+// What they launch with that workspace: feather_mxfp4_mm_plan.
+void mx_rows_parts(int64_t M, int64_t N, int64_t K, int64_t* plan);
+void mx_tiles_parts(int64_t M, int64_t N, int64_t K, int64_t* plan);
 
 }  // namespace feather

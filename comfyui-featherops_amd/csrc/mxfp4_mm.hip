@@ -442,6 +442,15 @@ size_t mx_tiles_workspace(int64_t M, int64_t N, int64_t K) {
     return split_bytes(M - plan.m1, N - plan.n1, plan.rest);
 }
 
+void mx_tiles_parts(int64_t M, int64_t N, int64_t K, int64_t* plan) {
+    const Plan p = make_plan(M, N, mx_ksteps(K));
+    auto part = [](int64_t* out, const Choice& c) { out[0] = kTiles[c.tile].bm, out[1] = kTiles[c.tile].bn, out[2] = c.ksplit; };
+    part(plan, p.first);
+    if (p.m1 || p.n1) part(plan + 3, p.rest);
+    plan[6] = p.m1;
+    plan[7] = p.n1;
+}
+
 int mx_mm_tiles(const MxMmArgs& p, hipStream_t stream) {
     const Plan plan = make_plan(p.M, p.N, mx_ksteps(p.K));
     if (!plan.m1 && !plan.n1) return run(p, plan.first, 0, 0, p.M, p.N, stream);

@@ -276,6 +276,13 @@ RowsPlan rows_plan(int64_t M, int64_t N, int64_t K) {
 
 size_t mx_rows_workspace(int64_t M, int64_t N, int64_t K) { return rows_plan(M, N, K).ws_bytes; }
 
+void mx_rows_parts(int64_t M, int64_t N, int64_t K, int64_t* plan) {
+    const RowsPlan p = rows_plan(M, N, K);
+    plan[0] = M <= 16 ? 16 : 32;
+    plan[1] = p.nt * 16;
+    plan[2] = p.ksplit;
+}
+
 int mx_mm_rows(const MxMmArgs& p, hipStream_t stream) {
     if (p.a_type != kMxPacked && !mx_rows_in_reach(p.M, p.a_stride)) return FEATHER_ERR_UNSUPPORTED;
     RowsPlan plan = rows_plan(p.M, p.N, p.K);

@@ -69,6 +69,7 @@ SIGNATURES: dict[str, tuple] = {
     "feather_mxfp4_prepack": (_int, [_vp, _vp, _vp, _vp, _i64, _i64, _vp]),
     "feather_mxfp4_unprepack": (_int, [_vp, _vp, _vp, _vp, _i64, _i64, _vp]),
     "feather_mxfp4_mm_takes_16bit": (_int, [_i64, _i64, _i64, _i64]),
+    "feather_mxfp4_mm_plan": (_int, [_i64, _i64, _i64, ctypes.POINTER(_i64)]),
     "feather_mxfp4_mm_workspace_size": (ctypes.c_size_t, [_i64, _i64, _i64, _int]),
     "feather_mxfp4_mm": (_int, [_vp, _vp, _int, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _int, _vp,
                                 ctypes.c_size_t, _vp]),

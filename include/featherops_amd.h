@@ -368,6 +368,10 @@ int feather_mxfp4_unprepack(const uint8_t* codes, const uint8_t* scales, uint8_t
  * sums run in another order.
  */
 int feather_mxfp4_mm_takes_16bit(int64_t M, int64_t N, int64_t K, int64_t a_row_stride);
+/* What feather_mxfp4_mm launches for a shape with the workspace below: plan[0..2] are the rows and columns of a
+ * workgroup's tile and the number of workgroups that share a tile's K; where the result is composed of two launches,
+ * plan[3..5] are the second one's, which starts at row plan[6] or column plan[7] (zeros otherwise). */
+int feather_mxfp4_mm_plan(int64_t M, int64_t N, int64_t K, int64_t* plan);
 size_t feather_mxfp4_mm_workspace_size(int64_t M, int64_t N, int64_t K, int a_dtype);
 int feather_mxfp4_mm(const void* a, const uint8_t* a_scales, int a_dtype, int64_t a_row_stride, const uint8_t* b,
                      const uint8_t* b_scales, const uint16_t* bias, uint16_t* c, int64_t M, int64_t N, int64_t K,
