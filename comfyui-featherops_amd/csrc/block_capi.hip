@@ -1,6 +1,8 @@
 // extern "C" entry points of the MXFP4 operators and the block norms (declared in
 // include/featherops_amd.h). Sizes, types and pointers are checked here, before
 // anything is launched.
+#include <initializer_list>
+
 #include "block_norm.h"
 #include "featherops_amd.h"
 #include "mxfp4.h"
@@ -18,6 +20,12 @@ bool mx_sizes_ok(int64_t rows, int64_t cols) {
     return rows >= 0 && cols > 0 && rows <= kMaxRows && cols < kMaxCols && mx_groups(rows) * mx_ksteps(cols) < (int64_t(1) << 23);
 }
 bool value_type(int t) { return t == FEATHER_DTYPE_F16 || t == FEATHER_DTYPE_BF16 || t == FEATHER_DTYPE_F32; }
+// Packed buffers are read in 16-byte units, by copies into LDS among others.
+bool aligned(std::initializer_list<const void*> packed) {
+    uintptr_t bits = 0;
+    for (const void* p : packed) bits |= reinterpret_cast<uintptr_t>(p);
+    return bits % 16 == 0;
+}
 bool mm_sizes_ok(int64_t M, int64_t N, int64_t K) { return mx_sizes_ok(M, K) && N > 0 && mx_sizes_ok(N, K); }
 
 }  // namespace
@@ -36,7 +44,7 @@ int feather_mxfp4_quantize(const void* x, int x_dtype, int64_t rows, int64_t col
                            uint8_t* scales, hipStream_t stream) {
     if (!mx_sizes_ok(rows, cols) || !value_type(x_dtype) || (rows > 1 && row_stride < 0)) return FEATHER_ERR_INVALID;
     if (rows == 0) return FEATHER_OK;
-    if (!x || !codes || !scales) return FEATHER_ERR_INVALID;
+    if (!x || !codes || !scales || !aligned({codes, scales})) return FEATHER_ERR_INVALID;
     return mx_quantize(x, x_dtype, rows, cols, row_stride, codes, scales, stream);
 }
 
@@ -44,7 +52,7 @@ int feather_mxfp4_dequantize(const uint8_t* codes, const uint8_t* scales, void* 
                              int64_t cols, hipStream_t stream) {
     if (!mx_sizes_ok(rows, cols) || !value_type(out_dtype)) return FEATHER_ERR_INVALID;
     if (rows == 0) return FEATHER_OK;
-    if (!codes || !scales || !out) return FEATHER_ERR_INVALID;
+    if (!codes || !scales || !out || !aligned({codes, scales})) return FEATHER_ERR_INVALID;
     return mx_dequantize(codes, scales, out, out_dtype, rows, cols, stream);
 }
 
@@ -52,7 +60,7 @@ int feather_mxfp4_prepack(const uint8_t* codes_rows, const uint8_t* scales_rows,
                           int64_t rows, int64_t cols, hipStream_t stream) {
     if (!mx_sizes_ok(rows, cols)) return FEATHER_ERR_INVALID;
     if (rows == 0) return FEATHER_OK;
-    if (!codes_rows || !scales_rows || !codes || !scales) return FEATHER_ERR_INVALID;
+    if (!codes_rows || !scales_rows || !codes || !scales || !aligned({codes, scales})) return FEATHER_ERR_INVALID;
     return mx_prepack(codes_rows, scales_rows, codes, scales, rows, cols, stream);
 }
 
@@ -60,7 +68,7 @@ int feather_mxfp4_unprepack(const uint8_t* codes, const uint8_t* scales, uint8_t
                             int64_t rows, int64_t cols, hipStream_t stream) {
     if (!mx_sizes_ok(rows, cols)) return FEATHER_ERR_INVALID;
     if (rows == 0) return FEATHER_OK;
-    if (!codes_rows || !scales_rows || !codes || !scales) return FEATHER_ERR_INVALID;
+    if (!codes_rows || !scales_rows || !codes || !scales || !aligned({codes, scales})) return FEATHER_ERR_INVALID;
     return mx_unprepack(codes, scales, codes_rows, scales_rows, rows, cols, stream);
 }
 
@@ -92,6 +100,7 @@ int feather_mxfp4_mm(const void* a, const uint8_t* a_scales, int a_dtype, int64_
     if (M == 0) return FEATHER_OK;
     if (!a || (packed && !a_scales) || !b || !b_scales || !c || (!packed && M > 1 && a_row_stride < 0))
         return FEATHER_ERR_INVALID;
+    if (!aligned({b, b_scales}) || (packed && !aligned({a, a_scales}))) return FEATHER_ERR_INVALID;
     const MxMmArgs args{static_cast<const uint8_t*>(a), a_scales, a_dtype, a_row_stride, b, b_scales, bias, c, M,
                         static_cast<int>(N), static_cast<int>(K), output_dtype == FEATHER_DTYPE_BF16,
                         static_cast<uint8_t*>(workspace), workspace ? workspace_bytes : 0};
@@ -108,7 +117,7 @@ int feather_block_norm(const feather_block_norm_args* p, hipStream_t stream) {
     if (p->rows == 0) return FEATHER_OK;
     const bool to_codes = p->codes || p->scales;
     if (!p->x || (p->h && !p->x_out) || (!p->h && (p->gate || p->post_weight)) || (p->gate && p->gate_group <= 0) ||
-        ((p->scale || p->shift) && p->mod_group <= 0) || (to_codes ? !p->codes || !p->scales || p->y : !p->y))
+        ((p->scale || p->shift) && p->mod_group <= 0) || (to_codes ? !p->codes || !p->scales || p->y || !aligned({p->codes, p->scales}) : !p->y))
         return FEATHER_ERR_INVALID;
     auto group = [&](int64_t g) { return static_cast<uint32_t>(g < p->rows ? g : p->rows); };
     const NormArgs a{p->x, p->x_row_stride, p->h, p->h_row_stride, p->gate, p->gate_row_stride, p->scale,

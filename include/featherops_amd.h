@@ -331,7 +331,7 @@ int feather_dequantize_e5m2(const uint8_t* packed, const float* scale, void* out
  *          [r / 64][k / 128][r / 16 % 4][16 * (k % 128 / 32) + r % 16]
  *   scales [groups][steps][64][4]: that block's in byte r / 16 % 4 of
  *          [r / 64][k / 128][16 * (k % 128 / 32) + r % 16]
- * Buffers of the packed form are 16-byte aligned. rows <= 2^30, cols < 2^24, and
+ * Buffers of the packed form are 16-byte aligned (FEATHER_ERR_INVALID otherwise). rows <= 2^30, cols < 2^24, and
  * groups * steps < 2^23 (2^36 values).
  */
 size_t feather_mxfp4_codes_bytes(int64_t rows, int64_t cols);  /* of the packed form; 0 for sizes outside the domain */
