@@ -39,17 +39,8 @@ __device__ __forceinline__ Raw8<kF32> load8(const uint8_t* p) {
 // values [0, n) of p, zeros beyond
 template <bool kF32>
 __device__ __forceinline__ Raw8<kF32> load_part(const uint8_t* p, int n) {
-    uint32_t w[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        if constexpr (kF32) {
-            w[i] = i < n ? reinterpret_cast<const uint32_t*>(p)[i] : 0u;
-        } else if (i < 4) {
-            const uint16_t* q = reinterpret_cast<const uint16_t*>(p);
-            w[i] = (2 * i < n ? static_cast<uint32_t>(q[2 * i]) : 0u) |
-                   (2 * i + 1 < n ? static_cast<uint32_t>(q[2 * i + 1]) << 16 : 0u);
-        }
-    }
+    uint32_t w[kF32 ? 8 : 4];
+    load_few8<kF32>(p, n, w);
     Raw8<kF32> r;
     r.v[0] = make_uint4(w[0], w[1], w[2], w[3]);
     if constexpr (kF32) r.v[1] = make_uint4(w[4], w[5], w[6], w[7]);

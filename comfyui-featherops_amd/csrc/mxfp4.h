@@ -25,9 +25,22 @@
 // depends on another row).
 #pragma once
 
+#include <type_traits>
+#include <utility>
+
 #include "feather_common.h"
 
 namespace feather {
+
+template <int... I, class F>
+__device__ __forceinline__ void unrolled_impl(std::integer_sequence<int, I...>, F&& f) {
+    (f(std::integral_constant<int, I>{}), ...);
+}
+// f(0_c) .. f(n-1_c): indices as constants, which the MFMA's scale selectors need.
+template <int N, class F>
+__device__ __forceinline__ void unrolled(F&& f) {
+    unrolled_impl(std::make_integer_sequence<int, N>{}, f);
+}
 
 constexpr int kMxBlock = 32;
 constexpr int kMxStepK = 128;
@@ -72,6 +85,21 @@ template <bool kBf16>
 __device__ __forceinline__ uint32_t mx_round_pair(float a, float b) {
     if constexpr (kBf16) return f32x2_to_bf16x2_raw(a, b);
     else return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2_t{a, b}, f16x2_t));
+}
+
+// The first n of 8 values from p, zeros beyond: kF32 ? 8 : 4 words.
+template <bool kF32>
+__device__ __forceinline__ void load_few8(const uint8_t* p, int n, uint32_t (&w)[kF32 ? 8 : 4]) {
+#pragma unroll
+    for (int k = 0; k < (kF32 ? 8 : 4); ++k) {
+        if constexpr (kF32) {
+            w[k] = k < n ? reinterpret_cast<const uint32_t*>(p)[k] : 0u;
+        } else {
+            const uint16_t* q = reinterpret_cast<const uint16_t*>(p);
+            w[k] = (2 * k < n ? static_cast<uint32_t>(q[2 * k]) : 0u) |
+                   (2 * k + 1 < n ? static_cast<uint32_t>(q[2 * k + 1]) << 16 : 0u);
+        }
+    }
 }
 
 enum MxType { kMxF16 = 0, kMxBf16 = 1, kMxF32 = 2 };
@@ -153,16 +181,7 @@ struct MxPieces {
     // the same for a row of fewer than 8 values: the n from p on
     __device__ __forceinline__ void load_few(int i, const uint8_t* p, int n) {
         uint32_t w[kVecs * 4];
-#pragma unroll
-        for (int k = 0; k < kVecs * 4; ++k) {
-            if constexpr (T == kMxF32) {
-                w[k] = k < n ? reinterpret_cast<const uint32_t*>(p)[k] : 0u;
-            } else {
-                const uint16_t* q = reinterpret_cast<const uint16_t*>(p);
-                w[k] = (2 * k < n ? static_cast<uint32_t>(q[2 * k]) : 0u) |
-                       (2 * k + 1 < n ? static_cast<uint32_t>(q[2 * k + 1]) << 16 : 0u);
-            }
-        }
+        load_few8<T == kMxF32>(p, n, w);
 #pragma unroll
         for (int k = 0; k < kVecs; ++k) v[i][k] = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
     }

@@ -9,7 +9,6 @@
 //   round of workgroups: (154, 10240, 4096) 11.2 us with 22 MB of weights, (1024, 5120, 5120) 21.5 us.
 #include <algorithm>
 #include <type_traits>
-#include <utility>
 
 #include "featherops_amd.h"
 #include "lds_dma.h"
@@ -17,16 +16,6 @@
 
 namespace feather {
 namespace {
-
-template <int... I, class F>
-__device__ __forceinline__ void unrolled_impl(std::integer_sequence<int, I...>, F&& f) {
-    (f(std::integral_constant<int, I>{}), ...);
-}
-// f(0_c) .. f(n-1_c): indices as constants, which the MFMA's scale selectors need.
-template <int N, class F>
-__device__ __forceinline__ void unrolled(F&& f) {
-    unrolled_impl(std::make_integer_sequence<int, N>{}, f);
-}
 
 // dma16_lds, and the same for 4 bytes per lane, with an offset that the instruction adds to both addresses:
 // copies a KB apart in LDS share one M0.

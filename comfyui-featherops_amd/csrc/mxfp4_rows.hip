@@ -7,7 +7,6 @@
 // 3 are the launch, the first load's way and the join of the eight waves.
 #include <algorithm>
 #include <type_traits>
-#include <utility>
 
 #include "featherops_amd.h"
 #include "mxfp4.h"
@@ -16,15 +15,6 @@ namespace feather {
 namespace {
 
 constexpr int kWaves = 8;
-
-template <int... I, class F>
-__device__ __forceinline__ void unrolled_impl(std::integer_sequence<int, I...>, F&& f) {
-    (f(std::integral_constant<int, I>{}), ...);
-}
-template <int N, class F>
-__device__ __forceinline__ void unrolled(F&& f) {
-    unrolled_impl(std::make_integer_sequence<int, N>{}, f);
-}
 
 struct RowsArgs {
     const uint8_t* a;
