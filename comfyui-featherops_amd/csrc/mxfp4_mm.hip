@@ -3,8 +3,8 @@
 //
 // Bounds, measured (MI355X, packed operands, weights from HBM):
 //   one row of the largest tile on every CU and more: the matrix cores at the clock that the power allows. The
-//   instruction alone sustains 6.4 to 7.1 PFLOP/s; (16384, 5120, 13824) runs at 5.0, (32768, 13824, 5120) at 4.4,
-//   of which the stores of a tile, 128 KB a CU that no other tile's work covers, take 11%.
+//   instruction alone sustains 6.4 to 7.1 PFLOP/s; (16384, 5120, 13824) runs at 4.7 (5.1 at best), (32768, 13824, 5120)
+//   at 4.2 to 4.5, of which the stores of a tile, 128 KB a CU that no other tile's work covers, take 11%.
 //   up to some hundred rows: the operands' way from HBM through one workgroup's ring, 50 to 60 GB/s a CU, in one
 //   round of workgroups: (154, 10240, 4096) 11.2 us with 22 MB of weights, (1024, 5120, 5120) 21.5 us.
 #include <algorithm>
@@ -258,7 +258,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mx_tile_kernel(const TileArgs
 
     // Epilogue: bias added in fp32, one rounding to the output type. A lane has four columns of each
     // fragment; neighbouring quarters of the wave (lane ^ 16) trade one fragment of a pair for the other,
-    // so that every lane stores 8 columns and a row gets 64 contiguous bytes from one instruction.
+    // so that every lane stores 8 columns and a row gets 64 contiguous bytes from one instruction. (Rows of C off
+    // 16-byte boundaries, N no multiple of 8, make unaligned stores: 3844 x 7679 x 722 45 us, x 7676 28, x 7680 25.)
     const int kb = lane >> 4;
     unrolled<FN / 2>([&](auto h) {
         constexpr int j = 2 * h;

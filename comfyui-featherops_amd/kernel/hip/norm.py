@@ -18,7 +18,9 @@ by default x's). out_dtype="mxfp4" gives y as an MXFP4Tensor for mxfp4_mm instea
 x is fp32 or of the block's type. gate, scale and shift broadcast against x: (cols,), (batch, 1, cols) or
 x's own shape, slices of a larger modulation tensor included. Vectors of the block's type are read as
 they are; if any has another type (fp32 modulation beside bf16 weights), all are read as fp32 (those that
-are not are cast first). Up to 16384 columns. Runs in libfeatherops_amd.so on torch's current stream; there is no other compute path.
+are not are cast first, on every call). scale and shift of which one is per sample and the other for all rows are
+both written out row by row first: give both the same form. Up to 16384 columns. Runs in libfeatherops_amd.so on
+torch's current stream; there is no other compute path.
 """
 
 from __future__ import annotations
