@@ -180,3 +180,35 @@ def test_bias_patches(layer_module, seen, product):
     linear.bias_function = []
     linear(torch.zeros(3, 64, dtype=torch.bfloat16))
     assert product[-1][2] is linear.bias
+
+
+def test_assigned_weight(layer_module, seen, product):
+    linear = load(layer_module, {"weight": torch.zeros(4, 64, dtype=torch.bfloat16)}, 4, 64, excluded=("up",))
+    assert linear.mx_weight is None
+    operand = layer_module.MXFP4Tensor(torch.full((4352,), 5, dtype=torch.uint8), (4, 64))
+    linear.mx_weight = operand
+    assert linear.is_quantized and torch.equal(linear.weight, operand.data)
+    linear(torch.zeros(3, 64, dtype=torch.bfloat16))
+    assert product[-1][1].data is linear.weight
+    with pytest.raises(ValueError, match="expected a"):
+        linear.mx_weight = operand._replace(shape=(64, 4))
+
+
+def test_forward_under_compile(layer_module, seen):
+    """One graph for the first token count, one for every other, with 16-bit and with 4-bit activations."""
+    linear = load(layer_module, {"weight": torch.zeros(4, 64), "bias": torch.zeros(4)}, 4, 64).to("meta")
+    quantise = importlib.import_module("featherops_amd.kernel.hip.mxfp4").quantize_mxfp4
+    graphs = []
+
+    def backend(gm, _):
+        graphs.append(gm)
+        return gm.forward
+
+    for fn in (linear, lambda x: linear(quantise(x))):
+        torch._dynamo.reset()
+        graphs.clear()
+        compiled = torch.compile(fn, backend=backend, fullgraph=True)
+        for n in (3, 5, 200):
+            assert compiled(torch.empty(n, 64, dtype=torch.bfloat16, device="meta")).shape == (n, 4)
+        assert len(graphs) <= 2
+    torch._dynamo.reset()
