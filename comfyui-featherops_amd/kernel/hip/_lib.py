@@ -74,6 +74,9 @@ SIGNATURES: dict[str, tuple] = {
     "feather_mxfp4_mm": (_int, [_vp, _vp, _int, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _int, _vp,
                                 ctypes.c_size_t, _vp]),
     "feather_block_norm": (_int, [_vp, _vp]),
+    "feather_rope_table": (_int, [_vp, _int, _i64, ctypes.POINTER(_int), _int, ctypes.c_double, _int, _vp, _vp]),
+    "feather_qk_norm_rope": (_int, [_vp, _vp]),
+    "feather_attention": (_int, [_vp, _vp]),
     "feather_status_string": (ctypes.c_char_p, [_int]),
     "feather_abi_version": (_int, []),
 }

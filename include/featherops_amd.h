@@ -41,6 +41,7 @@ extern "C" {
 #define FEATHER_DTYPE_BF16 1
 #define FEATHER_DTYPE_F32 2
 #define FEATHER_DTYPE_MXFP4 3 /* packed MXFP4 codes and scales, see below */
+#define FEATHER_DTYPE_BOOL 4  /* a byte, zero or not: attention masks */
 #define FEATHER_B_E4M3FN 0
 #define FEATHER_B_E5M2 1
 
@@ -416,6 +417,92 @@ typedef struct feather_block_norm_args {
     float eps, residual_scale;
 } feather_block_norm_args;
 int feather_block_norm(const feather_block_norm_args* args, hipStream_t stream);
+
+/*
+ * Rotary positions of several axes. Row r of table (rows, pairs, 2), fp32, holds
+ * cos and sin of positions[r][axis of pair] * theta^(-2 j / d): axis i has
+ * axis_dims[i] / 2 pairs, one axis behind the other, at most 8 axes and 128 pairs;
+ * j counts an axis's pairs and d is its axis_dims, or with shared_ladder j counts all pairs and d is
+ * the sum of axis_dims. Angles are fp64. positions: (rows, axes), contiguous.
+ * No counterpart in the reference.
+ */
+#define FEATHER_POSITION_I32 0
+#define FEATHER_POSITION_I64 1
+#define FEATHER_POSITION_F32 2
+#define FEATHER_POSITION_F64 3
+int feather_rope_table(const void* positions, int position_dtype, int64_t rows, const int* axis_dims, int axes, double theta,
+                       int shared_ladder, float* table, hipStream_t stream);
+
+/*
+ * Queries and keys (batch, tokens, heads, head_dim): normed, weighted, turned by
+ * their positions, in fp32, rounded once.
+ *   norm 0: none. 1: v / sqrt(mean(v^2) + eps) over a head; weights (head_dim,).
+ *   2: over all heads of a token; weights (heads, head_dim); heads times head_dim rounded up
+ *   to a power of two is at most 16384.
+ *   table (tokens, pairs, 2) of feather_rope_table, one for each sample with a
+ *   table_batch_stride (floats), or NULL. Pair p of a head is values 2 p and 2 p + 1, or with
+ *   pairs_of_halves p and pairs + p; values from 2 pairs on are not turned.
+ * head_dim: a multiple of 8 up to 256. Strides count elements; q_out and k_out are
+ * contiguous; any alignment of the element types. k_heads 0: no keys. Weights may be
+ * NULL; weight_dtype is dtype or fp32. No counterpart in the reference.
+ */
+typedef struct feather_rope_args {
+    const void* q;
+    const void* k;
+    void* q_out;
+    void* k_out;
+    const void* q_weight;
+    const void* k_weight;
+    const float* table;
+    int64_t batch, tokens, q_heads, k_heads, head_dim, pairs;
+    int64_t q_batch_stride, q_token_stride, q_head_stride;
+    int64_t k_batch_stride, k_token_stride, k_head_stride;
+    int64_t table_batch_stride;
+    int dtype, weight_dtype;
+    int norm, pairs_of_halves;
+    float eps;
+} feather_rope_args;
+int feather_qk_norm_rope(const feather_rope_args* args, hipStream_t stream);
+
+/*
+ * Attention: out[i] = sum_j p[i][j] v[j], p = softmax over j of scale * q[i] . k[j] + mask[i][j],
+ * over the keys j that query i may see; a query that sees none gets zeros. fp32 scores, sums
+ * and maxima; the weights p are rounded to dtype, and out once.
+ *   q, out (batch, q_tokens, heads, head_dim), k, v (batch, k_tokens, kv_heads, head_dim);
+ *   heads / kv_heads consecutive heads share a key head. out is contiguous.
+ *   k_lengths (batch,) or NULL: a sample's keys are its first k_lengths ones (clamped to
+ *   0 .. k_tokens); what lies behind them is not read.
+ *   causal: query i of n sees keys up to i + (keys - n): the last query sees all.
+ *   mask (batch, heads, q_tokens, k_tokens) or NULL, strides in elements, 0 where one is
+ *   shared, keys contiguous: bytes (zero: not seen), or dtype or fp32 values, added.
+ *   q_offsets, k_offsets (batch + 1,), both or neither: packed sequences instead of
+ *   samples: q, out (q_tokens, heads, head_dim), k, v (k_tokens, kv_heads, head_dim), sequence
+ *   s has the tokens from offset s to offset s + 1. Rows of out in front of the first and behind the
+ *   last sequence are zeros. Offsets must not fall; they are clamped to the tensors, never
+ *   followed out of them. No mask, no k_lengths.
+ * dtype F16 or BF16; head_dim a multiple of 8 up to 256; q, k, v, out at 16-byte
+ * boundaries, strides multiples of 8, a token stride below 2^23; scale positive.
+ * No counterpart in the reference.
+ */
+typedef struct feather_attention_args {
+    const void* q;
+    const void* k;
+    const void* v;
+    void* out;
+    const void* mask;
+    const int32_t* q_offsets;
+    const int32_t* k_offsets;
+    const int32_t* k_lengths;
+    int64_t batch, q_tokens, k_tokens, heads, kv_heads, head_dim;
+    int64_t q_batch_stride, q_token_stride, q_head_stride;
+    int64_t k_batch_stride, k_token_stride, k_head_stride;
+    int64_t v_batch_stride, v_token_stride, v_head_stride;
+    int64_t mask_batch_stride, mask_head_stride, mask_query_stride;
+    int dtype, mask_dtype;
+    int causal;
+    float scale;
+} feather_attention_args;
+int feather_attention(const feather_attention_args* args, hipStream_t stream);
 
 /* Text for a status code. */
 const char* feather_status_string(int status);
