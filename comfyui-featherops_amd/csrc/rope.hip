@@ -55,9 +55,33 @@ __device__ __forceinline__ void store8(uint8_t* p, const float (&f)[8]) {
     } else {
         uint32_t w[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = f32x2_to_out_bits<T == kMxBf16>(f[2 * i], f[2 * i + 1]);
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (T == kMxBf16) w[i] = f32x2_to_bf16x2_raw(f[2 * i], f[2 * i + 1]);
+            else w[i] = f32x2_to_out_bits<false>(f[2 * i], f[2 * i + 1]);
+        }
         __builtin_memcpy(p, w, 16);
     }
+}
+
+// The sum over each `lanes` lanes (a power of two), in all of them.
+template <int kControl>
+__device__ __forceinline__ float add_lane(float x) {
+    return x + bits_f32(static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(f32_bits(x)), kControl, 0xf, 0xf, true)));
+}
+__device__ __forceinline__ float sum_lanes(float x, int lanes) {
+    if (lanes > 1) x = add_lane<0xB1>(x);   // the neighbour's
+    if (lanes > 2) x = add_lane<0x4E>(x);   // the other pair's of four
+    if (lanes > 4) x = add_lane<0x141>(x);  // mirrored in eight, whose fours are alike by now
+    if (lanes > 8) x = add_lane<0x140>(x);  // and in sixteen
+    if (lanes > 16) {
+        const auto r = __builtin_amdgcn_permlane16_swap(f32_bits(x), f32_bits(x), false, false);
+        x = bits_f32(r[0]) + bits_f32(r[1]);
+    }
+    if (lanes > 32) {
+        const auto r = __builtin_amdgcn_permlane32_swap(f32_bits(x), f32_bits(x), false, false);
+        x = bits_f32(r[0]) + bits_f32(r[1]);
+    }
+    return x;
 }
 
 // The eight values of a lane in LDS, in two planes of four so that neighbours' 16 bytes lie next to each other.
@@ -67,8 +91,8 @@ struct Plane {
 
 // kPasses: heads of a lane. A pass has 64 / lanes heads, or 256 / lanes where the norm is over the row.
 template <int T, int kPasses, bool kRow>
-__global__ __launch_bounds__(kThreads) void qk_norm_rope_kernel(const RopeArgs p, int lanes, int64_t items, int chunks_q,
-                                                                int chunks) {
+__global__ __launch_bounds__(kThreads) void qk_norm_rope_kernel(const RopeArgs p, int lanes, uint32_t items, uint32_t chunks_q,
+                                                                uint32_t chunks) {
     __shared__ Plane planes[kThreads / 64];
     __shared__ float sums[kThreads / 64];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
@@ -78,136 +102,161 @@ __global__ __launch_bounds__(kThreads) void qk_norm_rope_kernel(const RopeArgs p
     const bool has = d < p.dim;
     Plane& plane = planes[wave];
 
-    for (int64_t item = kRow ? blockIdx.x : static_cast<int64_t>(blockIdx.x) * (kThreads / 64) + wave; item < items;
-         item += static_cast<int64_t>(gridDim.x) * (kRow ? 1 : kThreads / 64)) {
-        const int64_t token = item / chunks;
-        const int chunk = static_cast<int>(item - token * chunks);
-        const int of_keys = chunk >= chunks_q;
-        const RopeSide& side = p.side[of_keys];
-        const int64_t b = token / p.per_sample, s = token - b * p.per_sample;
-        const int head0 = (chunk - of_keys * chunks_q) * heads_a_pass * kPasses + head_in_pass;
-        const uint8_t* x = side.x + b * side.batch_stride + s * side.token_stride + d * kSize<T>;
+    const uint32_t item = kRow ? blockIdx.x : blockIdx.x * (kThreads / 64) + wave;
+    if (item >= items) return;
+    const uint32_t token = item / chunks, chunk = item - token * chunks;
+    const bool of_keys = chunk >= chunks_q;
+    const RopeSide& side = p.side[of_keys];
+    const uint32_t b = token / static_cast<uint32_t>(p.per_sample), s = token - b * p.per_sample;
+    const int head0 = (chunk - (of_keys ? chunks_q : 0)) * heads_a_pass * kPasses + head_in_pass;
+    const uint8_t* x = side.x + b * side.batch_stride + s * side.token_stride + d * kSize<T>;
 
-        Values8<T> raw[kPasses];
+    Values8<T> raw[kPasses];
 #pragma unroll
-        for (int u = 0; u < kPasses; ++u) {
-            const int head = head0 + u * heads_a_pass;
-            raw[u] = {};
-            if (has && head < side.heads) raw[u] = load8<T>(x + head * side.head_stride);
+    for (int u = 0; u < kPasses; ++u) {
+        const int head = head0 + u * heads_a_pass;
+        raw[u] = {};
+        if (has && head < side.heads) raw[u] = load8<T>(x + head * side.head_stride);
+    }
+    // weights: one for all heads, or with a norm over the row each head's
+    constexpr int kWeights = kRow ? kPasses : 1;
+    Values8<kMxF32> weight[kWeights];
+    if (side.weight && has) {
+#pragma unroll
+        for (int u = 0; u < kWeights; ++u) {
+            const int head = kRow ? head0 + u * heads_a_pass : 0, at = head * p.dim + d;
+            if (head >= side.heads) continue;
+            const uint8_t* from = static_cast<const uint8_t*>(side.weight);
+            if (p.weight_f32) weight[u] = load8<kMxF32>(from + at * 4);
+            else weight[u].w[0] = load8<T>(from + at * kSize<T>).w[0];  // (fp32 values have fp32 weights)
         }
-        // the turn of each value: its pair's cosine and, with the sign of its place in the pair, sine
-        float cosine[8], sine[8];
+    }
+    // the turn of each value: its pair's cosine and, with the sign of its place in the pair, sine
+    float cosine[8], sine[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) cosine[i] = 1.0f, sine[i] = 0.0f;
-        if (p.table && has) {
-            const float* row = p.table + b * p.table_batch + s * p.pairs * 2;
-            if (p.halves) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int e = d + i;
-                    if (e < 2 * p.pairs) {
-                        const float* t = row + (e < p.pairs ? e : e - p.pairs) * 2;
-                        cosine[i] = t[0];
-                        sine[i] = e < p.pairs ? -t[1] : t[1];
-                    }
-                }
+    for (int i = 0; i < 8; ++i) cosine[i] = 1.0f, sine[i] = 0.0f;
+    const int turned = 2 * p.pairs;
+    if (p.table && d < turned) {
+        const float* row = p.table + b * p.table_batch + static_cast<int64_t>(s) * turned;
+        if (!p.halves) {
+            float t[8];
+            if (d + 8 <= turned) {
+                __builtin_memcpy(t, row + d, 32);
             } else {
 #pragma unroll
-                for (int i = 0; i < 8; i += 2)
-                    if (d + i < 2 * p.pairs) {
-                        cosine[i] = cosine[i + 1] = row[d + i];
-                        sine[i + 1] = row[d + i + 1];
-                        sine[i] = -sine[i + 1];
-                    }
+                for (int i = 0; i < 8; ++i) t[i] = d + i < turned ? row[d + i] : i % 2 ? 0.0f : 1.0f;
             }
-        }
-        float weight[8];
-        auto load_weight = [&](int at) {
-            if (p.weight_f32) widen8<kMxF32>(load8<kMxF32>(static_cast<const uint8_t*>(side.weight) + at * 4), weight);
-            else widen8<T>(load8<T>(static_cast<const uint8_t*>(side.weight) + at * kSize<T>), weight);
-        };
-        if (!kRow && side.weight && has) load_weight(d);
-
-        float v[kPasses][8], square[kPasses];
 #pragma unroll
-        for (int u = 0; u < kPasses; ++u) {
-            widen8<T>(raw[u], v[u]);
-            square[u] = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) square[u] += v[u][i] * v[u][i];
-        }
-        if (kRow) {
-            float all = 0.0f;
-#pragma unroll
-            for (int u = 0; u < kPasses; ++u) all += square[u];
-#pragma unroll
-            for (int m = 1; m < 64; m *= 2) all += __shfl_xor(all, m);
-            __syncthreads();  // (the sums of the item before have been read)
-            if (lane == 0) sums[wave] = all;
-            __syncthreads();
-            all = 0.0f;
-#pragma unroll
-            for (int w = 0; w < kThreads / 64; ++w) all += sums[w];
-            const float by = 1.0f / __builtin_sqrtf(all / (static_cast<float>(side.heads) * p.dim) + p.eps);
-#pragma unroll
-            for (int u = 0; u < kPasses; ++u)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[u][i] *= by;
-        } else if (p.norm) {
-            for (int m = 1; m < lanes; m *= 2)
-#pragma unroll
-                for (int u = 0; u < kPasses; ++u) square[u] += __shfl_xor(square[u], m);
-#pragma unroll
-            for (int u = 0; u < kPasses; ++u) {
-                const float by = 1.0f / __builtin_sqrtf(square[u] / p.dim + p.eps);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[u][i] *= by;
+            for (int i = 0; i < 8; i += 2) {
+                cosine[i] = cosine[i + 1] = t[i];
+                sine[i] = -t[i + 1];
+                sine[i + 1] = t[i + 1];
             }
-        }
-
-        uint8_t* out = side.out + token * side.heads * p.dim * kSize<T> + d * kSize<T>;
+        } else if (p.pairs % 8 == 0) {
+            const bool second = d >= p.pairs;
+            float t[16];
+            __builtin_memcpy(t, row + (second ? d - p.pairs : d) * 2, 64);
 #pragma unroll
-        for (int u = 0; u < kPasses; ++u) {
-            const int head = head0 + u * heads_a_pass;
-            if (side.weight) {
-                if (kRow && has && head < side.heads) load_weight(head * p.dim + d);
-                if (has && (!kRow || head < side.heads)) {
+            for (int i = 0; i < 8; ++i) {
+                cosine[i] = t[2 * i];
+                sine[i] = second ? t[2 * i + 1] : -t[2 * i + 1];
+            }
+        } else {
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) v[u][i] *= weight[i];
+            for (int i = 0; i < 8; ++i) {
+                const int e = d + i;
+                if (e < turned) {
+                    const float* t = row + (e < p.pairs ? e : e - p.pairs) * 2;
+                    cosine[i] = t[0];
+                    sine[i] = e < p.pairs ? -t[1] : t[1];
                 }
             }
-            if (p.table) {
-                float other[8];
-                if (p.halves) {
-                    plane.quad[0][lane] = make_float4(v[u][0], v[u][1], v[u][2], v[u][3]);
-                    plane.quad[1][lane] = make_float4(v[u][4], v[u][5], v[u][6], v[u][7]);
-                    wave_lds_sync();
-                    const int first = lane / lanes * lanes;  // the lane with the head's first values
-                    if (p.pairs % 4 == 0) {
-                        // four values at once have their partners next to each other, on one side
+        }
+    }
+
+    float v[kPasses][8], square[kPasses];
 #pragma unroll
-                        for (int i = 0; i < 8; i += 4) {
-                            const int e = d + i, from = e < p.pairs ? e + p.pairs : e < 2 * p.pairs ? e - p.pairs : e;
-                            const float4 q = plane.quad[from / 4 % 2][(first + from / 8) % 64];
-                            other[i] = q.x, other[i + 1] = q.y, other[i + 2] = q.z, other[i + 3] = q.w;
-                        }
-                    } else {
+    for (int u = 0; u < kPasses; ++u) {
+        widen8<T>(raw[u], v[u]);
+        square[u] = 0.0f;
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            const int e = d + i, from = e < p.pairs ? e + p.pairs : e < 2 * p.pairs ? e - p.pairs : e;
-                            other[i] = reinterpret_cast<const float*>(&plane.quad[from / 4 % 2][(first + from / 8) % 64])[from % 4];
-                        }
+        for (int i = 0; i < 8; ++i) square[u] += v[u][i] * v[u][i];
+    }
+    if (kRow) {
+        float all = 0.0f;
+#pragma unroll
+        for (int u = 0; u < kPasses; ++u) all += square[u];
+        all = sum_lanes(all, 64);
+        if (lane == 0) sums[wave] = all;
+        __syncthreads();
+        all = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kThreads / 64; ++w) all += sums[w];
+        const float by = 1.0f / __builtin_sqrtf(all / (static_cast<float>(side.heads) * p.dim) + p.eps);
+#pragma unroll
+        for (int u = 0; u < kPasses; ++u)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[u][i] *= by;
+    } else if (p.norm) {
+        const float one = 1.0f / p.dim;
+#pragma unroll
+        for (int u = 0; u < kPasses; ++u) {
+            const float by = __builtin_amdgcn_rsqf(sum_lanes(square[u], lanes) * one + p.eps);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[u][i] *= by;
+        }
+    }
+    if (side.weight) {
+#pragma unroll
+        for (int u = 0; u < kPasses; ++u) {
+            float f[8];
+            if (p.weight_f32) {
+                widen8<kMxF32>(weight[kRow ? u : 0], f);
+            } else {
+                Values8<T> h{};
+                h.w[0] = weight[kRow ? u : 0].w[0];
+                widen8<T>(h, f);
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[u][i] *= f[i];
+        }
+    }
+
+    uint8_t* out = side.out + static_cast<int64_t>(token) * side.heads * p.dim * kSize<T> + d * kSize<T>;
+#pragma unroll
+    for (int u = 0; u < kPasses; ++u) {
+        const int head = head0 + u * heads_a_pass;
+        if (p.table) {
+            float other[8];
+            if (p.halves) {
+                plane.quad[0][lane] = make_float4(v[u][0], v[u][1], v[u][2], v[u][3]);
+                plane.quad[1][lane] = make_float4(v[u][4], v[u][5], v[u][6], v[u][7]);
+                wave_lds_sync();
+                const int first = lane / lanes * lanes;  // the lane with the head's first values
+                if (p.pairs % 4 == 0) {
+                    // four values at once have their partners next to each other, on one side
+#pragma unroll
+                    for (int i = 0; i < 8; i += 4) {
+                        const int e = d + i, from = e < p.pairs ? e + p.pairs : e < turned ? e - p.pairs : e;
+                        const float4 q = plane.quad[from / 4 % 2][(first + from / 8) % 64];
+                        other[i] = q.x, other[i + 1] = q.y, other[i + 2] = q.z, other[i + 3] = q.w;
                     }
-                    wave_lds_sync();  // (read before the next pass writes)
                 } else {
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) other[i] = v[u][i ^ 1];
+                    for (int i = 0; i < 8; ++i) {
+                        const int e = d + i, from = e < p.pairs ? e + p.pairs : e < turned ? e - p.pairs : e;
+                        other[i] = reinterpret_cast<const float*>(&plane.quad[from / 4 % 2][(first + from / 8) % 64])[from % 4];
+                    }
                 }
+                wave_lds_sync();  // (read before the next pass writes)
+            } else {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) v[u][i] = v[u][i] * cosine[i] + other[i] * sine[i];
+                for (int i = 0; i < 8; ++i) other[i] = v[u][i ^ 1];
             }
-            if (has && head < side.heads) store8<T>(out + static_cast<int64_t>(head) * p.dim * kSize<T>, v[u]);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[u][i] = v[u][i] * cosine[i] + other[i] * sine[i];
         }
+        if (has && head < side.heads) store8<T>(out + static_cast<int64_t>(head) * p.dim * kSize<T>, v[u]);
     }
 }
 
@@ -216,9 +265,9 @@ int launch(const RopeArgs& p, int lanes, hipStream_t stream) {
     const int heads = (kRow ? kThreads : 64) / lanes * kPasses;
     const int chunks_q = (p.side[0].heads + heads - 1) / heads, chunks = chunks_q + (p.side[1].heads + heads - 1) / heads;
     const int64_t items = p.tokens * chunks, blocks = kRow ? items : (items + kThreads / 64 - 1) / (kThreads / 64);
+    if (blocks * kThreads > 0xffffffffll) return FEATHER_ERR_UNSUPPORTED;  // (terabytes)
     auto* kernel = qk_norm_rope_kernel<T, kPasses, kRow>;
-    kernel<<<dim3(static_cast<uint32_t>(std::min<int64_t>(blocks, 1 << 22))), kThreads, 0, stream>>>(p, lanes, items, chunks_q,
-                                                                                                  chunks);
+    kernel<<<dim3(static_cast<uint32_t>(blocks)), kThreads, 0, stream>>>(p, lanes, static_cast<uint32_t>(items), chunks_q, chunks);
     return hipGetLastError() == hipSuccess ? FEATHER_OK : FEATHER_ERR_LAUNCH;
 }
 
@@ -231,13 +280,16 @@ int of_type(const RopeArgs& p, hipStream_t stream) {
         const int passes = (most * lanes + kThreads - 1) / kThreads;
         if (passes <= 1) return launch<T, 1, true>(p, lanes, stream);
         if (passes <= 2) return launch<T, 2, true>(p, lanes, stream);
+        if (passes <= 3) return launch<T, 3, true>(p, lanes, stream);
         if (passes <= 4) return launch<T, 4, true>(p, lanes, stream);
         return launch<T, 8, true>(p, lanes, stream);
     }
-    // few tokens: a wave for every 64 / lanes heads
-    const int passes = p.tokens < 256 ? 1 : (most * lanes + 63) / 64;
-    if (passes <= 1) return launch<T, 1, false>(p, lanes, stream);
-    if (passes <= 2) return launch<T, 2, false>(p, lanes, stream);
+    // Few tokens: a wave for every 64 / lanes heads. Many: a wave takes three or four times as many, which leaves the fewest
+    // lanes idle at the row's end.
+    const int all = (most * lanes + 63) / 64;
+    if (p.tokens < 256 || all <= 1) return launch<T, 1, false>(p, lanes, stream);
+    if (all <= 2) return launch<T, 2, false>(p, lanes, stream);
+    if ((all + 2) / 3 * 3 < (all + 3) / 4 * 4) return launch<T, 3, false>(p, lanes, stream);
     return launch<T, 4, false>(p, lanes, stream);
 }
 
