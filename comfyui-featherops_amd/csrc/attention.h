@@ -30,7 +30,19 @@ struct AttnArgs {
     float scale;
 };
 
-int attention_tiles_f16(const AttnArgs& p, hipStream_t stream);
-int attention_tiles_bf16(const AttnArgs& p, hipStream_t stream);
+// Which kernel takes a call, and how.
+struct AttnPlan {
+    int waves;      // attention_rows.h with 4 or 8 waves; 0: attention_tiles.h
+    int64_t slots;  // blocks of rows, of one head or of one group of heads
+    int splits;     // workgroups that share a block's keys, at most
+    int least;      // tiles of 32 keys that one of them has at least
+    size_t workspace;
+};
+constexpr size_t kAttnCounterBytes = 65536;
+constexpr int kAttnMostSplits = 64;
+AttnPlan attention_plan(const AttnArgs& p);
+
+int attention_f16(const AttnArgs& p, const AttnPlan& plan, void* workspace, hipStream_t stream);
+int attention_bf16(const AttnArgs& p, const AttnPlan& plan, void* workspace, hipStream_t stream);
 
 }  // namespace feather

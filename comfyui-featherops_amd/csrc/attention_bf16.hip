@@ -1,8 +1,10 @@
-// Attention over many queries in bf16 (attention_tiles.h).
-#include "attention_tiles.h"
+// Attention in bf16.
+#include "attention_launch.h"
 
 namespace feather {
 
-int attention_tiles_bf16(const AttnArgs& p, hipStream_t stream) { return attention_tiles<true>(p, stream); }
+int attention_bf16(const AttnArgs& p, const AttnPlan& plan, void* workspace, hipStream_t stream) {
+    return attention_of_type<true>(p, plan, workspace, stream);
+}
 
 }  // namespace feather

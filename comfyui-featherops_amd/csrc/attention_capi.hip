@@ -146,12 +146,34 @@ int feather_qk_norm_rope(const feather_rope_args* a, hipStream_t stream) {
     return qk_norm_rope(p, stream);
 }
 
-int feather_attention(const feather_attention_args* a, hipStream_t stream) {
+size_t feather_attention_workspace_size(const feather_attention_args* a) {
+    AttnArgs p{};
+    bool empty = false;
+    return attention_args(a, p, empty) != FEATHER_OK || empty ? 0 : attention_plan(p).workspace;
+}
+
+int feather_attention_plan(const feather_attention_args* a, int64_t* plan) {
+    if (!plan) return FEATHER_ERR_INVALID;
+    AttnArgs p{};
+    bool empty = false;
+    const int status = attention_args(a, p, empty);
+    plan[0] = plan[1] = plan[2] = 0;
+    if (status != FEATHER_OK || empty) return status;
+    const AttnPlan chosen = attention_plan(p);
+    plan[0] = chosen.waves;
+    plan[1] = chosen.splits;
+    plan[2] = chosen.slots * (chosen.waves ? p.kv_heads : p.heads);
+    return FEATHER_OK;
+}
+
+int feather_attention(const feather_attention_args* a, void* workspace, size_t workspace_bytes, hipStream_t stream) {
     AttnArgs p{};
     bool empty = false;
     const int status = attention_args(a, p, empty);
     if (status != FEATHER_OK || empty) return status;
-    return p.bf16 ? attention_tiles_bf16(p, stream) : attention_tiles_f16(p, stream);
+    AttnPlan plan = attention_plan(p);
+    if (!workspace || workspace_bytes < plan.workspace) plan.splits = 1;
+    return p.bf16 ? attention_bf16(p, plan, workspace, stream) : attention_f16(p, plan, workspace, stream);
 }
 
 }  // extern "C"

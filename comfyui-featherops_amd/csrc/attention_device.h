@@ -3,6 +3,7 @@
 #pragma once
 
 #include "attention.h"
+#include "featherops_amd.h"
 #include "lds_dma.h"
 
 namespace feather {
@@ -181,5 +182,217 @@ constexpr float kLog2e = 1.4426950408889634f;
 template <bool kBf16>
 constexpr float kWeightBias = kBf16 ? 0.0f : 7.0f;
 constexpr float kMaxLag = 8.0f;
+
+// ---- a wave's 32 queries ----
+
+// Eight mask values of consecutive keys as they lie in memory, of which the first n exist (the rest reads as zeros).
+template <int kMask>
+constexpr int kMaskBytes = kMask == kMaskBool ? 1 : kMask == kMaskHalf ? 2 : 4;
+template <int kMask>
+__device__ __forceinline__ void load_mask8(const uint8_t* p, int n, uint32_t (&w)[2 * kMaskBytes<kMask>]) {
+    if (n >= 8) {
+        __builtin_memcpy(w, p, 8 * kMaskBytes<kMask>);
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 2 * kMaskBytes<kMask>; ++i) w[i] = 0;
+#pragma unroll
+    for (int j = 0; j < 7; ++j) {
+        if (j >= n) continue;
+        if constexpr (kMask == kMaskBool) w[j / 4] |= static_cast<uint32_t>(p[j]) << (8 * (j % 4));
+        else if constexpr (kMask == kMaskHalf) w[j / 2] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(p)[j]) << (16 * (j % 2));
+        else w[j] = reinterpret_cast<const uint32_t*>(p)[j];
+    }
+}
+
+// The mask's values for a wave's 32 queries and a tile's keys: lanes l and l + 32 load eight keys of the same query, l
+// those of group 2 j, l + 32 of 2 j + 1.
+template <bool kBf16, int kMask, int kKeyBlocks>
+struct AttnMaskRegs {
+    // values that are added to the scores: the scale comes before them
+    static constexpr bool kAdds = kMask == kMaskHalf || kMask == kMaskF32;
+    uint32_t raw[kKeyBlocks][2][kMask ? 2 * kMaskBytes<kMask> : 1];
+
+    // those of the tile whose first key is key0, from the query's row; it has `keys` of them
+    __device__ __forceinline__ void load(const uint8_t* from, int key0, int keys) {
+        if constexpr (kMask != kMaskNone) {
+#pragma unroll
+            for (int kb = 0; kb < kKeyBlocks; ++kb)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const int key = key0 + kb * 32 + (2 * j + static_cast<int>(threadIdx.x) % 64 / 32) * 8;
+                    load_mask8<kMask>(from + static_cast<int64_t>(key) * kMaskBytes<kMask>, keys - key, raw[kb][j]);
+                }
+        }
+    }
+    // They are in their registers from here on.
+    __device__ __forceinline__ void arrive() {
+        if constexpr (kMask != kMaskNone) {
+#pragma unroll
+            for (int kb = 0; kb < kKeyBlocks; ++kb)
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int i = 0; i < 2 * kMaskBytes<kMask>; ++i) asm volatile("" : "+v"(raw[kb][j][i]));
+        }
+    }
+    __device__ __forceinline__ void put(f32x16 (&s)[kKeyBlocks], float scale) {
+        if constexpr (kMask != kMaskNone) {
+            constexpr int kWords = kMaskBytes<kMask>;  // of four keys
+#pragma unroll
+            for (int kb = 0; kb < kKeyBlocks; ++kb)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    // lanes 32 apart trade four keys, so that each has four of both groups
+                    uint32_t w[2][kWords];
+#pragma unroll
+                    for (int i = 0; i < kWords; ++i) {
+                        const auto x = __builtin_amdgcn_permlane32_swap(raw[kb][j][i], raw[kb][j][kWords + i], false, false);
+                        w[0][i] = x[0];
+                        w[1][i] = x[1];
+                    }
+#pragma unroll
+                    for (int g = 0; g < 2; ++g)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int at = (2 * j + g) * 4 + e;
+                            if constexpr (kMask == kMaskBool) {
+                                s[kb][at] = (w[g][0] >> (8 * e)) & 0xff ? s[kb][at] : -INFINITY;
+                            } else {
+                                float add;
+                                if constexpr (kMask == kMaskHalf) add = out_bits_to_f32<kBf16>(static_cast<uint16_t>(w[g][e / 2] >> (16 * (e % 2))));
+                                else add = bits_f32(w[g][e]);
+                                s[kb][at] = s[kb][at] * scale + add;
+                            }
+                        }
+                }
+        }
+    }
+};
+
+// -inf for the tile's keys from `limit` on.
+template <int kKeyBlocks>
+__device__ __forceinline__ void attn_cut(f32x16 (&s)[kKeyBlocks], int key0, int limit) {
+    const int first = key0 + static_cast<int>(threadIdx.x) % 64 / 32 * 4;
+#pragma unroll
+    for (int kb = 0; kb < kKeyBlocks; ++kb)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+            if (first + kb * 32 + e / 4 * 8 + e % 4 >= limit) s[kb][e] = -INFINITY;
+}
+
+// Where a lane reads in a tile: keys' chunk 2 s + lane / 32 of row lane % 32; values' four rows 4 (lane / 32) + i / 4 of
+// block b's 32 columns, lane i of 16 giving four columns.
+template <int kDim>
+__device__ __forceinline__ void attn_lds_places(uint32_t keys, uint32_t values, uint32_t (&k_at)[kDim / 16], uint32_t (&v_at)[kDim / 32]) {
+    const int lane = threadIdx.x % 64, l32 = lane % 32, half = lane / 32;
+#pragma unroll
+    for (int s = 0; s < kDim / 16; ++s) k_at[s] = keys + l32 * (kDim * 2) + ((2 * s + half) ^ swz_k<kDim>(l32)) * 16;
+    const int i = lane % 16, r = 4 * half + i / 4;
+#pragma unroll
+    for (int b = 0; b < kDim / 32; ++b) {
+        const int byte = b * 64 + (lane / 16 % 2) * 32 + (i % 4) * 8;
+        v_at[b] = values + r * (kDim * 2) + ((byte / 16) ^ swz_v<kDim>(r)) * 16 + byte % 16;
+    }
+}
+
+// Far below every score, but finite, and finite times the factor: a row that has seen nothing stays at weights 0.
+template <bool kAdds>
+__device__ __forceinline__ float kLowest(float factor) {
+    return kAdds ? -3.402823466e38f : -8.0e37f / fmaxf(factor, 1.0f);
+}
+
+// One pass over the keys for 32 queries, a lane and the lane 32 away having one of them.
+//
+// The products are taken transposed, S^T = K Q^T and O^T = V^T P^T: a lane then has one query's
+// column of scores, so maximum and sum run inside the lane, and the scores' registers, rounded to 16
+// bits, are the second product's operand as they stand. The order of the 16 keys of an MFMA
+// is free as long as both operands have it; V's is the one that the score layout leaves,
+// which the transposing LDS read delivers. The maximum is replaced (and the sums scaled) only where
+// a score exceeds it by more than 2^8: its value cancels in the result.
+template <int kDim, bool kBf16, int kMask, int kKeyBlocks>
+struct AttnWave {
+    static constexpr int kSteps = kDim / 16, kBlocks = kDim / 32, kRowBytes = kDim * 2;
+    static constexpr float kBias = kWeightBias<kBf16>;
+    using Mask = AttnMaskRegs<kBf16, kMask, kKeyBlocks>;
+    static constexpr bool kAdds = Mask::kAdds;
+
+    u32x4 qf[kSteps];  // the queries: K Q^T's second operand
+    uint32_t k_at[kSteps], v_at[kBlocks];
+    f32x16 o[kBlocks];  // element 4 g + j of block b: column 32 b + 8 g + 4 (lane / 32) + j
+    float factor, scale, top, total;
+    Mask mask;
+    const uint8_t* mask_row;
+
+    // Tiles of keys lie at `keys` in LDS, of values at `values` (plus what scores() and add() are given).
+    __device__ __forceinline__ void start(uint32_t keys, uint32_t values, float by) {
+        attn_lds_places<kDim>(keys, values, k_at, v_at);
+        scale = by;
+        factor = kAdds ? kLog2e : by * kLog2e;
+        top = kLowest<kAdds>(factor);
+        total = 0.0f;
+#pragma unroll
+        for (int b = 0; b < kBlocks; ++b) o[b] = f32x16{};
+    }
+
+    __device__ __forceinline__ void scores(uint32_t stage, f32x16 (&s)[kKeyBlocks]) {
+#pragma unroll
+        for (int kb = 0; kb < kKeyBlocks; ++kb) s[kb] = f32x16{};
+#pragma unroll
+        for (int st = 0; st < kSteps; ++st)
+#pragma unroll
+            for (int kb = 0; kb < kKeyBlocks; ++kb)
+                s[kb] = mfma32<kBf16>(lds_read16(k_at[st] + stage + kb * 32 * kRowBytes), qf[st], s[kb]);
+    }
+
+    // The mask's values on the scores, and -inf for keys from `limit` on where some of the tile's are (`cut`).
+    __device__ __forceinline__ void masked(f32x16 (&s)[kKeyBlocks], int key0, int limit, bool cut) {
+        mask.put(s, scale);
+        if (cut) attn_cut<kKeyBlocks>(s, key0, limit);
+    }
+
+    __device__ __forceinline__ void weights(f32x16 (&s)[kKeyBlocks], u32x4 (&pf)[2 * kKeyBlocks]) {
+        float high = s[0][0];
+#pragma unroll
+        for (int kb = 0; kb < kKeyBlocks; ++kb)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) high = fmaxf(high, s[kb][e]);
+        high = max_halves(high);
+        if (__any((high - top) * factor > kMaxLag)) {
+            const float next = fmaxf(top, high);
+            const float alpha = __builtin_amdgcn_exp2f((top - next) * factor);
+            top = next;
+            total *= alpha;
+#pragma unroll
+            for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[b][e] *= alpha;
+        }
+        const float shift = kBias - top * factor;
+#pragma unroll
+        for (int kb = 0; kb < kKeyBlocks; ++kb)
+#pragma unroll
+            for (int e = 0; e < 16; e += 2) {
+                float w[2];
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    w[j] = __builtin_amdgcn_exp2f(kAdds ? (s[kb][e + j] - top) * factor + kBias : s[kb][e + j] * factor + shift);
+                    total += w[j];
+                }
+                pf[kb * 2 + e / 8][e % 8 / 2] = pack2<kBf16>(w[0], w[1]);
+            }
+    }
+
+    __device__ __forceinline__ void add(uint32_t stage, const u32x4 (&pf)[2 * kKeyBlocks]) {
+#pragma unroll
+        for (int g = 0; g < 2 * kKeyBlocks; ++g)
+#pragma unroll
+            for (int b = 0; b < kBlocks; ++b) {
+                const u32x2 lo = lds_read_transposed(v_at[b] + stage + g * 16 * kRowBytes);
+                const u32x2 hi = lds_read_transposed(v_at[b] + stage + (g * 16 + 8) * kRowBytes);
+                o[b] = mfma32<kBf16>(u32x4{lo[0], lo[1], hi[0], hi[1]}, pf[g], o[b]);
+            }
+    }
+};
 
 }  // namespace feather

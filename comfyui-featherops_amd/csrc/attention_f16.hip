@@ -1,8 +1,10 @@
-// Attention over many queries in fp16 (attention_tiles.h).
-#include "attention_tiles.h"
+// Attention in fp16.
+#include "attention_launch.h"
 
 namespace feather {
 
-int attention_tiles_f16(const AttnArgs& p, hipStream_t stream) { return attention_tiles<false>(p, stream); }
+int attention_f16(const AttnArgs& p, const AttnPlan& plan, void* workspace, hipStream_t stream) {
+    return attention_of_type<false>(p, plan, workspace, stream);
+}
 
 }  // namespace feather

@@ -1,120 +1,138 @@
 // Attention over many queries: o = softmax(scale * q k^T + mask) v, one pass over the keys with a
 // running maximum and sum.
 //
-// A wave holds 32 queries of one head, a workgroup of four 128; tiles of kKeys keys and values pass
-// through a ring of two stages in LDS that all waves share, copied while the one before is worked on.
-// The products are taken transposed, S^T = K Q^T and O^T = V^T P^T: a lane then has one query's
-// column of scores, so maximum and sum run inside the lane, and the scores' registers, rounded to 16
-// bits, are the second product's operand as they stand. The order of the 16 keys of an MFMA
-// is free as long as both operands have it; V's is the one that the score layout leaves,
-// which the transposing LDS read delivers. The maximum is replaced (and the sums scaled) only where
-// a score exceeds it by more than 2^8: its value cancels in the result.
+// A wave holds 32 queries of one head, a workgroup of four 128. Keys and values pass through two
+// rings of units of 32 keys in LDS that all waves share; two waves copy keys, two copy values, several
+// units ahead. In its turn u a wave makes the weights of unit u from its scores, which is work for the vector
+// units, and beside it runs the products that give the scores of unit u + 1 and that add the values of
+// unit u - 1: the instructions of both stand alternately in the code, since a wave issues them in order and the
+// second of two products would hold up whatever stands behind it. (With the products of a unit first and
+// its weights behind them, 32760 x 32760 x 12 heads of 128 took 7.0 ms: the two overlapped only between the two waves of
+// a SIMD.)
+//
+// The products are taken transposed, as in AttnWave. They are inline asm, which keeps their order and their
+// accumulators' place: results in accumulation registers where the vector registers do not hold everything.
 #pragma once
 
 #include "attention_device.h"
-#include "featherops_amd.h"
 
 namespace feather {
 
-template <int kDim>
+template <int kDim, int kMask>
 struct AttnTile {
     static constexpr int kWaves = 4;
     static constexpr int kRows = 32 * kWaves;
-    static constexpr int kKeys = kDim == 256 ? 32 : 64;
-    static constexpr int kTileBytes = kKeys * kDim * 2;            // of keys or of values
-    static constexpr int kCopies = kTileBytes / 1024 / kWaves;     // instructions a wave, for each of them
-    static constexpr int kLds = 4 * kTileBytes;
+    static constexpr int kUnitBytes = 32 * kDim * 2;  // of keys or of values
+    static constexpr int kCopies = kUnitBytes / 2048;  // instructions of each of two waves
+    static constexpr int kRing = 4;                    // units in each ring
+    // Units that are copied at once, and turns between barriers. A mask's values are loaded by the compiler's own loads,
+    // whose waits, as it knows of no copies, are waits for all copies before them: so two turns apart.
+    static constexpr int kBatch = kMask == kMaskNone ? 1 : 2;
+    static constexpr int kLds = 2 * kRing * kUnitBytes;
+    static constexpr bool kAccumulation = kDim == 256;  // results in accumulation registers
 };
 
-// Four mask values of consecutive keys, of which the first n exist.
-template <int kMask, bool kBf16>
-__device__ __forceinline__ void mask4(const uint8_t* p, int n, float add[4]) {
-    if (n <= 0) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) add[j] = 0.0f;
-        return;
-    }
-    if constexpr (kMask == kMaskBool) {
-        uint32_t w;
-        if (n >= 4) {
-            __builtin_memcpy(&w, p, 4);
-        } else {
-            w = p[0] | (n > 1 ? p[1] << 8 : 0) | (n > 2 ? p[2] << 16 : 0);
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) add[j] = (w >> (8 * j)) & 0xff ? 0.0f : -INFINITY;
-    } else if constexpr (kMask == kMaskHalf) {
-        uint32_t w[2] = {0, 0};
-        if (n >= 4) {
-            __builtin_memcpy(w, p, 8);
-        } else {
-            const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
-            w[0] = h[0] | (n > 1 ? h[1] << 16 : 0);
-            w[1] = n > 2 ? h[2] : 0;
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) add[j] = out_bits_to_f32<kBf16>(static_cast<uint16_t>(w[j / 2] >> (16 * (j % 2))));
+// Their hazards are the code's own business: a source that another vector instruction wrote needs two wait states before
+// the product (kPadded puts them there), whoever else reads a result waits for it.
+#define FEATHER_MFMA32(type, before, result, from, after) \
+    asm volatile(before "v_mfma_f32_32x32x16_" type " %0, %1, %2, " from after : result(c) : "v"(a), "v"(b))
+template <bool kBf16>
+__device__ __forceinline__ void mfma_first(f32x16& c, u32x4 a, u32x4 b) {
+    if constexpr (kBf16) FEATHER_MFMA32("bf16", "s_nop 1\n\t", "=&v", "0", "");
+    else FEATHER_MFMA32("f16", "s_nop 1\n\t", "=&v", "0", "");
+}
+template <bool kBf16, bool kAccumulation, bool kPadded>
+__device__ __forceinline__ void mfma_next(f32x16& c, u32x4 a, u32x4 b) {
+    if constexpr (kAccumulation) {
+        if constexpr (kBf16) FEATHER_MFMA32("bf16", "s_nop 1\n\t", "+a", "%0", "");
+        else FEATHER_MFMA32("f16", "s_nop 1\n\t", "+a", "%0", "");
+    } else if constexpr (kPadded) {
+        if constexpr (kBf16) FEATHER_MFMA32("bf16", "s_nop 1\n\t", "+v", "%0", "");
+        else FEATHER_MFMA32("f16", "s_nop 1\n\t", "+v", "%0", "");
     } else {
-        if (n >= 4) {
-            __builtin_memcpy(add, p, 16);
-        } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) add[j] = j < n ? reinterpret_cast<const float*>(p)[j] : 0.0f;
-        }
+        if constexpr (kBf16) FEATHER_MFMA32("bf16", "", "+v", "%0", "");
+        else FEATHER_MFMA32("f16", "", "+v", "%0", "");
     }
 }
+// One with the waits on both sides: its result is in its registers behind it (at most 19 wait states).
+template <bool kBf16, bool kAccumulation>
+__device__ __forceinline__ void mfma_alone(f32x16& c, u32x4 a, u32x4 b) {
+    if constexpr (kAccumulation) {
+        if constexpr (kBf16) FEATHER_MFMA32("bf16", "s_nop 1\n\t", "+a", "%0", "\n\ts_nop 15\n\ts_nop 3");
+        else FEATHER_MFMA32("f16", "s_nop 1\n\t", "+a", "%0", "\n\ts_nop 15\n\ts_nop 3");
+    } else {
+        if constexpr (kBf16) FEATHER_MFMA32("bf16", "s_nop 1\n\t", "+v", "%0", "\n\ts_nop 15\n\ts_nop 3");
+        else FEATHER_MFMA32("f16", "s_nop 1\n\t", "+v", "%0", "\n\ts_nop 15\n\ts_nop 3");
+    }
+}
+#undef FEATHER_MFMA32
+// Until the scores are in their registers: reads of them stay behind.
+__device__ __forceinline__ void settle(f32x16& s) { asm volatile("s_nop 15\n\ts_nop 3" : "+v"(s)); }
 
 template <int kDim, bool kBf16, int kMask>
-__global__ __launch_bounds__(256, kDim <= 128 ? 2 : 1) void attention_tile_kernel(const AttnArgs p, int slots, int64_t per_xcd) {
-    using T = AttnTile<kDim>;
-    constexpr int kSteps = kDim / 16, kBlocks = kDim / 32, kKeyBlocks = T::kKeys / 32;
-    constexpr int kRowBytes = kDim * 2;
-    extern __shared__ __attribute__((aligned(1024))) uint8_t ring[];
+__global__ __launch_bounds__(256, kDim > 128 ? 1 : kDim == 64 && kMask == kMaskNone ? 4 : 2) void attention_tile_kernel(const AttnArgs p, int slots, int64_t per_xcd) {
+    using T = AttnTile<kDim, kMask>;
+    using Mask = AttnMaskRegs<kBf16, kMask, 1>;
+    constexpr int kSteps = kDim / 16, kBlocks = kDim / 32, kRowBytes = kDim * 2;
+    constexpr bool kAdds = Mask::kAdds;
+    constexpr float kBias = kWeightBias<kBf16>;
+    __shared__ __attribute__((aligned(1024))) uint8_t rings[T::kLds];
 
     // workgroup i runs on XCD i % 8: each XCD takes consecutive blocks of few heads, whose keys its L2 keeps
     const int64_t id = static_cast<int64_t>(blockIdx.x % kNumXcd) * per_xcd + blockIdx.x / kNumXcd;
-    const int head_slot = static_cast<int>(id / slots);
-    if (blockIdx.x / kNumXcd >= per_xcd || head_slot >= p.heads) return;
-    // (causal: the blocks with most keys first)
-    const int slot = static_cast<int>(id - static_cast<int64_t>(head_slot) * slots);
+    const int head = static_cast<int>(id / slots);
+    if (blockIdx.x / kNumXcd >= per_xcd || head >= p.heads) return;
+    const int slot = static_cast<int>(id - static_cast<int64_t>(head) * slots);
     AttnJob job;
+    // (causal: the blocks with most keys first)
     if (!attn_job<T::kRows>(p, p.causal ? slots - 1 - slot : slot, 1, job)) return;
-    const int head = head_slot, kv_head = head / p.group;
+    const int kv_head = head / p.group;
 
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
     const int l32 = lane % 32, half = lane / 32;
-    const int row0 = job.row0 + wave * 32, row = row0 + l32;
-    // keys [0, limit) are this lane's query's; [0, wg_keys) some query's of the workgroup
+    const int row0 = job.row0 + wave * 32;
+    // keys [0, limit) are this lane's query's; the wave's queries see wave_keys at most and wave_least at least
     const int shift = job.keys - job.rows;  // the last query sees all keys
-    const int limit = p.causal ? min(job.keys, row + shift + 1) : job.keys;
-    const int wave_keys = p.causal ? min(job.keys, row0 + 31 + shift + 1) : job.keys;
+    const int limit = p.causal ? min(job.keys, row0 + l32 + shift + 1) : job.keys;
+    const int wave_keys = row0 >= job.rows ? 0 : p.causal ? min(job.keys, row0 + 32 + shift) : job.keys;
     const int wave_least = p.causal ? min(job.keys, row0 + shift + 1) : job.keys;
     const int wg_keys = p.causal ? min(job.keys, min(job.row0 + T::kRows, job.rows) + shift) : job.keys;
-    const int tiles = wg_keys > 0 ? (wg_keys + T::kKeys - 1) / T::kKeys : 0;
+    // units, in twos; two at least, of which a wave without keys sees none
+    const int units = max(1, (wave_keys + 63) / 64) * 2, all_units = (wg_keys + 31) / 32;
 
-    const uint8_t* k = p.k + job.b * p.k_batch + job.k_start * p.k_row + kv_head * p.k_head;
-    const uint8_t* v = p.v + job.b * p.v_batch + job.k_start * p.v_row + kv_head * p.v_head;
-    const uint32_t lds = lds_addr_of(ring);
-    uint32_t k_off[T::kCopies], v_off[T::kCopies];
+    // waves 0 and 1 copy keys, 2 and 3 values
+    const bool copies_keys = wave < 2;
+    const int64_t copy_row = copies_keys ? p.k_row : p.v_row;
+    const uint8_t* copy_from = copies_keys ? p.k + job.b * p.k_batch + job.k_start * p.k_row + kv_head * p.k_head
+                                           : p.v + job.b * p.v_batch + job.k_start * p.v_row + kv_head * p.v_head;
+    const uint32_t lds_k = lds_addr_of(rings), lds_v = lds_k + T::kRing * T::kUnitBytes;
+    const uint32_t copy_to = (copies_keys ? lds_k : lds_v) + wave % 2 * (T::kCopies * 1024);
+    uint32_t copy_off[T::kCopies];
 #pragma unroll
-    for (int i = 0; i < T::kCopies; ++i) {
-        k_off[i] = tile_offset<kDim, false>(wave * T::kCopies + i, lane, p.k_row, p.dim);
-        v_off[i] = tile_offset<kDim, true>(wave * T::kCopies + i, lane, p.v_row, p.dim);
-    }
-    auto copy_tile = [&](int t) {
-        const int key0 = t * T::kKeys;
-        const int64_t rows_left = job.keys - key0 - 1;
-        const i32x4 kb = buffer_of(k + key0 * p.k_row, rows_left * p.k_row + p.dim * 2);
-        const i32x4 vb = buffer_of(v + key0 * p.v_row, rows_left * p.v_row + p.dim * 2);
-        const uint32_t at = lds + (t & 1) * (2 * T::kTileBytes) + wave * (T::kCopies * 1024);
+    for (int i = 0; i < T::kCopies; ++i)
+        copy_off[i] = copies_keys ? tile_offset<kDim, false>(wave % 2 * T::kCopies + i, lane, copy_row, p.dim)
+                                  : tile_offset<kDim, true>(wave % 2 * T::kCopies + i, lane, copy_row, p.dim);
+    auto copy_unit = [&](int u) {  // (past the last key: zeros)
+        const int64_t key0 = u * 32;
+        const i32x4 b = buffer_of(copy_from + key0 * copy_row, key0 < job.keys ? (job.keys - key0 - 1) * copy_row + p.dim * 2 : 0);
+        const uint32_t at = copy_to + u % T::kRing * T::kUnitBytes;
 #pragma unroll
-        for (int i = 0; i < T::kCopies; ++i) buffer_to_lds(kb, k_off[i], at + i * 1024);
-#pragma unroll
-        for (int i = 0; i < T::kCopies; ++i) buffer_to_lds(vb, v_off[i], at + T::kTileBytes + i * 1024);
+        for (int i = 0; i < T::kCopies; ++i) buffer_to_lds(b, copy_off[i], at + i * 1024);
     };
-    if (tiles) copy_tile(0);
+    // What is copied before turn u: keys up to u + kRing, in the place of those that turn u - 1 has read last, and values up
+    // to u + kRing - 2 likewise.
+    const int ahead = copies_keys ? T::kRing : T::kRing - 2;
+    // Before turn u, the first one too (unit 0's keys have been read by then): what it and the kBatch - 1 behind it read of this wave's copies has landed (one turn at a time: all but
+    // the last unit's), and its reads of what is copied over next are done; then everyone's.
+    auto wait_batch = [&] {
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(T::kBatch == 1 ? T::kCopies : 0) : "memory");
+    };
+    auto copy_batch = [&](int u) {
+#pragma unroll
+        for (int i = 1 - T::kBatch; i <= 0; ++i) copy_unit(u + ahead + i);
+    };
+    for (int u = 0; u <= ahead - T::kBatch; ++u) copy_unit(u);
 
-    // queries: the second operand of K Q^T, kept in registers
     u32x4 qf[kSteps];
     {
         const uint8_t* q = p.q + job.b * p.q_batch + (job.q_start + static_cast<int64_t>(row0)) * p.q_row + head * p.q_head;
@@ -126,168 +144,216 @@ __global__ __launch_bounds__(256, kDim <= 128 ? 2 : 1) void attention_tile_kerne
                                                   qb, d < p.dim ? static_cast<uint32_t>(l32 * p.q_row) + d * 2 : kPastEnd, 0, 0));
         }
     }
-
-    // where in a tile this lane reads: keys' chunk 2 s + half of row l32; values' four rows 4 half + i / 4 of
-    // block b's 32 columns, lane i of 16 giving four columns
     uint32_t k_at[kSteps], v_at[kBlocks];
-#pragma unroll
-    for (int s = 0; s < kSteps; ++s) k_at[s] = lds + l32 * kRowBytes + ((2 * s + half) ^ swz_k<kDim>(l32)) * 16;
-    {
-        const int i = lane % 16, r = 4 * half + i / 4;
-#pragma unroll
-        for (int b = 0; b < kBlocks; ++b) {
-            const int byte = b * 64 + (lane / 16 % 2) * 32 + (i % 4) * 8;
-            v_at[b] = lds + T::kTileBytes + r * kRowBytes + ((byte / 16) ^ swz_v<kDim>(r)) * 16 + byte % 16;
-        }
-    }
-
-    const float factor = kMask ? kLog2e : p.scale * kLog2e;
-    constexpr float kBias = kWeightBias<kBf16>;
-    // far below every score, but finite, and finite times the factor: a row that has seen nothing stays at weights 0
-    float top = kMask ? -3.402823466e38f : -8.0e37f / fmaxf(factor, 1.0f);
-    float total = 0.0f;
-    f32x16 o[kBlocks];
+    attn_lds_places<kDim>(lds_k, lds_v, k_at, v_at);
+    // masks of two units each: what a turn cuts with was loaded two turns before (fp32 masks, which are too wide for that,
+    // in the turn before)
+    constexpr int kSets = kMask == kMaskF32 ? 1 : 2;
+    Mask mask[kSets][2];
+    const uint8_t* mask_row = nullptr;
+    if constexpr (kMask != kMaskNone)
+        mask_row = p.mask + job.b * p.mask_batch + head * p.mask_head + min(row0 + l32, job.rows - 1) * p.mask_row;
+    const float factor = kAdds ? kLog2e : p.scale * kLog2e;
+    float top = kLowest<kAdds>(factor), by, total = 0.0f;
+    f32x16 o[kBlocks], s0[1], s1[1];  // results; scores of even and odd units
+    u32x4 p0[2], p1[2];               // their weights
 #pragma unroll
     for (int b = 0; b < kBlocks; ++b) o[b] = f32x16{};
-    const uint8_t* mask = nullptr;
-    if constexpr (kMask != kMaskNone)
-        mask = p.mask + job.b * p.mask_batch + head * p.mask_head + min(row, job.rows - 1) * p.mask_row;
+    p1[0] = p1[1] = u32x4{};
+    auto read_k = [&](int s, uint32_t at) { return lds_read16(k_at[s] + at); };
+    auto read_v = [&](int n, uint32_t at) {  // block n % kBlocks of 16 keys
+        const uint32_t from = v_at[n % kBlocks] + at + n / kBlocks * 16 * kRowBytes;
+        const u32x2 lo = lds_read_transposed(from), hi = lds_read_transposed(from + 8 * kRowBytes);
+        return u32x4{lo[0], lo[1], hi[0], hi[1]};
+    };
+    // the mask on unit u's scores, and what a query does not see of it
+    auto cut = [&](f32x16 (&s)[1], Mask& mask, int u) {
+        const bool past = u * 32 + 32 > wave_least;
+        if (kMask != kMaskNone || past) settle(s[0]);
+        mask.put(s, p.scale);
+        if (past) attn_cut<1>(s, u * 32, limit);
+    };
+    auto load_masks = [&](Mask (&m)[2], int u) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) m[i].load(mask_row, (u + i) * 32, job.keys);
+    };
+    // Adds a unit's values at `at` with its weights; the results are in their registers behind it.
+    auto add_unit = [&](const u32x4 (&pf)[2], uint32_t at) {
+#pragma unroll
+        for (int n = 0; n < kSteps; ++n) mfma_alone<kBf16, T::kAccumulation>(o[n % kBlocks], read_v(n, at), pf[n / kBlocks]);
+    };
 
-    for (int t = 0; t < tiles; ++t) {
-        // this wave's copies of tile t have landed and its reads of the other stage are done; then everyone's
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        if (t + 1 < tiles) copy_tile(t + 1);
-        const int key0 = t * T::kKeys;
-        if (key0 >= wave_keys) continue;
-        const uint32_t stage = (t & 1) * (2 * T::kTileBytes);
-
-        f32x16 s[kKeyBlocks];
-#pragma unroll
-        for (int kb = 0; kb < kKeyBlocks; ++kb) s[kb] = f32x16{};
-#pragma unroll
-        for (int st = 0; st < kSteps; ++st)
-#pragma unroll
-            for (int kb = 0; kb < kKeyBlocks; ++kb)
-                s[kb] = mfma32<kBf16>(lds_read16(k_at[st] + stage + kb * 32 * kRowBytes), qf[st], s[kb]);
-
-        if constexpr (kMask != kMaskNone) {
-#pragma unroll
-            for (int kb = 0; kb < kKeyBlocks; ++kb)
-#pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    const int key = key0 + kb * 32 + g * 8 + half * 4;
-                    constexpr int kSize = kMask == kMaskBool ? 1 : kMask == kMaskHalf ? 2 : 4;
-                    float add[4];
-                    mask4<kMask, kBf16>(mask + static_cast<int64_t>(key) * kSize, job.keys - key, add);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) s[kb][g * 4 + j] = s[kb][g * 4 + j] * p.scale + add[j];
-                }
-        }
-        if (key0 + T::kKeys > wave_least) {
-#pragma unroll
-            for (int kb = 0; kb < kKeyBlocks; ++kb)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const int key = key0 + kb * 32 + (e / 4) * 8 + half * 4 + e % 4;
-                    if (key >= limit) s[kb][e] = -INFINITY;
-                }
-        }
-
-        float high = s[0][0];
-#pragma unroll
-        for (int kb = 0; kb < kKeyBlocks; ++kb)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) high = fmaxf(high, s[kb][e]);
-        high = max_halves(high);
+    // Unit u: its weights from its scores `now`; beside that the products that give the scores of the unit ahead, whose keys
+    // are at ka, and that add the unit before with its weights `old` and values at va. The keys of the unit after
+    // that are at kn. high: the scores' maximum, of `now` on the way in, of `next` on the way out.
+    u32x4 kf[3];
+    float high;
+    auto turn = [&](int u, f32x16 (&now)[1], f32x16 (&next)[1], u32x4 (&pf)[2], u32x4 (&old)[2], uint32_t ka, uint32_t va, uint32_t kn, Mask& its_mask,
+                    bool first, bool last) {
+        // (whether the turn begins a batch, with copies and after a barrier before which nothing is read ahead; whether it ends one)
+        // A maximum that has fallen behind is replaced. The unit before, whose weights are relative to it, is added now; its
+        // turn for it finds none.
         if (__any((high - top) * factor > kMaxLag)) {
-            const float next = fmaxf(top, high);
-            const float alpha = __builtin_amdgcn_exp2f((top - next) * factor);
-            top = next;
+            add_unit(old, va);
+            const float to = fmaxf(top, high);
+            const float alpha = __builtin_amdgcn_exp2f((top - to) * factor);
+            top = to;
+            by = kBias - to * factor;
             total *= alpha;
 #pragma unroll
             for (int b = 0; b < kBlocks; ++b)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) o[b][e] *= alpha;
+            old[0] = old[1] = u32x4{};
         }
-        const float shift_by = kBias - top * factor;
-        u32x4 pf[2 * kKeyBlocks];
+        // Two scores to weights, in two steps a product apart; the first product has the copies beside it.
+        float w[2];
+        auto beside = [&](int slot) {
 #pragma unroll
-        for (int kb = 0; kb < kKeyBlocks; ++kb)
+            for (int h = (slot - 1) * 16 / (2 * kSteps - 1); h < slot * 16 / (2 * kSteps - 1); ++h) {
+                const int e = h / 2 * 2;
+                if (h % 2 == 0) {
 #pragma unroll
-            for (int e = 0; e < 16; e += 2) {
-                float w[2];
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    w[j] = __builtin_amdgcn_exp2f(kMask ? (s[kb][e + j] - top) * factor + kBias
-                                                        : s[kb][e + j] * factor + shift_by);
-                    total += w[j];
+                    for (int j = 0; j < 2; ++j)
+                        w[j] = __builtin_amdgcn_exp2f(kAdds ? (now[0][e + j] - top) * factor + kBias : now[0][e + j] * factor + by);
+                } else {
+                    total += w[0];
+                    total += w[1];
+                    uint32_t both = pack2<kBf16>(w[0], w[1]);
+                    asm volatile("" : "+v"(both), "+v"(total));  // (here, not where they are used)
+                    pf[e / 8][e % 8 / 2] = both;
                 }
-                pf[kb * 2 + e / 8][e % 8 / 2] = pack2<kBf16>(w[0], w[1]);
             }
+        };
+        u32x4 vf[3];
+        static_assert(kSteps == 2 * kBlocks);
+        if (T::kBatch > 1 && first) {
+            kf[0] = read_k(0, ka);
+            kf[1] = read_k(1, ka);
+        }
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+            if (s + 2 < kSteps) kf[(s + 2) % 3] = read_k(s + 2, ka);
+            else vf[s + 2 - kSteps] = read_v(s + 2 - kSteps, va);
+            __builtin_amdgcn_sched_barrier(0);
+            if (s == 0) mfma_first<kBf16>(next[0], kf[0], qf[0]);
+            else mfma_next<kBf16, false, T::kAccumulation>(next[0], kf[s % 3], qf[s]);
+            __builtin_amdgcn_sched_barrier(0);
+            if (s) beside(s);
+            else if (first) copy_batch(u);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        cut(next, its_mask, u + 1);
+        if (kMask != kMaskNone && kSets == 1 && last) load_masks(mask[0], u + 2);
+        high = -INFINITY;
+#pragma unroll
+        for (int n = 0; n < kSteps; ++n) {
+            if (n + 2 < kSteps) vf[(n + 2) % 3] = read_v(n + 2, va);
+            else if (T::kBatch == 1 || !last) kf[n + 2 - kSteps] = read_k(n + 2 - kSteps, kn);
+            __builtin_amdgcn_sched_barrier(0);
+            mfma_next<kBf16, T::kAccumulation, T::kAccumulation>(o[n % kBlocks], vf[n % 3], old[n / kBlocks]);
+            __builtin_amdgcn_sched_barrier(0);
+            beside(kSteps + n);
+            // (the scores have settled: half of the products later)
+            constexpr int kFrom = kSteps / 2;
+            if (n >= kFrom) {
+#pragma unroll
+                for (int e = (n - kFrom) * 8 / kFrom * 2; e < (n - kFrom + 1) * 8 / kFrom * 2; e += 2)
+                    high = fmaxf(fmaxf(high, next[0][e]), next[0][e + 1]);
+            }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        high = max_halves(high);
+    };
 
+    // Units 0 to 2 of the keys and 0 of the values have landed.
+    Mask mask0;
+    mask0.load(mask_row, 0, job.keys);
+    load_masks(mask[0], 1);
+    wait_vmcnt<T::kBatch == 1 ? T::kCopies : 0>();
+    asm volatile("s_barrier" ::: "memory");
 #pragma unroll
-        for (int g = 0; g < 2 * kKeyBlocks; ++g)
-#pragma unroll
-            for (int b = 0; b < kBlocks; ++b) {
-                const u32x2 lo = lds_read_transposed(v_at[b] + stage + g * 16 * kRowBytes);
-                const u32x2 hi = lds_read_transposed(v_at[b] + stage + (g * 16 + 8) * kRowBytes);
-                o[b] = mfma32<kBf16>(u32x4{lo[0], lo[1], hi[0], hi[1]}, pf[g], o[b]);
-            }
+    for (int s = 0; s < kSteps; ++s) {
+        if (s == 0) mfma_first<kBf16>(s0[0], read_k(0, 0), qf[0]);
+        else mfma_next<kBf16, false, true>(s0[0], read_k(s, 0), qf[s]);
     }
+    if (T::kBatch == 1) {
+        kf[0] = read_k(0, T::kUnitBytes);
+        kf[1] = read_k(1, T::kUnitBytes);
+    }
+    if (kMask == kMaskNone) settle(s0[0]);
+    cut(s0, mask0, 0);
+    high = top;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) high = fmaxf(high, s0[0][e]);
+    top = high = max_halves(high);
+    by = kBias - top * factor;
 
-    total = sum_halves(total);
-    const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
+    // Two turns at a time, as the scores' registers alternate; two such in a row, so that places in the rings are constants.
+    constexpr uint32_t kUnit = T::kUnitBytes;
+    for (int u0 = 0; u0 < units; u0 += T::kRing) {
+#pragma unroll
+        for (int j = 0; j < T::kRing; ++j) {
+            const int u = u0 + j;
+            if (j == 2 && u >= units) break;
+            const bool first = j % T::kBatch == 0, last = (j + 1) % T::kBatch == 0;
+            const int set = j / 2 % kSets;
+            if (first) {
+                wait_batch();
+                if constexpr (kMask != kMaskNone) {  // (their wait here: further on it would be one for the next copies)
+                    mask[set][0].arrive();
+                    mask[set][1].arrive();
+                    if (kSets == 2) load_masks(mask[kSets - 1 - set], u + 3);
+                }
+            }
+            const uint32_t ka = (j + 1) % T::kRing * kUnit, kn = (j + 2) % T::kRing * kUnit;
+            // (unit 0 has none before it: weights of zero, on values that are there)
+            const uint32_t va = j ? (j - 1) * kUnit : u0 ? (T::kRing - 1) * kUnit : 0;
+            if (j % 2 == 0) turn(u, s0, s1, p0, p1, ka, va, kn, mask[set][0], first, last);
+            else turn(u, s1, s0, p1, p0, ka, va, kn, mask[set][1], first, last);
+        }
+    }
+    add_unit(p1, (units - 1) % T::kRing * kUnit);
+    for (int u = units; u < all_units; u += T::kBatch) {
+        wait_batch();
+        copy_batch(u);
+    }
+    wait_vmcnt<0>();  // (no copy may be on its way when the workgroup's LDS goes to another)
+
+    const int64_t out_row = static_cast<int64_t>(p.heads) * p.dim * 2;
+    uint16_t* out = p.out + ((static_cast<int64_t>(job.b) * p.sq + job.q_start + row0) * p.heads + head) * p.dim;
+    const auto ob = resource_of(out, (job.rows - row0 - 1) * out_row + p.dim * 2);
+    const float sum = sum_halves(total);
+    const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
+    // (the lane again: kept over the loop it would cost registers)
+    const int place_of = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u)), out_l32 = place_of % 32, out_half = place_of / 32;
     // element 4 g + j of block b is column 32 b + 8 g + 4 half + j: lanes 32 apart trade four columns, so that each
     // stores eight
-    uint16_t* out = p.out + ((static_cast<int64_t>(job.b) * p.sq + job.q_start + row0) * p.heads + head) * p.dim;
-    const int64_t out_row = static_cast<int64_t>(p.heads) * p.dim * 2;
-    const auto ob = resource_of(out, (job.rows - row0 - 1) * out_row + p.dim * 2);
 #pragma unroll
     for (int b = 0; b < kBlocks; ++b)
 #pragma unroll
         for (int g = 0; g < 4; g += 2) {
-            uint32_t w[2][2];
+            uint32_t h[2][2];
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll
                 for (int j = 0; j < 2; ++j)
-                    w[i][j] = pack2<kBf16>(o[b][(g + i) * 4 + j * 2] * inverse, o[b][(g + i) * 4 + j * 2 + 1] * inverse);
-            const auto x = __builtin_amdgcn_permlane32_swap(w[0][0], w[1][0], false, false);
-            const auto y = __builtin_amdgcn_permlane32_swap(w[0][1], w[1][1], false, false);
-            const int d = b * 32 + (g + half) * 8;
+                    h[i][j] = pack2<kBf16>(o[b][(g + i) * 4 + j * 2] * inverse, o[b][(g + i) * 4 + j * 2 + 1] * inverse);
+            const auto x = __builtin_amdgcn_permlane32_swap(h[0][0], h[1][0], false, false);
+            const auto y = __builtin_amdgcn_permlane32_swap(h[0][1], h[1][1], false, false);
+            const int d = b * 32 + (g + out_half) * 8;
             __builtin_amdgcn_raw_buffer_store_b128(u32x4{x[0], y[0], x[1], y[1]}, ob,
-                                                   d < p.dim ? static_cast<uint32_t>(l32 * out_row) + d * 2 : kPastEnd, 0, 0);
+                                                   d < p.dim ? static_cast<uint32_t>(out_l32 * out_row) + d * 2 : kPastEnd, 0, 0);
         }
 }
 
 template <int kDim, bool kBf16, int kMask>
-int launch_attention_tiles(const AttnArgs& p, hipStream_t stream) {
-    using T = AttnTile<kDim>;
-    const int64_t slots = p.q_offsets ? p.sq / T::kRows + p.batch + 2
-                                      : static_cast<int64_t>(p.batch) * ((p.sq + T::kRows - 1) / T::kRows);
-    const int64_t per_xcd = (slots * p.heads + kNumXcd - 1) / kNumXcd;
-    if (slots > 0x7fffffff || per_xcd * kNumXcd * 256 > 0xffffffffll) return FEATHER_ERR_UNSUPPORTED;
+int launch_attention_tiles(const AttnArgs& p, const AttnPlan& plan, hipStream_t stream) {
+    const int64_t per_xcd = (plan.slots * p.heads + kNumXcd - 1) / kNumXcd;
+    if (plan.slots > 0x7fffffff || per_xcd * kNumXcd * 256 > 0xffffffffll) return FEATHER_ERR_UNSUPPORTED;
     auto* kernel = attention_tile_kernel<kDim, kBf16, kMask>;
-    kernel<<<dim3(static_cast<uint32_t>(per_xcd * kNumXcd)), 256, T::kLds, stream>>>(p, static_cast<int>(slots), per_xcd);
+    kernel<<<dim3(static_cast<uint32_t>(per_xcd * kNumXcd)), 256, 0, stream>>>(p, static_cast<int>(plan.slots), per_xcd);
     return hipGetLastError() == hipSuccess ? FEATHER_OK : FEATHER_ERR_LAUNCH;
-}
-
-template <int kDim, bool kBf16>
-int attention_tiles_mask(const AttnArgs& p, hipStream_t stream) {
-    switch (p.mask_type) {
-        case kMaskNone: return launch_attention_tiles<kDim, kBf16, kMaskNone>(p, stream);
-        case kMaskBool: return launch_attention_tiles<kDim, kBf16, kMaskBool>(p, stream);
-        case kMaskHalf: return launch_attention_tiles<kDim, kBf16, kMaskHalf>(p, stream);
-        default: return launch_attention_tiles<kDim, kBf16, kMaskF32>(p, stream);
-    }
-}
-
-template <bool kBf16>
-int attention_tiles(const AttnArgs& p, hipStream_t stream) {
-    if (p.dim <= 64) return attention_tiles_mask<64, kBf16>(p, stream);
-    if (p.dim <= 96) return attention_tiles_mask<96, kBf16>(p, stream);
-    if (p.dim <= 128) return attention_tiles_mask<128, kBf16>(p, stream);
-    return attention_tiles_mask<256, kBf16>(p, stream);
 }
 
 }  // namespace feather

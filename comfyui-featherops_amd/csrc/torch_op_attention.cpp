@@ -17,6 +17,7 @@
 #include <tuple>
 
 #include "featherops_amd.h"
+#include "torch_workspace.h"
 
 namespace {
 
@@ -308,7 +309,11 @@ at::Tensor run_attention(const at::Tensor& q, const at::Tensor& k, const at::Ten
     a.dtype = q.scalar_type() == at::kHalf ? FEATHER_DTYPE_F16 : FEATHER_DTYPE_BF16;
     a.causal = causal;
     a.scale = static_cast<float>(scale.has_value() ? *scale : 1.0 / std::sqrt(static_cast<double>(a.head_dim)));
-    check_status(feather_attention(&a, stream_of(q)), what);
+    const hipStream_t stream = stream_of(q);
+    const size_t bytes = feather_attention_workspace_size(&a);
+    at::Tensor ws;
+    if (bytes) ws = feather::workspace_for(q.device(), stream, bytes);
+    check_status(feather_attention(&a, bytes ? ws.data_ptr() : nullptr, bytes ? static_cast<size_t>(ws.numel()) : 0, stream), what);
     return out;
 }
 

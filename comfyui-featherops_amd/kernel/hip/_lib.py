@@ -76,7 +76,9 @@ SIGNATURES: dict[str, tuple] = {
     "feather_block_norm": (_int, [_vp, _vp]),
     "feather_rope_table": (_int, [_vp, _int, _i64, ctypes.POINTER(_int), _int, ctypes.c_double, _int, _vp, _vp]),
     "feather_qk_norm_rope": (_int, [_vp, _vp]),
-    "feather_attention": (_int, [_vp, _vp]),
+    "feather_attention": (_int, [_vp, _vp, ctypes.c_size_t, _vp]),
+    "feather_attention_workspace_size": (ctypes.c_size_t, [_vp]),
+    "feather_attention_plan": (_int, [_vp, ctypes.POINTER(_i64)]),
     "feather_status_string": (ctypes.c_char_p, [_int]),
     "feather_abi_version": (_int, []),
 }

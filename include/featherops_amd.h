@@ -482,7 +482,9 @@ int feather_qk_norm_rope(const feather_rope_args* args, hipStream_t stream);
  *   followed out of them. No mask, no k_lengths.
  * dtype F16 or BF16; head_dim a multiple of 8 up to 256; q, k, v, out at 16-byte
  * boundaries, strides multiples of 8, a token stride below 2^23; scale positive.
- * No counterpart in the reference.
+ * Workspace: the size below (0: none needed), the contract of feather_launch_scaled_mm_ws
+ * (its first 64 KB zero before the first use and left zero); with less, a query's keys are not shared
+ * among workgroups, and the sums run in another order. No counterpart in the reference.
  */
 typedef struct feather_attention_args {
     const void* q;
@@ -502,7 +504,12 @@ typedef struct feather_attention_args {
     int causal;
     float scale;
 } feather_attention_args;
-int feather_attention(const feather_attention_args* args, hipStream_t stream);
+size_t feather_attention_workspace_size(const feather_attention_args* args);
+/* What feather_attention launches with that workspace: plan[0] is 0 for blocks of 128 queries of a head, or the waves of a
+ * workgroup of the form for few rows (32 rows of a group of heads), plan[1] how many workgroups share a block's keys at most,
+ * plan[2] the number of blocks. Pointers are checked but not followed. */
+int feather_attention_plan(const feather_attention_args* args, int64_t* plan);
+int feather_attention(const feather_attention_args* args, void* workspace, size_t workspace_bytes, hipStream_t stream);
 
 /* Text for a status code. */
 const char* feather_status_string(int status);

@@ -99,10 +99,10 @@ def test_attention_entry_refuses(lib):
              dict(q_offsets=P), dict(k_offsets=P), dict(q_offsets=P, k_offsets=P, k_lengths=P),
              dict(q_offsets=P, k_offsets=P, mask=P), dict(q_offsets=P, k_offsets=P, batch=0)]
     for case in cases:
-        assert lib.feather_attention(ctypes.byref(AttentionArgs(**{**GOOD, **case})), None) == 1, case
-    assert lib.feather_attention(None, None) == 1
+        assert lib.feather_attention(ctypes.byref(AttentionArgs(**{**GOOD, **case})), None, 0, None) == 1, case
+    assert lib.feather_attention(None, None, 0, None) == 1
     for case in (dict(q_tokens=0), dict(batch=0)):
-        assert lib.feather_attention(ctypes.byref(AttentionArgs(**{**GOOD, **case, "q": None, "out": None})), None) == 0
+        assert lib.feather_attention(ctypes.byref(AttentionArgs(**{**GOOD, **case, "q": None, "out": None})), None, 0, None) == 0
 
 
 def meta(*shape, dtype=BF16):
