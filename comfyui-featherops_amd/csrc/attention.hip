@@ -3,9 +3,10 @@
 // Three forms: attention_tiles.h (128 queries of a head a workgroup), and attention_rows.h with 4 or 8 waves and the keys
 // of 32 rows shared by up to 64 workgroups. Each has a time, in microseconds, of a fixed part, a part for each
 // workgroup that a CU gets, and one for its tiles: by their latency one after the other where a CU has one workgroup,
-// by throughput where it has several. Fitted to 9,500 shapes (1 to 4 samples, 1 to 40 heads in groups of 1 to 8, 1 to
-// 16384 queries and keys, a third causal, two fifths with masks), each form and split timed on an MI355X: the form taken is 1.4%
-// slower than the fastest of all in the mean, 8% at the 95th percentile.
+// by throughput where it has several. Fitted to 30,000 shapes (1 to 4 samples, 1 to 40 heads in groups of 1 to 8, 1 to
+// 16384 queries and keys, a third causal, two fifths with masks), each form and split timed on an MI355X: the form taken is 1.3%
+// slower than the fastest of all in the mean, 8% at the 95th percentile. Most often fastest: few rows with 4 waves and unshared
+// keys (44% of the shapes), with 8 (16%), blocks of 128 queries (16%), shared keys (24%).
 #include "attention.h"
 
 #include <algorithm>
@@ -21,10 +22,10 @@ struct DimTimes {
     Times tiles, masked_tiles, rows[2];  // rows: of 4 and 8 waves (a wide head has no 8)
 };
 constexpr DimTimes kTimes[] = {
-    {64, {3.64, 1.78, 0.380, 0.304}, {3.80, 3.24, 0.644, 0.425}, {{3.56, 1.08, 0.802, 0.460}, {2.97, 1.86, 0.964, 0.845}}},
-    {96, {3.24, 2.71, 0.429, 0.390}, {2.86, 4.69, 0.715, 0.547}, {{3.45, 1.53, 0.952, 0.694}, {0.47, 4.46, 1.320, 1.320}}},
-    {128, {3.94, 2.76, 0.481, 0.481}, {2.80, 5.32, 0.746, 0.593}, {{2.81, 2.56, 1.083, 0.825}, {0.72, 5.11, 1.474, 1.474}}},
-    {256, {6.78, 3.29, 1.123, 1.123}, {8.46, 3.47, 1.388, 1.388}, {{0.83, 7.41, 1.840, 1.840}, {}}},
+    {64, {3.67, 1.74, 0.376, 0.304}, {4.23, 2.96, 0.667, 0.423}, {{3.48, 1.14, 0.807, 0.447}, {2.78, 2.05, 0.973, 0.804}}},
+    {96, {3.24, 2.74, 0.430, 0.381}, {2.92, 4.77, 0.736, 0.534}, {{3.32, 1.67, 0.955, 0.666}, {0.45, 4.53, 1.312, 1.312}}},
+    {128, {3.65, 2.97, 0.477, 0.477}, {2.70, 5.41, 0.801, 0.591}, {{2.73, 2.67, 1.082, 0.816}, {0.47, 5.34, 1.465, 1.465}}},
+    {256, {6.80, 2.77, 0.933, 0.933}, {7.72, 3.97, 1.374, 1.374}, {{0.54, 7.63, 1.821, 1.821}, {}}},
 };
 // joining the sums of several workgroups: a call, and each row of each of them (half of that with 8 waves)
 constexpr double kJoin = 3.8, kJoinRow = 0.00012;  // the latter times the head's dimension

@@ -221,7 +221,9 @@ struct AttnMaskRegs {
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
                     const int key = key0 + kb * 32 + (2 * j + static_cast<int>(threadIdx.x) % 64 / 32) * 8;
-                    load_mask8<kMask>(from + static_cast<int64_t>(key) * kMaskBytes<kMask>, keys - key, raw[kb][j]);
+                    const uint8_t* at = from + static_cast<int64_t>(key) * kMaskBytes<kMask>;
+                    if (key0 + kKeyBlocks * 32 <= keys) __builtin_memcpy(raw[kb][j], at, 8 * kMaskBytes<kMask>);
+                    else load_mask8<kMask>(at, keys - key, raw[kb][j]);
                 }
         }
     }

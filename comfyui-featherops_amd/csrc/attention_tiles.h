@@ -66,11 +66,16 @@ __device__ __forceinline__ void mfma_alone(f32x16& c, u32x4 a, u32x4 b) {
     }
 }
 #undef FEATHER_MFMA32
-// Until the scores are in their registers: reads of them stay behind.
-__device__ __forceinline__ void settle(f32x16& s) { asm volatile("s_nop 15\n\ts_nop 3" : "+v"(s)); }
+// Until an accumulator's values are in its registers: reads of them stay behind.
+template <bool kAccumulation = false>
+__device__ __forceinline__ void settle(f32x16& c) {
+    if constexpr (kAccumulation) asm volatile("s_nop 15\n\ts_nop 3" : "+a"(c));
+    else asm volatile("s_nop 15\n\ts_nop 3" : "+v"(c));
+}
 
 template <int kDim, bool kBf16, int kMask>
-__global__ __launch_bounds__(256, kDim > 128 ? 1 : kDim == 64 && kMask == kMaskNone ? 4 : 2) void attention_tile_kernel(const AttnArgs p, int slots, int64_t per_xcd) {
+__global__ __launch_bounds__(256, kDim > 128 ? 1 : kDim == 64 && kMask == kMaskNone ? 4 : 2) void attention_tile_kernel(
+    const AttnArgs p, int slots, int64_t per_xcd) {
     using T = AttnTile<kDim, kMask>;
     using Mask = AttnMaskRegs<kBf16, kMask, 1>;
     constexpr int kSteps = kDim / 16, kBlocks = kDim / 32, kRowBytes = kDim * 2;
@@ -91,8 +96,9 @@ __global__ __launch_bounds__(256, kDim > 128 ? 1 : kDim == 64 && kMask == kMaskN
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
     const int l32 = lane % 32, half = lane / 32;
     const int row0 = job.row0 + wave * 32;
-    // keys [0, limit) are this lane's query's; the wave's queries see wave_keys at most and wave_least at least
-    const int shift = job.keys - job.rows;  // the last query sees all keys
+    // The last query sees all keys. Keys [0, limit) are this lane's query's, and the wave's queries see wave_keys at most and
+    // wave_least at least.
+    const int shift = job.keys - job.rows;
     const int limit = p.causal ? min(job.keys, row0 + l32 + shift + 1) : job.keys;
     const int wave_keys = row0 >= job.rows ? 0 : p.causal ? min(job.keys, row0 + 32 + shift) : job.keys;
     const int wave_least = p.causal ? min(job.keys, row0 + shift + 1) : job.keys;
@@ -122,8 +128,9 @@ __global__ __launch_bounds__(256, kDim > 128 ? 1 : kDim == 64 && kMask == kMaskN
     // What is copied before turn u: keys up to u + kRing, in the place of those that turn u - 1 has read last, and values up
     // to u + kRing - 2 likewise.
     const int ahead = copies_keys ? T::kRing : T::kRing - 2;
-    // Before turn u, the first one too (unit 0's keys have been read by then): what it and the kBatch - 1 behind it read of this wave's copies has landed (one turn at a time: all but
-    // the last unit's), and its reads of what is copied over next are done; then everyone's.
+    // Before turn u, the first one too (unit 0's keys have been read by then): what it and the kBatch - 1 behind it read of
+    // this wave's copies has landed (one turn at a time: all but the last unit's), and its reads of what is copied over
+    // next are done; then everyone's.
     auto wait_batch = [&] {
         asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(T::kBatch == 1 ? T::kCopies : 0) : "memory");
     };
@@ -177,12 +184,6 @@ __global__ __launch_bounds__(256, kDim > 128 ? 1 : kDim == 64 && kMask == kMaskN
 #pragma unroll
         for (int i = 0; i < 2; ++i) m[i].load(mask_row, (u + i) * 32, job.keys);
     };
-    // Adds a unit's values at `at` with its weights; the results are in their registers behind it.
-    auto add_unit = [&](const u32x4 (&pf)[2], uint32_t at) {
-#pragma unroll
-        for (int n = 0; n < kSteps; ++n) mfma_alone<kBf16, T::kAccumulation>(o[n % kBlocks], read_v(n, at), pf[n / kBlocks]);
-    };
-
     // Unit u: its weights from its scores `now`; beside that the products that give the scores of the unit ahead, whose keys
     // are at ka, and that add the unit before with its weights `old` and values at va. The keys of the unit after
     // that are at kn. high: the scores' maximum, of `now` on the way in, of `next` on the way out.
@@ -191,20 +192,28 @@ __global__ __launch_bounds__(256, kDim > 128 ? 1 : kDim == 64 && kMask == kMaskN
     auto turn = [&](int u, f32x16 (&now)[1], f32x16 (&next)[1], u32x4 (&pf)[2], u32x4 (&old)[2], uint32_t ka, uint32_t va, uint32_t kn, Mask& its_mask,
                     bool first, bool last) {
         // (whether the turn begins a batch, with copies and after a barrier before which nothing is read ahead; whether it ends one)
-        // A maximum that has fallen behind is replaced. The unit before, whose weights are relative to it, is added now; its
-        // turn for it finds none.
-        if (__any((high - top) * factor > kMaxLag)) {
-            add_unit(old, va);
-            const float to = fmaxf(top, high);
-            const float alpha = __builtin_amdgcn_exp2f((top - to) * factor);
-            top = to;
-            by = kBias - to * factor;
+        // A maximum that has fallen behind is raised, by a power of two of the weights: that leaves the rounded ones of the unit
+        // before, which are still to be added, as exact as they were. (A row that had seen nothing starts anew.)
+        const float behind = (high - top) * factor;
+        if (__any(behind > kMaxLag)) {
+            const float steps = behind > 0.0f ? ceilf(behind) : 0.0f;
+            const bool anew = steps > 512.0f;
+            const float alpha = anew ? 0.0f : __builtin_amdgcn_ldexpf(1.0f, -static_cast<int>(steps));
+            top = anew ? high : top + steps / factor;
+            by = kBias - top * factor;
             total *= alpha;
 #pragma unroll
-            for (int b = 0; b < kBlocks; ++b)
+            for (int b = 0; b < kBlocks; ++b) {
+                settle<T::kAccumulation>(o[b]);
 #pragma unroll
                 for (int e = 0; e < 16; ++e) o[b][e] *= alpha;
-            old[0] = old[1] = u32x4{};
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const uint32_t w = old[i / 4][i % 4];
+                old[i / 4][i % 4] = pack2<kBf16>(out_bits_to_f32<kBf16>(static_cast<uint16_t>(w)) * alpha,
+                                                 out_bits_to_f32<kBf16>(static_cast<uint16_t>(w >> 16)) * alpha);
+            }
         }
         // Two scores to weights, in two steps a product apart; the first product has the copies beside it.
         float w[2];
@@ -266,12 +275,14 @@ __global__ __launch_bounds__(256, kDim > 128 ? 1 : kDim == 64 && kMask == kMaskN
         high = max_halves(high);
     };
 
+    // Unit 0 has none before it: weights of zero, and values of zero in the place that is copied to last.
+    for (int i = threadIdx.x; i < T::kUnitBytes / 16; i += 256)
+        reinterpret_cast<u32x4*>(rings + (2 * T::kRing - 1) * T::kUnitBytes)[i] = u32x4{};
     // Units 0 to 2 of the keys and 0 of the values have landed.
     Mask mask0;
     mask0.load(mask_row, 0, job.keys);
     load_masks(mask[0], 1);
-    wait_vmcnt<T::kBatch == 1 ? T::kCopies : 0>();
-    asm volatile("s_barrier" ::: "memory");
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(T::kBatch == 1 ? T::kCopies : 0) : "memory");
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
         if (s == 0) mfma_first<kBf16>(s0[0], read_k(0, 0), qf[0]);
@@ -307,13 +318,15 @@ __global__ __launch_bounds__(256, kDim > 128 ? 1 : kDim == 64 && kMask == kMaskN
                 }
             }
             const uint32_t ka = (j + 1) % T::kRing * kUnit, kn = (j + 2) % T::kRing * kUnit;
-            // (unit 0 has none before it: weights of zero, on values that are there)
-            const uint32_t va = j ? (j - 1) * kUnit : u0 ? (T::kRing - 1) * kUnit : 0;
+            const uint32_t va = (j + T::kRing - 1) % T::kRing * kUnit;
             if (j % 2 == 0) turn(u, s0, s1, p0, p1, ka, va, kn, mask[set][0], first, last);
             else turn(u, s1, s0, p1, p0, ka, va, kn, mask[set][1], first, last);
         }
     }
-    add_unit(p1, (units - 1) % T::kRing * kUnit);
+    // the last unit's values; the results are in their registers behind it
+#pragma unroll
+    for (int n = 0; n < kSteps; ++n)
+        mfma_alone<kBf16, T::kAccumulation>(o[n % kBlocks], read_v(n, (units - 1) % T::kRing * kUnit), p1[n / kBlocks]);
     for (int u = units; u < all_units; u += T::kBatch) {
         wait_batch();
         copy_batch(u);
