@@ -35,6 +35,8 @@ int attention_args(const feather_attention_args* a, AttnArgs& p, bool& empty) {
         (a->dtype != FEATHER_DTYPE_F16 && a->dtype != FEATHER_DTYPE_BF16) || !(a->scale > 0.0f) || !std::isfinite(a->scale) ||
         (a->causal != 0 && a->causal != 1))
         return FEATHER_ERR_INVALID;
+    // rows of a group of heads are counted in 32 bits
+    if (a->q_tokens * (a->heads / a->kv_heads) > kMaxTokens) return FEATHER_ERR_INVALID;
     const bool packed = a->q_offsets || a->k_offsets;
     if (packed && (!a->q_offsets || !a->k_offsets || a->k_lengths || a->mask || a->batch < 1)) return FEATHER_ERR_INVALID;
     if (a->mask && a->mask_dtype != FEATHER_DTYPE_BOOL && a->mask_dtype != FEATHER_DTYPE_F32 && a->mask_dtype != a->dtype)

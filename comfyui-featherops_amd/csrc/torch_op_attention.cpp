@@ -219,6 +219,9 @@ void check_qkv(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, in
     TORCH_CHECK(k.sym_size(-1) == dim && v.sym_sizes() == k.sym_sizes(), "k and v must have one shape, and q's head_dim");
     TORCH_CHECK(heads >= 1 && heads <= 65536 && shared >= 1 && heads % shared == 0, "q's heads (", heads,
                 ") must be a multiple of k's (", shared, ")");
+    const int64_t most = int64_t(1) << 30;
+    TORCH_CHECK(q.sym_size(-3) <= most && k.sym_size(-3) <= most && q.sym_size(-3) * (heads / shared) <= most,
+                "q and k may have up to 2^30 tokens, q's times the heads that share a key head too");
 }
 
 double check_scale(const at::Tensor& q, std::optional<double> scale) {

@@ -1,5 +1,7 @@
 """Inputs and the error bound of the attention tests."""
 
+import ctypes
+
 import numpy as np
 import torch
 
@@ -39,3 +41,46 @@ def check(got, want, mags, reach, keys, label="", added=0.0):
     worst = float((off / tol).max()) if off.size else 0.0
     assert worst <= 1.0, f"{label}: {worst:.3g} times the bound"
     return worst
+
+
+class AttentionArgs(ctypes.Structure):
+    """feather_attention_args of include/featherops_amd.h."""
+
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("q", "k", "v", "out", "mask", "q_offsets", "k_offsets", "k_lengths")]
+                + [(n, ctypes.c_int64) for n in ("batch", "q_tokens", "k_tokens", "heads", "kv_heads", "head_dim",
+                                                 "q_batch_stride", "q_token_stride", "q_head_stride", "k_batch_stride",
+                                                 "k_token_stride", "k_head_stride", "v_batch_stride", "v_token_stride",
+                                                 "v_head_stride", "mask_batch_stride", "mask_head_stride", "mask_query_stride")]
+                + [(n, ctypes.c_int) for n in ("dtype", "mask_dtype", "causal")] + [("scale", ctypes.c_float)])
+
+
+def attention_args(B, Sq, Sk, H, Hk, D, **kw):
+    """Of contiguous bf16 tensors; the pointers stand for some until they are set."""
+    P = 4096
+    a = AttentionArgs(q=P, k=P, v=P, out=P, batch=B, q_tokens=Sq, k_tokens=Sk, heads=H, kv_heads=Hk, head_dim=D, dtype=1, mask_dtype=1,
+                      q_batch_stride=Sq * H * D, q_token_stride=H * D, q_head_stride=D, k_batch_stride=Sk * Hk * D,
+                      k_token_stride=Hk * D, k_head_stride=D, v_batch_stride=Sk * Hk * D, v_token_stride=Hk * D, v_head_stride=D,
+                      scale=0.1)
+    for name, value in kw.items():
+        setattr(a, name, value)
+    return a
+
+
+def plan_of(lib, args):
+    """(waves, splits, blocks), see feather_attention_plan."""
+    plan = (ctypes.c_int64 * 3)()
+    assert lib.feather_attention_plan(ctypes.byref(args), plan) == 0
+    return tuple(plan)
+
+
+# Shapes that each form takes where there is no mask, and some with one: ((waves, whether workgroups share a block's keys), (batch, q tokens, k tokens,
+# heads, kv heads, head_dim)). test_attention_host.py checks that they do.
+FORMS = [((0, False), (3, 1101, 140, 16, 2, 64)), ((0, False), (2, 777, 1300, 24, 8, 64)), ((0, False), (3, 1101, 157, 16, 16, 40)),
+         ((4, False), (3, 7, 77, 16, 2, 64)), ((4, True), (2, 1, 2111, 8, 2, 64)), ((8, False), (2, 142, 300, 8, 2, 64)),
+         ((8, True), (1, 33, 9011, 8, 8, 56)), ((0, False), (3, 1101, 140, 16, 2, 96)), ((0, False), (2, 777, 1300, 24, 8, 88)),
+         ((4, False), (3, 35, 77, 16, 2, 96)), ((4, True), (1, 1100, 5003, 8, 8, 96)), ((8, False), (1, 77, 301, 24, 24, 72)),
+         ((8, True), (2, 7, 9001, 8, 2, 96)), ((0, False), (3, 1101, 140, 16, 2, 128)), ((0, False), (2, 777, 1300, 24, 8, 128)),
+         ((0, False), (1, 1500, 459, 21, 7, 104)), ((4, False), (3, 7, 300, 15, 3, 128)), ((4, True), (1, 2, 1100, 24, 24, 128)),
+         ((8, False), (1, 77, 513, 24, 24, 128)), ((8, True), (2, 33, 5001, 5, 5, 120)), ((0, False), (3, 1101, 140, 16, 2, 256)),
+         ((0, False), (2, 777, 1300, 24, 8, 136)), ((4, False), (3, 35, 140, 16, 2, 256)), ((4, True), (2, 7, 9001, 8, 2, 256)),
+         ((4, True), (1, 65, 1100, 24, 24, 200))]

@@ -9,6 +9,7 @@ import numpy as np
 import pytest
 import torch
 
+from attention_util import AttentionArgs, attention_args, plan_of
 from oracle import attention_oracle as A
 
 BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
@@ -38,17 +39,6 @@ class RopeArgs(ctypes.Structure):
                                                  "q_token_stride", "q_head_stride", "k_batch_stride", "k_token_stride",
                                                  "k_head_stride", "table_batch_stride")]
                 + [(n, ctypes.c_int) for n in ("dtype", "weight_dtype", "norm", "pairs_of_halves")] + [("eps", ctypes.c_float)])
-
-
-class AttentionArgs(ctypes.Structure):
-    """feather_attention_args of include/featherops_amd.h."""
-
-    _fields_ = ([(n, ctypes.c_void_p) for n in ("q", "k", "v", "out", "mask", "q_offsets", "k_offsets", "k_lengths")]
-                + [(n, ctypes.c_int64) for n in ("batch", "q_tokens", "k_tokens", "heads", "kv_heads", "head_dim",
-                                                 "q_batch_stride", "q_token_stride", "q_head_stride", "k_batch_stride",
-                                                 "k_token_stride", "k_head_stride", "v_batch_stride", "v_token_stride",
-                                                 "v_head_stride", "mask_batch_stride", "mask_head_stride", "mask_query_stride")]
-                + [(n, ctypes.c_int) for n in ("dtype", "mask_dtype", "causal")] + [("scale", ctypes.c_float)])
 
 
 P = 4096  # stands for a pointer: every call below ends at a check before it is used
@@ -91,6 +81,7 @@ GOOD = dict(q=P, k=P, v=P, out=P, batch=2, q_tokens=5, k_tokens=7, heads=8, kv_h
 def test_attention_entry_refuses(lib):
     cases = [dict(q=None), dict(k=None), dict(v=None), dict(out=None), dict(q=P + 8), dict(k=P + 2), dict(v=P + 4), dict(out=P + 8),
              dict(batch=-1), dict(batch=65537), dict(q_tokens=-1), dict(k_tokens=-1), dict(q_tokens=1 << 31), dict(k_tokens=1 << 31),
+             dict(q_tokens=(1 << 28) + 1),  # times 4 heads of a group
              dict(heads=0), dict(kv_heads=0), dict(kv_heads=3), dict(kv_heads=16), dict(heads=1 << 17), dict(head_dim=0),
              dict(head_dim=100), dict(head_dim=264), dict(dtype=2), dict(dtype=4), dict(scale=0.0), dict(scale=-1.0),
              dict(scale=float("inf")), dict(scale=float("nan")), dict(causal=2), dict(q_token_stride=1028), dict(k_head_stride=4),
@@ -160,7 +151,8 @@ REFUSED = [
     (dict(scale=1e-60), "positive"), (dict(scale=float("nan")), "positive"), (dict(k_lengths=meta(2, dtype=torch.int64)), "int32"),
     (dict(k_lengths=meta(3, dtype=I32)), "int32"), (dict(mask=meta(5, 7, dtype=F16)), "mask must be bool"),
     (dict(mask=meta(5, 7, dtype=torch.uint8)), "mask must be bool"), (dict(mask=meta(5, 8)), "broadcast"),
-    (dict(mask=meta(2, 3, 5, 7)), "broadcast"), (dict(mask=meta(1, 2, 8, 5, 7)), "broadcast"), (dict(mask=meta()), "broadcast")]
+    (dict(mask=meta(2, 3, 5, 7)), "broadcast"), (dict(mask=meta(1, 2, 8, 5, 7)), "broadcast"), (dict(mask=meta()), "broadcast"),
+    (dict(q=meta(2, (1 << 28) + 1, 8, 64)), "2\\^30"), (dict(k=meta(2, (1 << 30) + 1, 2, 64), v=meta(2, (1 << 30) + 1, 2, 64)), "2\\^30")]
 
 
 @pytest.mark.parametrize("change,message", REFUSED)
@@ -228,3 +220,33 @@ def test_oracle_is_the_definition():
     assert np.allclose(o[1], v[0]) and (mags >= np.abs(o) - 1e-12).all()
     w = np.exp(q[3, 1] @ k[:, 0].T / np.sqrt(8))
     assert np.allclose(o[3, 1], w @ v[:, 0] / w.sum())
+
+
+def test_plans(lib):
+    """Every form has shapes that take it, with and without a mask; keys are shared only as far as there are counters, and
+    the workspace holds what is written."""
+    from attention_util import FORMS
+
+    wide = lambda D: next(w for w in (64, 96, 128, 256) if D <= w)  # noqa: E731
+    every = {((w, s), D) for D in (64, 96, 128, 256) for w, s in ((0, False), (4, False), (4, True), (8, False), (8, True))
+             if D < 256 or w < 8}
+    for mask in (None, P):
+        got = [(*plan_of(lib, attention_args(*shape, mask=mask))[:2], form, shape) for form, shape in FORMS]
+        assert {((waves, splits > 1), wide(shape[5])) for waves, splits, _, shape in got} == every
+        assert mask or all((waves, splits > 1) == form for waves, splits, form, _ in got), got
+    rng = np.random.default_rng(1)
+    for _ in range(4000):
+        B, Hk, G, D = (int(rng.choice(c)) for c in ((1, 2, 7, 64, 4000), (1, 2, 5, 8, 40), (1, 2, 8), (8, 64, 96, 104, 128, 256)))
+        Sq, Sk = (int(2 ** rng.uniform(0, 17)) for _ in range(2))
+        args = attention_args(B, Sq, Sk, Hk * G, Hk, D, causal=int(rng.integers(2)), mask=None if rng.integers(2) else P)
+        if rng.integers(2):
+            args.mask, args.q_offsets, args.k_offsets = None, P, P
+        waves, splits, blocks = plan_of(lib, args)
+        size = lib.feather_attention_workspace_size(ctypes.byref(args))
+        assert waves in (0, 4, 8) and 1 <= splits <= 64 and blocks >= 1
+        if splits == 1:
+            assert size == 0
+        else:
+            assert waves and blocks <= 16384 and size == 65536 + blocks * splits * 32 * (wide(D) + 4) * 4
+        if args.q_offsets is None:
+            assert blocks == (B * Hk * -(-Sq * G // 32) if waves else B * Hk * G * -(-Sq // 128))
