@@ -9,6 +9,21 @@ namespace feather {
 constexpr int kAttnMaxDim = 256;      // widest head
 constexpr int kAttnMaxBatch = 65536;  // samples or packed sequences
 
+// n / d for 0 <= n < 2^31, d > 0: with 2^shift >= d > 2^(shift - 1) and multiplier = ceil(2^(31 + shift) / d), 2 n * multiplier /
+// 2^(32 + shift) is above n / d by less than n / 2^31 / d. (Five divisions by sizes took a workgroup 0.4 us before its
+// first load.)
+struct AttnDivisor {
+    uint32_t multiplier, shift;
+    static AttnDivisor of(int64_t d) {
+        uint32_t shift = 0;
+        while ((int64_t(1) << shift) < d) ++shift;
+        return {static_cast<uint32_t>(((uint64_t(1) << (31 + shift)) + d - 1) / d), shift};
+    }
+    __device__ __forceinline__ int operator()(int n) const {
+        return static_cast<int>(__umulhi(static_cast<uint32_t>(n) << 1, multiplier) >> shift);
+    }
+};
+
 enum AttnMask { kMaskNone = 0, kMaskBool = 1, kMaskHalf = 2, kMaskF32 = 3 };
 
 struct AttnArgs {
@@ -28,6 +43,9 @@ struct AttnArgs {
     int sq, sk;  // tokens of a sample; packed: all tokens
     int mask_type, causal, bf16;
     float scale;
+    // set at the launch: blocks of all samples, of one sample, heads that share a key head, workgroups that share keys, and
+    // what a store takes of a head (rows)
+    AttnDivisor by_slots, by_blocks, by_group, by_splits, by_quads;
 };
 
 // Which kernel takes a call, and how.

@@ -33,7 +33,7 @@ template <int kRows>
 __device__ __forceinline__ bool attn_job(const AttnArgs& p, int slot, int per_token, AttnJob& job) {
     if (!p.q_offsets) {
         const int blocks = (p.sq * per_token + kRows - 1) / kRows;
-        job.b = slot / blocks;
+        job.b = p.by_blocks(slot);
         if (job.b >= p.batch) return false;
         job.row0 = (slot - job.b * blocks) * kRows;
         job.q_start = job.k_start = 0;
@@ -185,45 +185,48 @@ constexpr float kMaxLag = 8.0f;
 
 // ---- a wave's 32 queries ----
 
-// Eight mask values of consecutive keys as they lie in memory, of which the first n exist (the rest reads as zeros).
 template <int kMask>
 constexpr int kMaskBytes = kMask == kMaskBool ? 1 : kMask == kMaskHalf ? 2 : 4;
-template <int kMask>
-__device__ __forceinline__ void load_mask8(const uint8_t* p, int n, uint32_t (&w)[2 * kMaskBytes<kMask>]) {
-    if (n >= 8) {
-        __builtin_memcpy(w, p, 8 * kMaskBytes<kMask>);
-        return;
-    }
-#pragma unroll
-    for (int i = 0; i < 2 * kMaskBytes<kMask>; ++i) w[i] = 0;
-#pragma unroll
-    for (int j = 0; j < 7; ++j) {
-        if (j >= n) continue;
-        if constexpr (kMask == kMaskBool) w[j / 4] |= static_cast<uint32_t>(p[j]) << (8 * (j % 4));
-        else if constexpr (kMask == kMaskHalf) w[j / 2] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(p)[j]) << (16 * (j % 2));
-        else w[j] = reinterpret_cast<const uint32_t*>(p)[j];
-    }
-}
 
 // The mask's values for a wave's 32 queries and a tile's keys: lanes l and l + 32 load eight keys of the same query, l
-// those of group 2 j, l + 32 of 2 j + 1.
+// those of group 2 j, l + 32 of 2 j + 1. 16-bit values are loaded as the words that they lie in, and shifted into place when
+// they are used: with 16-byte loads at addresses that are no multiples of 4, 2 x 1003 x 1003 x 16 heads of 64 took 35 us for 27, so
+// 31 (8 bytes of a bool mask at any address cost less than this does).
 template <bool kBf16, int kMask, int kKeyBlocks>
 struct AttnMaskRegs {
     // values that are added to the scores: the scale comes before them
     static constexpr bool kAdds = kMask == kMaskHalf || kMask == kMaskF32;
-    uint32_t raw[kKeyBlocks][2][kMask ? 2 * kMaskBytes<kMask> : 1];
+    static constexpr int kWords = 2 * kMaskBytes<kMask>;                 // of eight values
+    static constexpr bool kShifts = kMask == kMaskHalf;
+    static constexpr int kLoaded = kShifts ? kWords + 1 : kWords;  // that they lie in
+    uint32_t raw[kKeyBlocks][2][kLoaded];
 
-    // those of the tile whose first key is key0, from the query's row; it has `keys` of them
+    // those of the tile whose first key is key0, from the query's row; it has `keys` of them (what lies behind them is not read)
     __device__ __forceinline__ void load(const uint8_t* from, int key0, int keys) {
         if constexpr (kMask != kMaskNone) {
+            const int skipped = kShifts ? static_cast<int>(reinterpret_cast<uintptr_t>(from) % 4) : 0;
+            const bool any = kShifts && __any(skipped);
 #pragma unroll
             for (int kb = 0; kb < kKeyBlocks; ++kb)
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
                     const int key = key0 + kb * 32 + (2 * j + static_cast<int>(threadIdx.x) % 64 / 32) * 8;
-                    const uint8_t* at = from + static_cast<int64_t>(key) * kMaskBytes<kMask>;
-                    if (key0 + kKeyBlocks * 32 <= keys) __builtin_memcpy(raw[kb][j], at, 8 * kMaskBytes<kMask>);
-                    else load_mask8<kMask>(at, keys - key, raw[kb][j]);
+                    const uint8_t* at = from - skipped + static_cast<int64_t>(key) * kMaskBytes<kMask>;
+                    uint32_t(&w)[kLoaded] = raw[kb][j];
+                    if (key0 + kKeyBlocks * 32 <= keys) {
+                        __builtin_memcpy(w, kMask == kMaskBool ? at : __builtin_assume_aligned(at, 4), kWords * 4);
+                        if (any) w[kLoaded - 1] = reinterpret_cast<const uint32_t*>(at)[skipped ? kLoaded - 1 : kWords - 1];
+                    } else if constexpr (kMask == kMaskBool) {
+#pragma unroll
+                        for (int i = 0; i < kWords; ++i) w[i] = 0;
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            if (key + i < keys) w[i / 4] |= static_cast<uint32_t>(at[i]) << (8 * (i % 4));
+                    } else {
+                        const int bytes = skipped + (keys - key) * kMaskBytes<kMask>;
+#pragma unroll
+                        for (int i = 0; i < kLoaded; ++i) w[i] = key < keys && i * 4 < bytes ? reinterpret_cast<const uint32_t*>(at)[i] : 0;
+                    }
                 }
         }
     }
@@ -235,21 +238,28 @@ struct AttnMaskRegs {
 #pragma unroll
                 for (int j = 0; j < 2; ++j)
 #pragma unroll
-                    for (int i = 0; i < 2 * kMaskBytes<kMask>; ++i) asm volatile("" : "+v"(raw[kb][j][i]));
+                    for (int i = 0; i < kLoaded; ++i) asm volatile("" : "+v"(raw[kb][j][i]));
         }
     }
-    __device__ __forceinline__ void put(f32x16 (&s)[kKeyBlocks], float scale) {
+    __device__ __forceinline__ void put(f32x16 (&s)[kKeyBlocks], float scale, const uint8_t* from) {
         if constexpr (kMask != kMaskNone) {
-            constexpr int kWords = kMaskBytes<kMask>;  // of four keys
+            constexpr int kHalf = kWords / 2;  // words of four keys
+            const uint32_t skipped = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(from)) % 4 * 8;  // bits
 #pragma unroll
             for (int kb = 0; kb < kKeyBlocks; ++kb)
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    // lanes 32 apart trade four keys, so that each has four of both groups
-                    uint32_t w[2][kWords];
+                    uint32_t own[kWords];
 #pragma unroll
                     for (int i = 0; i < kWords; ++i) {
-                        const auto x = __builtin_amdgcn_permlane32_swap(raw[kb][j][i], raw[kb][j][kWords + i], false, false);
+                        if constexpr (kShifts) own[i] = __builtin_amdgcn_alignbit(raw[kb][j][i + 1], raw[kb][j][i], skipped);
+                        else own[i] = raw[kb][j][i];
+                    }
+                    // lanes 32 apart trade four keys, so that each has four of both groups
+                    uint32_t w[2][kHalf];
+#pragma unroll
+                    for (int i = 0; i < kHalf; ++i) {
+                        const auto x = __builtin_amdgcn_permlane32_swap(own[i], own[kHalf + i], false, false);
                         w[0][i] = x[0];
                         w[1][i] = x[1];
                     }
@@ -349,7 +359,7 @@ struct AttnWave {
 
     // The mask's values on the scores, and -inf for keys from `limit` on where some of the tile's are (`cut`).
     __device__ __forceinline__ void masked(f32x16 (&s)[kKeyBlocks], int key0, int limit, bool cut) {
-        mask.put(s, scale);
+        mask.put(s, scale, mask_row);
         if (cut) attn_cut<kKeyBlocks>(s, key0, limit);
     }
 

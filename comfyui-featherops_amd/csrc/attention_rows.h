@@ -22,9 +22,8 @@ struct AttnRows {
 };
 
 template <int kDim, bool kBf16, int kMask, int kWaves>
-__global__ __launch_bounds__(64 * kWaves, kDim <= 128 ? 2 : 1) void attention_rows_kernel(const AttnArgs p, int slots, int64_t total,
-                                                                                      int splits, int least, uint32_t* counters,
-                                                                                      float* partials) {
+__global__ __launch_bounds__(64 * kWaves, kDim <= 128 ? 2 : 1) void attention_rows_kernel(const AttnArgs p, int slots, int total, int splits,
+                                                                                      int least, uint32_t* counters, float* partials) {
     using T = AttnRows<kDim>;
     using Wave = AttnWave<kDim, kBf16, kMask, 1>;
     constexpr int kThreads = 64 * kWaves;
@@ -32,11 +31,11 @@ __global__ __launch_bounds__(64 * kWaves, kDim <= 128 ? 2 : 1) void attention_ro
     __shared__ float tops[kWaves][32], totals[kWaves][32];
 
     // workgroup i runs on XCD i % 8: an XCD takes the row blocks that share keys
-    const int64_t per_xcd = (total + kNumXcd - 1) / kNumXcd;
-    const int64_t id = static_cast<int64_t>(blockIdx.x % kNumXcd) * per_xcd + blockIdx.x / kNumXcd;
-    if (blockIdx.x / kNumXcd >= per_xcd || id >= total) return;
-    const int slot = static_cast<int>(id % slots), rest = static_cast<int>(id / slots);
-    const int split = rest % splits, kv_head = rest / splits;
+    const int per_xcd = static_cast<int>(gridDim.x / kNumXcd);
+    const int id = static_cast<int>(blockIdx.x % kNumXcd) * per_xcd + static_cast<int>(blockIdx.x / kNumXcd);
+    if (id >= total) return;
+    const int rest = p.by_slots(id), slot = id - rest * slots;
+    const int kv_head = p.by_splits(rest), split = rest - kv_head * splits;
     AttnJob job;
     if (!attn_job<32>(p, slot, p.group, job)) return;
 
@@ -44,14 +43,14 @@ __global__ __launch_bounds__(64 * kWaves, kDim <= 128 ? 2 : 1) void attention_ro
     const int l32 = lane % 32, half = lane / 32;
     const int rows = min(32, job.rows - job.row0);
     // this lane's query, and the keys [0, limit) that it sees
-    const int row = job.row0 + min(l32, rows - 1), token = row / p.group, head = kv_head * p.group + row - token * p.group;
-    const int shift = job.keys - job.rows / p.group;
+    const int row = job.row0 + min(l32, rows - 1), token = p.by_group(row), head = kv_head * p.group + row - token * p.group;
+    const int shift = job.keys - p.by_group(job.rows);
     const int limit = p.causal ? min(job.keys, token + shift + 1) : job.keys;
-    const int seen = p.causal ? max(0, min(job.keys, (job.row0 + rows - 1) / p.group + shift + 1)) : job.keys;
-    const int every = p.causal ? min(job.keys, job.row0 / p.group + shift + 1) : job.keys;
+    const int seen = p.causal ? max(0, min(job.keys, p.by_group(job.row0 + rows - 1) + shift + 1)) : job.keys;
+    const int every = p.causal ? min(job.keys, p.by_group(job.row0) + shift + 1) : job.keys;
     // the splits' runs of tiles: as even as whole tiles allow, none shorter than `least`
     const int all_tiles = (seen + 31) / 32;
-    const int run = max(least, (all_tiles + splits - 1) / splits);
+    const int run = max(least, p.by_splits(all_tiles + splits - 1));
     const int live = max(1, (all_tiles + run - 1) / run);
     if (split >= live) return;
     const int first = split * run, tiles = min(run, all_tiles - first);
@@ -140,8 +139,7 @@ __global__ __launch_bounds__(64 * kWaves, kDim <= 128 ? 2 : 1) void attention_ro
 
     const int quads = p.dim / 4;
     auto store = [&](int r, int c, f32x4 sum, float inverse) {
-        const int64_t tok = (job.row0 + r) / p.group;
-        const int h = kv_head * p.group + (job.row0 + r) % p.group;
+        const int tok = p.by_group(job.row0 + r), h = kv_head * p.group + job.row0 + r - tok * p.group;
         uint16_t* out = p.out + ((static_cast<int64_t>(job.b) * p.sq + job.q_start + tok) * p.heads + h) * p.dim + c * 4;
         *reinterpret_cast<uint2*>(out) =
             make_uint2(pack2<kBf16>(sum[0] * inverse, sum[1] * inverse), pack2<kBf16>(sum[2] * inverse, sum[3] * inverse));
@@ -163,7 +161,7 @@ __global__ __launch_bounds__(64 * kWaves, kDim <= 128 ? 2 : 1) void attention_ro
     };
     if (live == 1) {
         for (int u = threadIdx.x; u < rows * quads; u += kThreads) {
-            const int r = u / quads, c = u - r * quads;
+            const int r = p.by_quads(u), c = u - r * quads;
             float top, sum_of;
             const f32x4 sum = joined(r, c, top, sum_of);
             store(r, c, sum, sum_of == 0.0f ? 0.0f : 1.0f / sum_of);
@@ -180,7 +178,7 @@ __global__ __launch_bounds__(64 * kWaves, kDim <= 128 ? 2 : 1) void attention_ro
     const int64_t place = (static_cast<int64_t>(kv_head) * slots + slot);
     const auto parts = resource_of(partials + place * splits * (kPartBytes / 4), static_cast<int64_t>(splits) * kPartBytes);
     for (int u = threadIdx.x; u < rows * quads; u += kThreads) {
-        const int r = u / quads, c = u - r * quads;
+        const int r = p.by_quads(u), c = u - r * quads;
         float top, sum_of;
         const f32x4 sum = joined(r, c, top, sum_of);
         const int at = split * kPartBytes + r * kRowFloats * 4;
@@ -230,7 +228,7 @@ __global__ __launch_bounds__(64 * kWaves, kDim <= 128 ? 2 : 1) void attention_ro
     int teams = 1;
     while (teams * 2 * places <= kThreads) teams *= 2;
     auto gather = [&](int u, int from) {
-        const int r = u / quads, at = r * kRowFloats * 4 + 16 + (u - r * quads) * 16;
+        const int r = p.by_quads(u), at = r * kRowFloats * 4 + 16 + (u - r * quads) * 16;
         f32x4 sum = f32x4{};
         constexpr int kAhead = 8;
         for (int s0 = from; s0 < live; s0 += kAhead * teams) {
@@ -245,7 +243,10 @@ __global__ __launch_bounds__(64 * kWaves, kDim <= 128 ? 2 : 1) void attention_ro
         return sum;
     };
     if (teams == 1) {
-        for (int u = threadIdx.x; u < places; u += kThreads) store(u / quads, u % quads, gather(u, 0), inverses[u / quads]);
+        for (int u = threadIdx.x; u < places; u += kThreads) {
+            const int r = p.by_quads(u);
+            store(r, u - r * quads, gather(u, 0), inverses[r]);
+        }
     } else {
         const int team = threadIdx.x / places, u = threadIdx.x - team * places;
         if (team < teams) sums[team * places + u] = gather(u, team);
@@ -253,7 +254,8 @@ __global__ __launch_bounds__(64 * kWaves, kDim <= 128 ? 2 : 1) void attention_ro
         if (team == 0) {
             f32x4 sum = sums[u];
             for (int i = 1; i < teams; ++i) sum += sums[i * places + u];
-            store(u / quads, u % quads, sum, inverses[u / quads]);
+            const int r = p.by_quads(u);
+            store(r, u - r * quads, sum, inverses[r]);
         }
     }
     if (threadIdx.x == 0)  // ready for the next call on this stream
@@ -264,10 +266,16 @@ template <int kDim, bool kBf16, int kMask, int kWaves>
 int launch_attention_rows(const AttnArgs& p, const AttnPlan& plan, void* workspace, hipStream_t stream) {
     const int64_t total = plan.slots * p.kv_heads * plan.splits;
     const int64_t grid = (total + kNumXcd - 1) / kNumXcd * kNumXcd;
-    if (plan.slots > 0x7fffffff || grid * 64 * kWaves > 0xffffffffll) return FEATHER_ERR_UNSUPPORTED;
+    if (grid * 64 * kWaves > 0xffffffffll) return FEATHER_ERR_UNSUPPORTED;
+    AttnArgs args = p;
+    args.by_slots = AttnDivisor::of(plan.slots);
+    args.by_blocks = AttnDivisor::of((static_cast<int64_t>(p.sq) * p.group + 31) / 32);
+    args.by_group = AttnDivisor::of(p.group);
+    args.by_splits = AttnDivisor::of(plan.splits);
+    args.by_quads = AttnDivisor::of(p.dim / 4);
     auto* kernel = attention_rows_kernel<kDim, kBf16, kMask, kWaves>;
     kernel<<<dim3(static_cast<uint32_t>(grid)), 64 * kWaves, 0, stream>>>(
-        p, static_cast<int>(plan.slots), total, plan.splits, plan.least, static_cast<uint32_t*>(workspace),
+        args, static_cast<int>(plan.slots), static_cast<int>(total), plan.splits, plan.least, static_cast<uint32_t*>(workspace),
         reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kAttnCounterBytes));
     return hipGetLastError() == hipSuccess ? FEATHER_OK : FEATHER_ERR_LAUNCH;
 }

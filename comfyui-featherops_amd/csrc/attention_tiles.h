@@ -34,35 +34,24 @@ struct AttnTile {
 
 // Their hazards are the code's own business: a source that another vector instruction wrote needs two wait states before
 // the product (kPadded puts them there), whoever else reads a result waits for it.
-#define FEATHER_MFMA32(type, before, result, from, after) \
-    asm volatile(before "v_mfma_f32_32x32x16_" type " %0, %1, %2, " from after : result(c) : "v"(a), "v"(b))
+#define FEATHER_MFMA32(type, before, result, from) \
+    asm volatile(before "v_mfma_f32_32x32x16_" type " %0, %1, %2, " from : result(c) : "v"(a), "v"(b))
 template <bool kBf16>
 __device__ __forceinline__ void mfma_first(f32x16& c, u32x4 a, u32x4 b) {
-    if constexpr (kBf16) FEATHER_MFMA32("bf16", "s_nop 1\n\t", "=&v", "0", "");
-    else FEATHER_MFMA32("f16", "s_nop 1\n\t", "=&v", "0", "");
+    if constexpr (kBf16) FEATHER_MFMA32("bf16", "s_nop 1\n\t", "=&v", "0");
+    else FEATHER_MFMA32("f16", "s_nop 1\n\t", "=&v", "0");
 }
 template <bool kBf16, bool kAccumulation, bool kPadded>
 __device__ __forceinline__ void mfma_next(f32x16& c, u32x4 a, u32x4 b) {
     if constexpr (kAccumulation) {
-        if constexpr (kBf16) FEATHER_MFMA32("bf16", "s_nop 1\n\t", "+a", "%0", "");
-        else FEATHER_MFMA32("f16", "s_nop 1\n\t", "+a", "%0", "");
+        if constexpr (kBf16) FEATHER_MFMA32("bf16", "s_nop 1\n\t", "+a", "%0");
+        else FEATHER_MFMA32("f16", "s_nop 1\n\t", "+a", "%0");
     } else if constexpr (kPadded) {
-        if constexpr (kBf16) FEATHER_MFMA32("bf16", "s_nop 1\n\t", "+v", "%0", "");
-        else FEATHER_MFMA32("f16", "s_nop 1\n\t", "+v", "%0", "");
+        if constexpr (kBf16) FEATHER_MFMA32("bf16", "s_nop 1\n\t", "+v", "%0");
+        else FEATHER_MFMA32("f16", "s_nop 1\n\t", "+v", "%0");
     } else {
-        if constexpr (kBf16) FEATHER_MFMA32("bf16", "", "+v", "%0", "");
-        else FEATHER_MFMA32("f16", "", "+v", "%0", "");
-    }
-}
-// One with the waits on both sides: its result is in its registers behind it (at most 19 wait states).
-template <bool kBf16, bool kAccumulation>
-__device__ __forceinline__ void mfma_alone(f32x16& c, u32x4 a, u32x4 b) {
-    if constexpr (kAccumulation) {
-        if constexpr (kBf16) FEATHER_MFMA32("bf16", "s_nop 1\n\t", "+a", "%0", "\n\ts_nop 15\n\ts_nop 3");
-        else FEATHER_MFMA32("f16", "s_nop 1\n\t", "+a", "%0", "\n\ts_nop 15\n\ts_nop 3");
-    } else {
-        if constexpr (kBf16) FEATHER_MFMA32("bf16", "s_nop 1\n\t", "+v", "%0", "\n\ts_nop 15\n\ts_nop 3");
-        else FEATHER_MFMA32("f16", "s_nop 1\n\t", "+v", "%0", "\n\ts_nop 15\n\ts_nop 3");
+        if constexpr (kBf16) FEATHER_MFMA32("bf16", "", "+v", "%0");
+        else FEATHER_MFMA32("f16", "", "+v", "%0");
     }
 }
 #undef FEATHER_MFMA32
@@ -75,7 +64,7 @@ __device__ __forceinline__ void settle(f32x16& c) {
 
 template <int kDim, bool kBf16, int kMask>
 __global__ __launch_bounds__(256, kDim > 128 ? 1 : kDim == 64 && kMask == kMaskNone ? 4 : 2) void attention_tile_kernel(
-    const AttnArgs p, int slots, int64_t per_xcd) {
+    const AttnArgs p, int slots, int per_xcd) {
     using T = AttnTile<kDim, kMask>;
     using Mask = AttnMaskRegs<kBf16, kMask, 1>;
     constexpr int kSteps = kDim / 16, kBlocks = kDim / 32, kRowBytes = kDim * 2;
@@ -84,10 +73,9 @@ __global__ __launch_bounds__(256, kDim > 128 ? 1 : kDim == 64 && kMask == kMaskN
     __shared__ __attribute__((aligned(1024))) uint8_t rings[T::kLds];
 
     // workgroup i runs on XCD i % 8: each XCD takes consecutive blocks of few heads, whose keys its L2 keeps
-    const int64_t id = static_cast<int64_t>(blockIdx.x % kNumXcd) * per_xcd + blockIdx.x / kNumXcd;
-    const int head = static_cast<int>(id / slots);
-    if (blockIdx.x / kNumXcd >= per_xcd || head >= p.heads) return;
-    const int slot = static_cast<int>(id - static_cast<int64_t>(head) * slots);
+    const int id = static_cast<int>(blockIdx.x % kNumXcd) * per_xcd + static_cast<int>(blockIdx.x / kNumXcd);
+    const int head = p.by_slots(id), slot = id - head * slots;
+    if (head >= p.heads) return;
     AttnJob job;
     // (causal: the blocks with most keys first)
     if (!attn_job<T::kRows>(p, p.causal ? slots - 1 - slot : slot, 1, job)) return;
@@ -177,7 +165,7 @@ __global__ __launch_bounds__(256, kDim > 128 ? 1 : kDim == 64 && kMask == kMaskN
     auto cut = [&](f32x16 (&s)[1], Mask& mask, int u) {
         const bool past = u * 32 + 32 > wave_least;
         if (kMask != kMaskNone || past) settle(s[0]);
-        mask.put(s, p.scale);
+        mask.put(s, p.scale, mask_row);
         if (past) attn_cut<1>(s, u * 32, limit);
     };
     auto load_masks = [&](Mask (&m)[2], int u) {
@@ -323,14 +311,26 @@ __global__ __launch_bounds__(256, kDim > 128 ? 1 : kDim == 64 && kMask == kMaskN
             else turn(u, s1, s0, p1, p0, ka, va, kn, mask[set][1], first, last);
         }
     }
-    // the last unit's values; the results are in their registers behind it
+    // the last unit's values
+    {
+        const uint32_t va = (units - 1) % T::kRing * kUnit;
+        u32x4 vf[3];
+        vf[0] = read_v(0, va);
+        vf[1] = read_v(1, va);
 #pragma unroll
-    for (int n = 0; n < kSteps; ++n)
-        mfma_alone<kBf16, T::kAccumulation>(o[n % kBlocks], read_v(n, (units - 1) % T::kRing * kUnit), p1[n / kBlocks]);
+        for (int n = 0; n < kSteps; ++n) {
+            if (n + 2 < kSteps) vf[(n + 2) % 3] = read_v(n + 2, va);
+            __builtin_amdgcn_sched_barrier(0);
+            mfma_next<kBf16, T::kAccumulation, T::kAccumulation>(o[n % kBlocks], vf[n % 3], p1[n / kBlocks]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    }
     for (int u = units; u < all_units; u += T::kBatch) {
         wait_batch();
         copy_batch(u);
     }
+#pragma unroll
+    for (int b = 0; b < kBlocks; ++b) settle<T::kAccumulation>(o[b]);
     wait_vmcnt<0>();  // (no copy may be on its way when the workgroup's LDS goes to another)
 
     const int64_t out_row = static_cast<int64_t>(p.heads) * p.dim * 2;
@@ -363,9 +363,12 @@ __global__ __launch_bounds__(256, kDim > 128 ? 1 : kDim == 64 && kMask == kMaskN
 template <int kDim, bool kBf16, int kMask>
 int launch_attention_tiles(const AttnArgs& p, const AttnPlan& plan, hipStream_t stream) {
     const int64_t per_xcd = (plan.slots * p.heads + kNumXcd - 1) / kNumXcd;
-    if (plan.slots > 0x7fffffff || per_xcd * kNumXcd * 256 > 0xffffffffll) return FEATHER_ERR_UNSUPPORTED;
+    if (per_xcd * kNumXcd * 256 > 0xffffffffll) return FEATHER_ERR_UNSUPPORTED;
+    AttnArgs args = p;
+    args.by_slots = AttnDivisor::of(plan.slots);
+    args.by_blocks = AttnDivisor::of((p.sq + 127) / 128);
     auto* kernel = attention_tile_kernel<kDim, kBf16, kMask>;
-    kernel<<<dim3(static_cast<uint32_t>(per_xcd * kNumXcd)), 256, 0, stream>>>(p, static_cast<int>(plan.slots), per_xcd);
+    kernel<<<dim3(static_cast<uint32_t>(per_xcd * kNumXcd)), 256, 0, stream>>>(args, static_cast<int>(plan.slots), static_cast<int>(per_xcd));
     return hipGetLastError() == hipSuccess ? FEATHER_OK : FEATHER_ERR_LAUNCH;
 }
 

@@ -63,6 +63,28 @@ def test_forms(at, cuda, form, kind):
             assert torch.equal(at.attention(q, k, v, causal=causal, mask=mask, k_lengths=lengths), o)
 
 
+@pytest.mark.parametrize("first", [0, 1, 2, 3])
+@pytest.mark.parametrize("kind", ["bool", "half", "fp32"])
+@pytest.mark.parametrize("shape", [(3, 1101, 157, 16, 16, 40), (2, 9, 301, 4, 2, 128)], ids=["tiles", "rows"])
+def test_mask_alignment(at, cuda, shape, kind, first):
+    """Rows that begin at any element, odd and even distances between them, and what lies around them of another sign."""
+    B, Sq, Sk, H, Hk, D = shape
+    g = torch.Generator().manual_seed(first)
+    q, k, v = qkv(g, B, Sq, Sk, H, Hk, D, F16)
+    for width in (Sk + 4, Sk + 7):
+        if kind == "bool":
+            whole = torch.zeros(Sq, width, dtype=torch.bool)
+            whole[:, first:first + Sk] = torch.rand(Sq, Sk, generator=g) < 0.7
+        else:
+            whole = torch.full((Sq, width), float("nan"))
+            whole[:, first:first + Sk] = torch.randn(Sq, Sk, generator=g) * 2.0
+            whole = whole.to(F16 if kind == "half" else F32)
+        mask = whole.cuda()[:, first:first + Sk]
+        for causal in (False, True):
+            o = at.attention(q, k, v, mask=mask, causal=causal)
+            check(o, *A.attention(d(q), d(k), d(v), causal, None, None, d(mask[None, None])), Sk, f"{width} {causal}", 8.0)
+
+
 @pytest.mark.parametrize("D", [64, 128, 200])
 def test_packed_tokens_over_long_caches(at, cuda, D):
     """One and few queries a sequence, whose keys workgroups share; a sequence without keys, one without queries."""
