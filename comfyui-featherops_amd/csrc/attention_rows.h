@@ -6,6 +6,11 @@
 // wave waits for another before the end. There the waves' sums are joined through
 // LDS, and where several workgroups share a row's keys, their sums through the workspace by the one
 // that arrives last, in the order of the keys: the result does not depend on who that is.
+//
+// Bound by the memory's latency and rate: a wave has one tile of keys and one of values on their way, which makes 64 to
+// 128 KB a CU. One token, 32 heads over 8, 32001 keys of 128: 31 us, 4.2 TB/s (a workgroup a block: 972); eight tokens over 1 to
+// 4096 keys: 15 us of kernel, 3.1 TB/s. A join through the workspace costs 4 us and more, so that one query over 729 keys x 16 heads
+// (7.8 us) is left to 16 workgroups.
 #pragma once
 
 #include "attention_device.h"

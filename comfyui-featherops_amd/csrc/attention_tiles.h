@@ -10,6 +10,13 @@
 // its weights behind them, 32760 x 32760 x 12 heads of 128 took 7.0 ms: the two overlapped only between the two waves of
 // a SIMD.)
 //
+// Now 5.8 ms (1.13 PFLOP/s; 0.99 to 1.06 at 4096 x 4096 x 24 heads of 128 and at 8192 x 8192 x 12 of 256): matrix units busy 58% of
+// the time at the 1.9 GHz that the card holds under it, no LDS bank conflicts, the rest waits for barriers and for LDS. Over 512
+// keys, 2 x 8190 x 40 heads: 250 us with a key mask, 690 TFLOP/s, of which a workgroup's start, its queries' load and its stores
+// take 100, as they overlap with the other workgroup of the CU alone (LDS and registers hold two).
+// 32 queries a wave: with 64 each key read from LDS served twice the products, but scores and results of both left no
+// registers to keep products and weights apart. Two teams of waves that take half the keys each were faster nowhere.
+//
 // The products are taken transposed, as in AttnWave. They are inline asm, which keeps their order and their
 // accumulators' place: results in accumulation registers where the vector registers do not hold everything.
 #pragma once
