@@ -266,7 +266,7 @@ int launch(const RopeArgs& p, int lanes, hipStream_t stream) {
     const int heads = (kRow ? kThreads : 64) / lanes * kPasses;
     const int chunks_q = (p.side[0].heads + heads - 1) / heads, chunks = chunks_q + (p.side[1].heads + heads - 1) / heads;
     const int64_t items = p.tokens * chunks, blocks = kRow ? items : (items + kThreads / 64 - 1) / (kThreads / 64);
-    if (blocks * kThreads > 0xffffffffll) return FEATHER_ERR_UNSUPPORTED;  // (terabytes)
+    if (blocks * kThreads > 0xffffffffll) return FEATHER_ERR_UNSUPPORTED;  // (2^24 workgroups)
     auto* kernel = qk_norm_rope_kernel<T, kPasses, kRow>;
     kernel<<<dim3(static_cast<uint32_t>(blocks)), kThreads, 0, stream>>>(p, lanes, static_cast<uint32_t>(items), chunks_q, chunks);
     return hipGetLastError() == hipSuccess ? FEATHER_OK : FEATHER_ERR_LAUNCH;
@@ -285,13 +285,12 @@ int of_type(const RopeArgs& p, hipStream_t stream) {
         if (passes <= 4) return launch<T, 4, true>(p, lanes, stream);
         return launch<T, 8, true>(p, lanes, stream);
     }
-    // Few tokens: a wave for every 64 / lanes heads. Many: a wave takes three or four times as many, which leaves the fewest
-    // lanes idle at the row's end.
+    // Few tokens: a wave for every 64 / lanes heads (100 tokens of 24 heads of 128: 4.0 us, with two passes 4.1). Many: two passes,
+    // for which the table is loaded once (20000 tokens of 24 heads of 96: 89 us with one pass, 70 with two). Three and four
+    // leave too few waves, or their last pass idle (65536 tokens of 32 + 4 heads of 128 221 us with two, 241 and 238;
+    // 3 x 1003 of 15 + 15 of 80 12.4, 15.1 and 12.5; only of 32760 x 40 + 40 three are 2% faster).
     const int all = (most * lanes + 63) / 64;
-    if (p.tokens < 256 || all <= 1) return launch<T, 1, false>(p, lanes, stream);
-    if (all <= 2) return launch<T, 2, false>(p, lanes, stream);
-    if ((all + 2) / 3 * 3 < (all + 3) / 4 * 4) return launch<T, 3, false>(p, lanes, stream);
-    return launch<T, 4, false>(p, lanes, stream);
+    return p.tokens < 256 || all <= 1 ? launch<T, 1, false>(p, lanes, stream) : launch<T, 2, false>(p, lanes, stream);
 }
 
 __global__ __launch_bounds__(kThreads) void rope_table_kernel(const RopeTableArgs p) {

@@ -443,7 +443,8 @@ int feather_rope_table(const void* positions, int position_dtype, int64_t rows, 
  *   table_batch_stride (floats), or NULL. Pair p of a head is values 2 p and 2 p + 1, or with
  *   pairs_of_halves p and pairs + p; values from 2 pairs on are not turned.
  * head_dim: a multiple of 8 up to 256. Strides count elements; q_out and k_out are
- * contiguous; any alignment of the element types. k_heads 0: no keys. Weights may be
+ * contiguous; any alignment of the element types; up to 2^24 workgroups (64 million tokens of few heads;
+ * FEATHER_ERR_UNSUPPORTED beyond). k_heads 0: no keys. Weights may be
  * NULL; weight_dtype is dtype or fp32. No counterpart in the reference.
  */
 typedef struct feather_rope_args {
