@@ -43,9 +43,10 @@ struct AttnArgs {
     int sq, sk;  // tokens of a sample; packed: all tokens
     int mask_type, causal, bf16;
     float scale;
-    // set at the launch: blocks of all samples, of one sample, heads that share a key head, workgroups that share keys, and
-    // what a store takes of a head (rows)
-    AttnDivisor by_slots, by_blocks, by_group, by_splits, by_quads;
+    // set at the launch: blocks of all samples, of one sample; heads of a class (tiles), heads that share a key head; rows:
+    // workgroups that share keys, and what a store takes of a head
+    AttnDivisor by_slots, by_blocks, by_class, by_group, by_splits, by_quads;
+    int classes, class_heads;
 };
 
 // Which kernel takes a call, and how.
