@@ -11,7 +11,8 @@
 // a SIMD.)
 //
 // Now 5.8 ms (1.13 PFLOP/s; 0.99 to 1.06 at 4096 x 4096 x 24 heads of 128 and at 8192 x 8192 x 12 of 256): matrix units busy 58% of
-// the time at the 1.9 GHz that the card holds under it, no LDS bank conflicts, the rest waits for barriers and for LDS. Over 512
+// the time at the 1.9 GHz that the card holds under it, no LDS bank conflicts; a wave's reads of keys and values (16 KB a unit) keep
+// LDS as busy as its products do its SIMD, and what does not fall side by side waits. Over 512
 // keys, 2 x 8190 x 40 heads: 250 us with a key mask, 690 TFLOP/s, of which a workgroup's start, its queries' load and its stores
 // take 100, as they overlap with the other workgroup of the CU alone (LDS and registers hold two).
 // 32 queries a wave: with 64 each key read from LDS served twice the products, but scores and results of both left no
