@@ -8,7 +8,7 @@
 // 100000 has 17 bits before the point, and an fp32 angle would keep 7 behind it.
 //
 // HBM bound: x is read once and stays in registers over the norm. 32760 tokens x 40 heads of 128 with a norm of the row:
-// 250 us, 5.4 TB/s (a 1 GiB copy: 5.1); 2 x 4250 x 24 heads with one of the head 35 us of kernel. A lane has 8 values of a head; a wave takes
+// 250 us, 5.4 TB/s (a 1 GiB copy: 5.1); 2 x 4250 x 24 heads with one of the head 37 us of kernel. A lane has 8 values of a head; a wave takes
 // one token's heads, several in a row, so that the table's values are loaded once for them. With pairs of
 // two halves the partner's values come through LDS. Where the norm is over all heads a workgroup has
 // the token.
