@@ -113,8 +113,9 @@ __global__ __launch_bounds__(256, kDim > 128 ? 1 : kDim == 64 && kMask == kMaskN
     const int wave_keys = row0 >= job.rows ? 0 : p.causal ? min(job.keys, row0 + 32 + shift) : job.keys;
     const int wave_least = p.causal ? min(job.keys, row0 + shift + 1) : job.keys;
     const int wg_keys = p.causal ? min(job.keys, min(job.row0 + T::kRows, job.rows) + shift) : job.keys;
-    // units, in twos; two at least, of which a wave without keys sees none
-    const int units = max(1, (wave_keys + 63) / 64) * 2, all_units = (wg_keys + 31) / 32;
+    // units, in twos; two at least, of which a wave without keys sees none. All waves pass the barriers of wg_units turns, the
+    // most that one of them has.
+    const int units = max(1, (wave_keys + 63) / 64) * 2, wg_units = max(1, (wg_keys + 63) / 64) * 2;
 
     // waves 0 and 1 copy keys, 2 and 3 values
     const bool copies_keys = wave < 2;
@@ -333,7 +334,9 @@ __global__ __launch_bounds__(256, kDim > 128 ? 1 : kDim == 64 && kMask == kMaskN
             else turn(u, s1, s0, p1, p0, ka, va, kn, mask[set][1], first, last);
         }
     }
-    // the last unit's values
+    // The last unit's values. The wait before its turn was one for them too where each turn has one; with two units a batch they
+    // came with its own batch.
+    if (T::kBatch > 1) wait_batch();
     {
         const uint32_t va = (units - 1) % T::kRing * kUnit;
         u32x4 vf[3];
@@ -347,9 +350,11 @@ __global__ __launch_bounds__(256, kDim > 128 ? 1 : kDim == 64 && kMask == kMaskN
         }
         __builtin_amdgcn_sched_barrier(0);
     }
-    for (int u = units; u < all_units; u += T::kBatch) {
-        wait_batch();
+    // the turns that other waves have more than this one: its share of their copies
+    for (int u = units; u < wg_units; u += T::kBatch) {
+        if (T::kBatch == 1) wait_batch();
         copy_batch(u);
+        if (T::kBatch > 1) wait_batch();  // (the one that stood before turn u came before the last unit's values)
     }
 #pragma unroll
     for (int b = 0; b < kBlocks; ++b) settle<T::kAccumulation>(o[b]);

@@ -135,3 +135,89 @@ def test_results_are_waited_for(kernels):
                     entry[f] = merged
                     todo.append(f)
         assert not bad, f"{name}: {sorted(bad)[:5]} ({len(bad)})"
+
+
+RING = 4  # units of 32 keys that have places in LDS, of keys and of values
+
+
+def wait_of(ops, counter):
+    m = re.search(rf"{counter}\((\d+)\)", " ".join(ops))
+    return int(m.group(1)) if m else None
+
+
+def follow_copies(graph, dim, batch, values, turns=10):
+    """Every path of a wave that copies keys, or values, through the compiled kernel, for all numbers of units up to `turns` of its own
+    and of the workgroup's. A barrier stands before the first turn and then before every `batch` turns, and all waves run the same
+    code between two of them: what lies in LDS behind a barrier is what a wave's wait before it has seen land, and what may be
+    overwritten behind it is what turns before it read. Turn u reads the keys of unit u + 1 (those of unit 0 come before the first turn) and the
+    values of unit u - 1 (of unit -1, zeros in place 3, at first); behind the last turn the last unit's values are read.
+    State: barriers passed, copies issued, landed, landed at the last barrier, reads. Returns (complaints, units read at the ends)."""
+    copies, reads = dim // 32, dim // 8 if values else dim // 16  # instructions for a unit
+    is_read = "ds_read_b64_tr" if values else "ds_read_b128"
+    first = (RING - 2 if values else RING) + 1 - batch  # units copied before the first barrier
+    lead = 0 if values else 1
+    bad, ends, seen, todo = set(), set(), set(), [("entry", (0, 0, 0, 0, 0))]
+    while todo:
+        label, state = todo.pop()
+        if (label, state) in seen:
+            continue
+        seen.add((label, state))
+        seq, follow = graph[label]
+        barriers, issued, landed, ready, read = state
+        turn = (barriers - 2) * batch  # the one that the last barrier stands before
+        lost = False
+        for i, (name, ops) in enumerate(seq):
+            if name.startswith("buffer_load") and "lds" in ops[-1].split():
+                before = issued // copies - RING  # the unit whose place this copy takes
+                if barriers == 0:
+                    lost = issued // copies >= RING
+                elif before > turn - (2 if values else 0):
+                    bad.add(f"{label}: unit {before + RING} is copied over unit {before} behind the barrier of turn {turn}")
+                issued += 1
+            elif name == "s_waitcnt":
+                left = wait_of(ops, "vmcnt")
+                if left is not None:
+                    landed = max(landed, issued - left)
+            elif name == "s_barrier":
+                if barriers == 0:
+                    lost = issued != first * copies
+                else:
+                    turn = (barriers - 1) * batch
+                    if issued != (turn + first) * copies:
+                        bad.add(f"{label}: {issued} copies before turn {turn}")
+                    if read >= 0 and read // reads < turn + lead:
+                        read = -1  # this wave has fewer units: it has read its last one
+                if i == 0 or seq[i - 1][0] != "s_waitcnt" or wait_of(seq[i - 1][1], "lgkmcnt") != 0:
+                    bad.add(f"{label}: reads may be on their way at a barrier")
+                barriers, ready = barriers + 1, landed
+                lost = lost or turn > turns
+            elif name.startswith(is_read) and barriers:
+                unit = read // reads - (1 if values else 0)
+                if read < 0:
+                    bad.add(f"{label}: a read behind the last turn's barriers")
+                elif (unit + 1) * copies > ready:
+                    bad.add(f"{label}: unit {unit} is read behind the barrier of turn {turn}, before which {ready // copies} have landed")
+                read += 1 if read >= 0 else 0
+            if lost:
+                break
+        if lost:
+            continue
+        if not follow and barriers:
+            if landed != issued:
+                bad.add(f"{label}: copies may be on their way at the end")
+            ends.add(read // reads if read >= 0 else -1)
+        todo += [(f, (barriers, issued, landed, ready, read)) for f in follow if f in graph]
+    return bad, ends
+
+
+@pytest.mark.parametrize("values", [False, True], ids=["keys", "values"])
+def test_copies_are_waited_for(kernels, values):
+    """Nothing is read from LDS before its copy has landed and a barrier has told so, nor written over before a barrier behind its
+    last read."""
+    for name, (body, _) in kernels.items():
+        dim, mask = map(int, re.search(r"kernelILi(\d+)ELb\dELi(\d)E", name).groups())
+        graph = blocks(body)
+        bad, ends = follow_copies(graph, dim, 2 if mask else 1, values)
+        assert not bad, f"{name}: {sorted(bad)[:5]} ({len(bad)})"
+        # paths of 2, 4, ... units, the first one's values of unit -1 to 1, its keys of unit 0 to 2
+        assert {3, 5, 7} <= ends, (name, ends)
