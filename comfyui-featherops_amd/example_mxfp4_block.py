@@ -150,6 +150,9 @@ def main() -> None:
     with torch.inference_mode():
         args_in = inputs(args.tokens, args.width)
         report(f"{sizes} hidden {args.hidden}", *build(args.width, args.hidden), args_in)
+        if args.width % args.head_dim:
+            print(f"{sizes}: no heads of {args.head_dim} in this width, no attention half")
+            return
         rest = args.head_dim // 8 * 3 // 2 * 2  # the two directions of a picture; time has what is left
         table = rope_table(positions(args.tokens), (args.head_dim - 2 * rest, rest, rest))
         report(f"{sizes} heads {args.width // args.head_dim}", *build_attention(args.width, args.head_dim), (*args_in, table))
