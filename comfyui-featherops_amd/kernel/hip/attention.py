@@ -20,7 +20,8 @@ Keys that causality or a mask takes from a query have weight zero in its sum, as
 values must be finite for it to stay so.
 
 Views are read in place if head_dim is contiguous and tokens and heads lie on 16-byte boundaries (a layer's joint output,
-heads in front of tokens, a slice of a cache), others are copied first. Runs in libfeatherops_amd.so on
+heads in front of tokens, a slice of a cache), others are copied first. A call has fewer than 2^24 workgroups (128 queries of a
+head each, or 32 of a group of heads; some forms 2^23) and is refused beyond. Runs in libfeatherops_amd.so on
 torch's current stream; there is no other compute path. Forward only: no gradients.
 """
 

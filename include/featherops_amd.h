@@ -483,8 +483,9 @@ int feather_qk_norm_rope(const feather_rope_args* args, hipStream_t stream);
  *   followed out of them. No mask, no k_lengths.
  * dtype F16 or BF16; head_dim a multiple of 8 up to 256; q, k, v, out at 16-byte
  * boundaries, strides multiples of 8, a token stride below 2^23; scale positive; batch up to 65536, k_tokens
- * and q_tokens times heads / kv_heads up to 2^30. Keys that causality or a mask takes from a query count with weight
- * zero: their values must be finite.
+ * and q_tokens times heads / kv_heads up to 2^30; fewer than 2^24 workgroups, or 2^23 of 8 waves (plan[1] * plan[2] of
+ * feather_attention_plan; FEATHER_ERR_UNSUPPORTED from there on: one query of 65536 samples x 256 heads, say). Keys that
+ * causality or a mask takes from a query count with weight zero: their values must be finite.
  * Workspace: the size below (0: none needed), the contract of feather_launch_scaled_mm_ws
  * (its first 64 KB zero before the first use and left zero); with less, a query's keys are not shared
  * among workgroups, and the sums run in another order. No counterpart in the reference.

@@ -250,3 +250,14 @@ def test_plans(lib):
             assert waves and blocks <= 16384 and size == 65536 + blocks * splits * 32 * (wide(D) + 4) * 4
         if args.q_offsets is None:
             assert blocks == (B * Hk * -(-Sq * G // 32) if waves else B * Hk * G * -(-Sq // 128))
+
+
+def test_more_workgroups_than_a_launch_holds(lib):
+    """2^32 threads and more are refused before a launch, in every form: few rows of 4 and of 8 waves, blocks of 128 queries."""
+    for waves, shape in ((4, (65536, 1, 8, 256, 256, 64)), (8, (32768, 1, 9000, 256, 256, 64)), (0, (65536, 33, 8, 256, 256, 128))):
+        args = attention_args(*shape)
+        form, splits, blocks = plan_of(lib, args)
+        threads = splits * blocks * 64 * (form or 4)
+        assert threads >= 2 ** 32, (form, splits, blocks)
+        assert form == waves
+        assert lib.feather_attention(ctypes.byref(args), None, 0, None) == 2
