@@ -13,6 +13,7 @@ using namespace feather;
 
 constexpr int64_t kMaxTokens = int64_t(1) << 30;
 constexpr int64_t kMaxHeads = 1 << 16;
+constexpr float kMaxScale = 0x1p127f;  // times log2(e) it is finite
 
 bool value_type(int t) { return t == FEATHER_DTYPE_F16 || t == FEATHER_DTYPE_BF16 || t == FEATHER_DTYPE_F32; }
 int round_up_pow2(int x) {
@@ -32,7 +33,7 @@ int attention_args(const feather_attention_args* a, AttnArgs& p, bool& empty) {
     if (!a || a->batch < 0 || a->batch > kAttnMaxBatch || a->q_tokens < 0 || a->q_tokens > kMaxTokens || a->k_tokens < 0 ||
         a->k_tokens > kMaxTokens || a->heads < 1 || a->heads > kMaxHeads || a->kv_heads < 1 || a->heads % a->kv_heads ||
         a->head_dim < 8 || a->head_dim > kAttnMaxDim || a->head_dim % 8 ||
-        (a->dtype != FEATHER_DTYPE_F16 && a->dtype != FEATHER_DTYPE_BF16) || !(a->scale > 0.0f) || !std::isfinite(a->scale) ||
+        (a->dtype != FEATHER_DTYPE_F16 && a->dtype != FEATHER_DTYPE_BF16) || !(a->scale > 0.0f) || a->scale > kMaxScale ||
         (a->causal != 0 && a->causal != 1))
         return FEATHER_ERR_INVALID;
     // rows of a group of heads are counted in 32 bits

@@ -227,7 +227,7 @@ void check_qkv(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, in
 double check_scale(const at::Tensor& q, std::optional<double> scale) {
     if (scale.has_value()) {
         const float s = static_cast<float>(*scale);
-        TORCH_CHECK(s > 0.0f && std::isfinite(s), "scale must be positive and finite");
+        TORCH_CHECK(s > 0.0f && s <= 0x1p127f, "scale must be positive and at most 2^127");
         return *scale;
     }
     return 0.0;

@@ -9,7 +9,8 @@
 over the keys that query i may see; a query that may see none gets zeros. q and the result are (batch, tokens, heads,
 head_dim), k and v (batch, tokens, kv heads, head_dim), in fp16 or bf16, head_dim a multiple of 8 up to 256;
 heads / kv heads consecutive query heads share a key head. Scores, maxima and sums are fp32; the weights p are
-rounded to the tensors' type, as is the result. scale is 1 / sqrt(head_dim) by default.
+rounded to the tensors' type, as is the result. scale is 1 / sqrt(head_dim) by default, positive and 2^127 at most; q . k and
+scale times it are to stay below 2^125 in magnitude.
 
 Which keys a query sees:
   causal     query i of n sees the keys up to i + (keys - n): the last query sees all of them;

@@ -482,7 +482,8 @@ int feather_qk_norm_rope(const feather_rope_args* args, hipStream_t stream);
  *   last sequence are zeros. Offsets must not fall; they are clamped to the tensors, never
  *   followed out of them. No mask, no k_lengths.
  * dtype F16 or BF16; head_dim a multiple of 8 up to 256; q, k, v, out at 16-byte
- * boundaries, strides multiples of 8, a token stride below 2^23; scale positive; batch up to 65536, k_tokens
+ * boundaries, strides multiples of 8, a token stride below 2^23; scale positive, up to 2^127, and q . k, like scale times
+ * that, below 2^125 in magnitude; batch up to 65536, k_tokens
  * and q_tokens times heads / kv_heads up to 2^30; fewer than 2^24 workgroups, or 2^23 of 8 waves (plan[1] * plan[2] of
  * feather_attention_plan; FEATHER_ERR_UNSUPPORTED from there on: one query of 65536 samples x 256 heads, say). Keys that
  * causality or a mask takes from a query count with weight zero: their values must be finite.

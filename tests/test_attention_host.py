@@ -261,3 +261,16 @@ def test_more_workgroups_than_a_launch_holds(lib):
         assert threads >= 2 ** 32, (form, splits, blocks)
         assert form == waves
         assert lib.feather_attention(ctypes.byref(args), None, 0, None) == 2
+
+
+@pytest.mark.parametrize("scale,status", [(2.0 ** 127, 0), (1e-44, 0), (2.4e38, 1), (float("inf"), 1), (float("nan"), 1), (0.0, 1)])
+def test_scales(lib, at, scale, status):
+    """The scale times log2(e) is an fp32 number, too: from 2^127.5 on it would be infinite, and every weight NaN."""
+    plan = (ctypes.c_int64 * 3)()
+    assert lib.feather_attention_plan(ctypes.byref(attention_args(1, 5, 7, 2, 2, 64, scale=scale)), plan) == status
+    q = meta(1, 5, 2, 64)
+    if status:
+        with pytest.raises(RuntimeError, match="positive and at most"):
+            at.attention(q, q, q, scale=scale)
+    else:
+        assert at.attention(q, q, q, scale=scale).shape == q.shape

@@ -1,6 +1,6 @@
-"""Masked attention in blocks of 128 queries on the GPU, for keys and values that no cache holds and that differ from call to
-call: what a workgroup copies then comes late, and what lies in LDS from another call is not the same. Against float64
-(oracle/attention_oracle.py)."""
+"""Masked attention on the GPU against float64 (oracle/attention_oracle.py). In blocks of 128 queries with keys and values that no
+cache holds and that differ from call to call: what a workgroup copies then comes late, and what lies in LDS from another call is
+not the same. Far scales."""
 
 import importlib
 
@@ -72,3 +72,17 @@ def test_new_keys_every_call(at, lib, caches_are_emptied, D, kind):
 @pytest.mark.parametrize("D", [72, 88, 128, 136, 256])
 def test_added_masks_of_many_keys(at, lib, caches_are_emptied, D, kind):
     run(at, lib, caches_are_emptied, 2, 2900, 1300, 24, 8, D, kind, BF16, D)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("Sq", [3, 1500])
+def test_far_scales(at, cuda, Sq, D):
+    """Scales up to the largest, with queries as small, and one that is a subnormal number, beside keys that are masked or behind
+    a query's own."""
+    g = torch.Generator().manual_seed(D + Sq)
+    q, k, v = qkv(g, 2, Sq, 300, 8, 8, D, BF16)
+    keep = (torch.rand(2, 1, 1, 300, generator=g) < 0.7).cuda()
+    for t, scale in ((q * 2.0 ** -100, 2.0 ** 100), (q * 2.0 ** -115, 2.0 ** 127), (q, 1e-44)):
+        for causal in (False, True):
+            o = at.attention(t, k, v, mask=keep, causal=causal, scale=scale)
+            check(o, *A.attention(d(t), d(k), d(v), causal, scale, None, d(keep)), 300, f"{scale} {causal}")
