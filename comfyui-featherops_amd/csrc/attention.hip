@@ -3,10 +3,12 @@
 // Three forms: attention_tiles.h (128 queries of a head a workgroup), and attention_rows.h with 4 or 8 waves and the keys
 // of 32 rows shared by up to 64 workgroups. Each has a time, in microseconds, of a fixed part, a part for each
 // workgroup that a CU gets, and one for its tiles: by their latency one after the other where a CU has one workgroup,
-// by throughput where it has several. Fitted to 30,000 shapes (1 to 4 samples, 1 to 40 heads in groups of 1 to 8, 1 to
-// 16384 queries and keys, a third causal, two fifths with masks), each form and split timed on an MI355X: the form taken is 1.3%
-// slower than the fastest of all in the mean, 8% at the 95th percentile. Most often fastest: few rows with 4 waves and unshared
-// keys (44% of the shapes), with 8 (16%), blocks of 128 queries (16%), shared keys (24%).
+// by throughput where it has several. The constants were fitted to samples without lengths, before masks were read by words and blocks
+// dealt out among the XCDs. With the kernels as they are, over 26,690 shapes (1 to 8 samples with and without lengths, 2 to 30 packed
+// sequences, 1 to 40 heads in groups of 1 to 8, 1 to 16384 queries and keys, a third causal, a fifth with masks), each form and
+// split timed on an MI355X: the form taken is 1.6% slower than the fastest of all in the mean, 10% at the 95th percentile; with lengths,
+// which the host does not know, 2.3% and 13%, packed 1.8% and 12%. Most often fastest: few rows with 4 waves and unshared
+// keys (43% of the shapes), with 8 (15%), blocks of 128 queries (25%), shared keys (18%).
 #include "attention.h"
 
 #include <algorithm>

@@ -10,11 +10,12 @@
 // its weights behind them, 32760 x 32760 x 12 heads of 128 took 7.0 ms: the two overlapped only between the two waves of
 // a SIMD.)
 //
-// Now 5.8 ms (1.13 PFLOP/s; 0.99 to 1.06 at 4096 x 4096 x 24 heads of 128 and at 8192 x 8192 x 12 of 256): matrix units busy 58% of
-// the time at the 1.9 GHz that the card holds under it, no LDS bank conflicts; a wave's reads of keys and values (16 KB a unit) keep
-// LDS as busy as its products do its SIMD, and what does not fall side by side waits. Over 512
-// keys, 2 x 8190 x 40 heads: 250 us with a key mask, 690 TFLOP/s, of which a workgroup's start, its queries' load and its stores
-// take 100, as they overlap with the other workgroup of the CU alone (LDS and registers hold two).
+// Now 5.8 to 5.95 ms (1.11 to 1.13 PFLOP/s; 1.02 at 4096 x 4096 x 24 heads of 128, 1.05 at 8192 x 8192 x 12 of 256): by the counters
+// matrix units busy 65% of the cycles (49 and 45%) at the 1.6 GHz that the card holds under it (1.9 and 2.0), no LDS bank conflicts, LDS
+// reads active in 32% (25 and 22), waves waiting 24% of theirs (28 and 34): what does not fall side by side in two waves a SIMD waits.
+// Over 512 keys, 2 x 8190 x 40 heads: 250 us with a key mask, 690 TFLOP/s, of which a workgroup's start, its queries' load and its
+// stores take 100, as they overlap with the other workgroup of the CU alone (LDS and registers hold two); 226 without a mask.
+// Numbers of keys that are no multiple of 32 cost a bool mask the loads of its last bytes, one by one: 77 keys 155 us, 96 keys 137.
 // 32 queries a wave: with 64 each key read from LDS served twice the products, but scores and results of both left no
 // registers to keep products and weights apart. Two teams of waves that take half the keys each were faster nowhere.
 //
