@@ -320,9 +320,9 @@ __device__ __forceinline__ float kLowest(float factor) {
 // column of scores, so maximum and sum run inside the lane, and the scores' registers, rounded to 16
 // bits, are the second product's operand as they stand. The order of the 16 keys of an MFMA
 // is free as long as both operands have it; V's is the one that the score layout leaves,
-// which the transposing LDS read delivers. (Rounded weights are what 16-bit products take; their sum has them unrounded. bf16 results
-// are off by 2.3e-3 in the 2-norm with that, and by 1.7e-3 from their own rounding alone.) The maximum is replaced (and the sums scaled) only where
-// a score exceeds it by more than 2^8: its value cancels in the result.
+// which the transposing LDS read delivers. (Rounded weights are what 16-bit products take; their sum has them unrounded. bf16
+// results are off by 2.3e-3 in the 2-norm with that, and by 1.7e-3 from their own rounding alone.) The maximum is replaced (and the
+// sums scaled) only where a score exceeds it by more than 2^8: its value cancels in the result.
 template <int kDim, bool kBf16, int kMask, int kKeyBlocks>
 struct AttnWave {
     static constexpr int kSteps = kDim / 16, kBlocks = kDim / 32, kRowBytes = kDim * 2;
